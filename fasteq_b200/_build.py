@@ -21,7 +21,8 @@ INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(PKG, "lib")
 JIT = os.path.join(LIB, "jit")
 CORE_SO = os.path.join(LIB, "libfasteq_b200_core.so")
-CORE_SOURCES = ["core.cu", "eqlinear.cu", "eqlinear_api.cu", "gemm_tf32x3.cu", "radial_chain.cu", "gate.cu", "neighbors.cu", "edge_geometry.cu", "silu.cu", "readout.cu"]
+CORE_SOURCES = ["core.cu", "eqlinear.cu", "eqlinear_api.cu", "gemm_tf32x3.cu", "radial_chain.cu", "gate.cu", "neighbors.cu", "edge_geometry.cu", "silu.cu", "readout.cu",
+                "product.cu", "expert_rows.cu"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-shared", "-diag-suppress", "177",
@@ -75,7 +76,7 @@ def build_core(force: bool = False) -> str:
 
 
 FRONT = os.path.join(CSRC, "front")
-FRONT_SOURCES = ["module.cpp", "prepared.cpp", "layers.cpp", "edges.cpp", "u1d.cpp"]
+FRONT_SOURCES = ["module.cpp", "prepared.cpp", "layers.cpp", "experts.cpp", "edges.cpp", "u1d.cpp"]
 _front_lock = threading.Lock()
 
 

@@ -1,0 +1,307 @@
+// Dense layers with an epilogue, one matrix for all rows or one per expert, and the rows' way into the experts' order and back.
+//
+// Without its epilogue the layer is bilinear: with  P(x, w) = x w^T,  D(g, w) = g w,  W(g, x) = g^T x  (each over an expert's rows) the gradients of any of
+// the three are the other two, so Product, ProductX and ProductW call one another and differentiate to every order.  The layer
+// itself is one launch forward (which leaves act'(z) for the gradients) and one per gradient; where its gradients are to be differentiated
+// it is taken apart into those and elementwise operations.
+#include "front.h"
+
+namespace front {
+namespace {
+
+enum Act : int64_t { kIdentity = 0, kSilu = 1, kTanh = 2, kSigmoid = 3, kAbs = 4 };
+
+// x [rows, K], w [experts, N, K]; offsets undefined: one matrix
+fasteq_product_problem problem(const Tensor& x, const Tensor& w, int64_t inner, int64_t act) {
+  fasteq_product_problem p{};
+  p.dtype = w.scalar_type() == at::kDouble ? FASTEQ_F64 : FASTEQ_F32;
+  p.experts = (int32_t)w.size(0); p.n = (int32_t)w.size(1); p.k = (int32_t)w.size(2);
+  p.inner = (int32_t)inner; p.act = (int32_t)act; p.rows = x.size(0);
+  return p;
+}
+const int32_t* offsets_of(const Tensor& offsets) { return offsets.defined() ? offsets.const_data_ptr<int32_t>() : nullptr; }
+
+Tensor run_forward(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& residual, const Tensor& offsets, int64_t inner, int64_t act,
+                   Tensor* slope) {
+  c10::cuda::CUDAGuard guard(x.device());
+  const Tensor xc = x.contiguous(), wc = w.contiguous(), bc = defined_contiguous(bias), rc = defined_contiguous(residual);
+  const auto p = problem(xc, wc, inner, act);
+  Tensor y = at::empty({xc.size(0), wc.size(1)}, xc.options());
+  if (slope) *slope = at::empty_like(y);
+  check(core.product_forward(&p, ptr(xc), ptr(wc), ptr(bc), ptr(rc), offsets_of(offsets), mptr(y), slope ? mptr(*slope) : nullptr, stream_of(xc)),
+        "fasteq_product_forward", core.last_cuda_error);
+  return y;
+}
+
+Tensor run_dgrad(const Tensor& g, const Tensor& slope, const Tensor& w, const Tensor& offsets, int64_t inner) {
+  c10::cuda::CUDAGuard guard(g.device());
+  const Tensor gc = g.contiguous(), wc = w.contiguous();
+  const auto p = problem(gc, wc, inner, 0);
+  Tensor gx = at::empty({gc.size(0), wc.size(2)}, gc.options());
+  check(core.product_dgrad(&p, ptr(gc), ptr(slope), ptr(wc), offsets_of(offsets), mptr(gx), stream_of(gc)), "fasteq_product_dgrad", core.last_cuda_error);
+  return gx;
+}
+
+// `shape`: the weights'
+Tensor run_wgrad(const Tensor& x, const Tensor& g, const Tensor& slope, const Tensor& offsets, int64_t inner, at::IntArrayRef shape, Tensor* grad_bias) {
+  c10::cuda::CUDAGuard guard(g.device());
+  const Tensor gc = g.contiguous(), xc = x.contiguous();
+  Tensor gw = at::empty(shape, gc.options());
+  const auto p = problem(xc, gw, inner, 0);
+  if (grad_bias) *grad_bias = at::empty({shape[0], shape[1]}, gc.options());
+  int64_t need = 0;
+  check(core.product_wgrad_scratch(&p, &need), "fasteq_product_wgrad_scratch", core.last_cuda_error);
+  Tensor scratch = at::empty({std::max<int64_t>(need, 16)}, gc.options().dtype(at::kByte));
+  check(core.product_wgrad(&p, ptr(xc), ptr(gc), ptr(slope), offsets_of(offsets), mptr(gw), grad_bias ? mptr(*grad_bias) : nullptr, scratch.data_ptr(),
+                           scratch.numel(), stream_of(gc)),
+        "fasteq_product_wgrad", core.last_cuda_error);
+  return gw;
+}
+
+Tensor product(const Tensor& x, const Tensor& w, const Tensor& offsets, int64_t inner);
+Tensor product_x(const Tensor& g, const Tensor& w, const Tensor& offsets, int64_t inner);
+Tensor product_w(const Tensor& g, const Tensor& x, const Tensor& offsets, int64_t inner, at::IntArrayRef shape);
+
+// P(x, w), D(g, w), W(g, x) as nodes; which = 0, 1, 2
+struct Bilinear : torch::autograd::Function<Bilinear> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& a, const Tensor& b, const std::optional<Tensor>& offsets, int64_t inner, int64_t which,
+                        std::vector<int64_t> shape) {
+    ctx->save_for_backward({a, b, offsets.value_or(Tensor())});
+    ctx->saved_data["i"] = inner; ctx->saved_data["w"] = which;
+    const Tensor o = offsets.value_or(Tensor());
+    if (which == 0) return run_forward(a, b, Tensor(), Tensor(), o, inner, kIdentity, nullptr);
+    if (which == 1) return run_dgrad(a, Tensor(), b, o, inner);
+    return run_wgrad(b, a, Tensor(), o, inner, shape, nullptr);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list go) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &a = saved[0], &b = saved[1], &o = saved[2], &h = go[0];
+    const int64_t inner = ctx->saved_data["i"].toInt(), which = ctx->saved_data["w"].toInt();
+    const bool need_a = ctx->needs_input_grad(0), need_b = ctx->needs_input_grad(1);
+    Tensor da, db;
+    if (which == 0) {                      // x, w
+      if (need_a) da = product_x(h, b, o, inner);
+      if (need_b) db = product_w(h, a, o, inner, b.sizes());
+    } else if (which == 1) {               // g, w; h like x
+      if (need_a) da = product(h, b, o, inner);
+      if (need_b) db = product_w(a, h, o, inner, b.sizes());
+    } else {                               // g, x; h like w
+      if (need_a) da = product(b, h, o, inner);
+      if (need_b) db = product_x(a, h, o, inner);
+    }
+    return {da, db, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+std::optional<Tensor> optional_of(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
+Tensor product(const Tensor& x, const Tensor& w, const Tensor& offsets, int64_t inner) { return Bilinear::apply(x, w, optional_of(offsets), inner, (int64_t)0, std::vector<int64_t>()); }
+Tensor product_x(const Tensor& g, const Tensor& w, const Tensor& offsets, int64_t inner) { return Bilinear::apply(g, w, optional_of(offsets), inner, (int64_t)1, std::vector<int64_t>()); }
+Tensor product_w(const Tensor& g, const Tensor& x, const Tensor& offsets, int64_t inner, at::IntArrayRef shape) {
+  return Bilinear::apply(g, x, optional_of(offsets), inner, (int64_t)2, shape.vec());
+}
+
+// The layer.  x [rows, K], w [experts, N, K], bias [experts, N], residual [rows, N]
+struct Layer : torch::autograd::Function<Layer> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const std::optional<Tensor>& bias, const std::optional<Tensor>& residual,
+                        const std::optional<Tensor>& offsets, int64_t inner, int64_t act, bool differentiated) {
+    const Tensor b = bias.value_or(Tensor()), o = offsets.value_or(Tensor());
+    Tensor slope;
+    Tensor y = run_forward(x, w, b, residual.value_or(Tensor()), o, inner, act, differentiated && act != kIdentity ? &slope : nullptr);
+    ctx->save_for_backward({x, w, b, o, slope});
+    ctx->saved_data["i"] = inner; ctx->saved_data["a"] = act; ctx->saved_data["r"] = residual.has_value();
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list go) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &w = saved[1], &b = saved[2], &o = saved[3], &slope = saved[4], &g = go[0];
+    const int64_t inner = ctx->saved_data["i"].toInt(), act = ctx->saved_data["a"].toInt();
+    // the context numbers the tensors it was given, not the places they could have had
+    const bool has_b = b.defined(), has_r = ctx->saved_data["r"].toBool();
+    const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = has_b && ctx->needs_input_grad(2);
+    Tensor gx, gw, gb;
+    const Tensor gr = has_r && ctx->needs_input_grad(has_b ? 3 : 2) ? g : Tensor();
+    if (at::GradMode::is_enabled()) {
+      // to be differentiated again.  The bias and its gradient are products with a column of ones, which stay inside the experts' rows
+      const Tensor ones = b.defined() ? at::ones({x.size(0), 1}, x.options()) : Tensor();
+      Tensor gz = g;
+      if (act != kIdentity) {
+        Tensor z = product(x, w, o, inner);
+        if (b.defined()) z = z + product(ones, b.unsqueeze(2), o, inner);
+        if (act == kSilu) gz = silu_gradient(g.contiguous(), z.contiguous());
+        else if (act == kTanh) gz = g * (1 - at::tanh(z).square());
+        else if (act == kSigmoid) { const Tensor s = at::sigmoid(z); gz = g * (s * (1 - s)); }
+        else gz = g * at::sgn(z).detach();
+      }
+      if (need_x) gx = product_x(gz, w, o, inner);
+      if (need_w) gw = product_w(gz, x, o, inner, w.sizes());
+      if (need_b) gb = product_w(gz, ones, o, inner, {b.size(0), b.size(1), 1}).squeeze(2);
+    } else {
+      if (need_x) gx = run_dgrad(g, slope, w, o, inner);
+      if (need_w || need_b) {
+        gw = run_wgrad(x, g, slope, o, inner, w.sizes(), need_b ? &gb : nullptr);
+        if (!need_w) gw = Tensor();
+      }
+    }
+    return {gx, gw, gb, gr, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// Checked by the callers in Python.  Rows of the last dimension; the result has x's leading extents.
+Tensor layer(const Tensor& x, const Tensor& w, const std::optional<Tensor>& bias, const std::optional<Tensor>& residual, const std::optional<Tensor>& offsets,
+             int64_t inner, int64_t act) {
+  std::vector<int64_t> shape = x.sizes().vec();
+  shape.back() = w.size(-2);
+  const int64_t K = w.size(-1), N = w.size(-2), rows = c10::multiply_integers(x.sizes().begin(), x.sizes().end() - 1);
+  const Tensor w3 = w.dim() == 2 ? w.unsqueeze(0) : w;
+  std::optional<Tensor> b2 = bias, r2 = residual;
+  if (b2 && b2->dim() == 1) b2 = b2->unsqueeze(0);
+  if (r2) r2 = r2->reshape({rows, N});
+  auto grad = [](const std::optional<Tensor>& t) { return t && t->requires_grad(); };
+  const bool differentiated = at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || grad(bias));
+  const Tensor x2 = x.reshape({rows, K});
+  return Layer::apply(x2, w3, b2, r2, offsets, inner, act, differentiated).reshape(shape);
+}
+
+// ------------------------------------------------------------------------------------------------ experts' order
+struct Order : torch::CustomClassHolder {
+  Tensor position, offsets;              // [tokens, slots] and [experts + 1], int32
+  int64_t experts, slots;
+  Order(Tensor p, Tensor o) : position(std::move(p)), offsets(std::move(o)), experts(offsets.size(0) - 1), slots(position.size(1)) {}
+};
+using OrderPtr = c10::intrusive_ptr<Order>;
+
+int32_t dtype_of(const Tensor& t) { return t.scalar_type() == at::kDouble ? FASTEQ_F64 : FASTEQ_F32; }
+int64_t width_of(const Tensor& t) { return c10::multiply_integers(t.sizes().begin() + 1, t.sizes().end()); }
+std::vector<int64_t> with_rows(const Tensor& t, int64_t rows) {
+  std::vector<int64_t> s = t.sizes().vec();
+  s[0] = rows;
+  return s;
+}
+
+Tensor run_gather(const Tensor& x, const Order& o) {
+  c10::cuda::CUDAGuard guard(x.device());
+  const Tensor xc = x.contiguous();
+  Tensor rows = at::empty(with_rows(x, x.size(0) * o.slots), xc.options());
+  check(core.expert_gather(dtype_of(xc), ptr(xc), o.position.const_data_ptr<int32_t>(), o.offsets.const_data_ptr<int32_t>(), (int32_t)o.experts, xc.size(0),
+                           (int32_t)o.slots, (int32_t)width_of(xc), mptr(rows), stream_of(xc)),
+        "fasteq_expert_gather", core.last_cuda_error);
+  return rows;
+}
+Tensor run_combine(const Tensor& rows, const Tensor& weight, const Order& o) {
+  c10::cuda::CUDAGuard guard(rows.device());
+  const Tensor rc = rows.contiguous(), wc = defined_contiguous(weight);
+  const int64_t tokens = o.position.size(0);
+  Tensor y = at::empty(with_rows(rows, tokens), rc.options());
+  check(core.expert_combine(dtype_of(rc), ptr(rc), ptr(wc), o.position.const_data_ptr<int32_t>(), o.offsets.const_data_ptr<int32_t>(), (int32_t)o.experts, tokens,
+                            (int32_t)o.slots, (int32_t)width_of(rc), mptr(y), stream_of(rc)),
+        "fasteq_expert_combine", core.last_cuda_error);
+  return y;
+}
+variable_list run_combine_backward(const Tensor& rows, const Tensor& weight, const Tensor& g, const Order& o, bool need_rows, bool need_weight) {
+  c10::cuda::CUDAGuard guard(rows.device());
+  const Tensor rc = rows.contiguous(), wc = defined_contiguous(weight), gc = g.contiguous();
+  Tensor gr = need_rows ? at::empty_like(rc) : Tensor(), gw = need_weight ? at::empty(o.position.sizes(), rc.options()) : Tensor();
+  check(core.expert_combine_backward(dtype_of(rc), ptr(rc), ptr(wc), ptr(gc), o.position.const_data_ptr<int32_t>(), o.offsets.const_data_ptr<int32_t>(),
+                                     (int32_t)o.experts, o.position.size(0), (int32_t)o.slots, (int32_t)width_of(rc), mptr(gr), mptr(gw), stream_of(rc)),
+        "fasteq_expert_combine_backward", core.last_cuda_error);
+  return {gr, gw};
+}
+
+Tensor combine(const Tensor& rows, const std::optional<Tensor>& weight, const OrderPtr& o);
+
+struct Gather : torch::autograd::Function<Gather> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const OrderPtr& o) {
+    ctx->saved_data["o"] = capsule(o);
+    return run_gather(x, *o);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list go) {
+    return {combine(go[0], std::nullopt, uncapsule<Order>(ctx->saved_data["o"])), Tensor()};
+  }
+};
+
+// <rows[position[t, s]], g[t]>: bilinear as well
+struct Dots : torch::autograd::Function<Dots> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Tensor& g, const OrderPtr& o) {
+    ctx->save_for_backward({rows, g});
+    ctx->saved_data["o"] = capsule(o);
+    return run_combine_backward(rows, Tensor(), g, *o, false, true)[1];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list go);
+};
+
+// rows w[t, s] g[t], 0 for no expert
+struct Spread : torch::autograd::Function<Spread> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& g, const OrderPtr& o) {
+    ctx->save_for_backward({weight, g});
+    ctx->saved_data["o"] = capsule(o);
+    c10::cuda::CUDAGuard guard(g.device());
+    const Tensor wc = weight.contiguous(), gc = g.contiguous();
+    Tensor rows = at::empty(with_rows(g, o->position.numel()), gc.options());
+    check(core.expert_combine_backward(dtype_of(gc), ptr(gc), ptr(wc), ptr(gc), o->position.const_data_ptr<int32_t>(), o->offsets.const_data_ptr<int32_t>(),
+                                       (int32_t)o->experts, o->position.size(0), (int32_t)o->slots, (int32_t)width_of(gc), mptr(rows), nullptr, stream_of(gc)),
+          "fasteq_expert_combine_backward", core.last_cuda_error);
+    return rows;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list go);
+};
+
+struct Combine : torch::autograd::Function<Combine> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& rows, const std::optional<Tensor>& weight, const OrderPtr& o) {
+    ctx->save_for_backward(weight ? variable_list{rows, *weight} : variable_list{});
+    ctx->saved_data["o"] = capsule(o);
+    return run_combine(rows, weight.value_or(Tensor()), *o);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list go) {
+    const OrderPtr o = uncapsule<Order>(ctx->saved_data["o"]);
+    const auto saved = ctx->get_saved_variables();
+    const bool need_rows = ctx->needs_input_grad(0);
+    if (saved.empty()) return {need_rows ? Tensor(Gather::apply(go[0], o)) : Tensor(), Tensor(), Tensor()};
+    const Tensor &rows = saved[0], &weight = saved[1];
+    const bool need_weight = ctx->needs_input_grad(1);
+    if (at::GradMode::is_enabled())
+      return {need_rows ? Tensor(Spread::apply(weight, go[0], o)) : Tensor(), need_weight ? Tensor(Dots::apply(rows, go[0], o)) : Tensor(), Tensor()};
+    auto d = run_combine_backward(rows, weight, go[0], *o, need_rows, need_weight);
+    return {d[0], d[1], Tensor()};
+  }
+};
+Tensor combine(const Tensor& rows, const std::optional<Tensor>& weight, const OrderPtr& o) { return Combine::apply(rows, weight, o); }
+
+variable_list Dots::backward(AutogradContext* ctx, variable_list go) {
+  const auto saved = ctx->get_saved_variables();
+  const OrderPtr o = uncapsule<Order>(ctx->saved_data["o"]);
+  return {ctx->needs_input_grad(0) ? Tensor(Spread::apply(go[0], saved[1], o)) : Tensor(),
+          ctx->needs_input_grad(1) ? combine(saved[0], go[0], o) : Tensor(), Tensor()};
+}
+variable_list Spread::backward(AutogradContext* ctx, variable_list go) {
+  const auto saved = ctx->get_saved_variables();
+  const OrderPtr o = uncapsule<Order>(ctx->saved_data["o"]);
+  return {ctx->needs_input_grad(0) ? Tensor(Dots::apply(go[0], saved[1], o)) : Tensor(),
+          ctx->needs_input_grad(1) ? combine(go[0], saved[0], o) : Tensor(), Tensor()};
+}
+
+// expert [tokens, slots], int32 or int64, contiguous
+OrderPtr make_order(const Tensor& expert, int64_t experts) {
+  c10::cuda::CUDAGuard guard(expert.device());
+  const auto ints = expert.options().dtype(at::kInt);
+  Tensor position = at::empty(expert.sizes(), ints), offsets = at::empty({experts + 1}, ints);
+  int64_t need = 0;
+  check(core.expert_plan_scratch(expert.numel(), (int32_t)experts, &need), "fasteq_expert_plan_scratch", core.last_cuda_error);
+  Tensor scratch = need ? at::empty({need}, expert.options().dtype(at::kByte)) : Tensor();
+  check(core.expert_plan(ptr(expert), (int32_t)expert.element_size(), expert.numel(), (int32_t)experts, position.data_ptr<int32_t>(), offsets.data_ptr<int32_t>(),
+                         mptr(scratch), stream_of(expert)),
+        "fasteq_expert_plan", core.last_cuda_error);
+  return c10::make_intrusive<Order>(position, offsets);
+}
+
+}  // namespace
+
+void bind_experts(py::module_& m) {
+  py::class_<Order, OrderPtr>(m, "ExpertOrder")
+      .def_readonly("position", &Order::position)
+      .def_readonly("offsets", &Order::offsets);
+  m.def("product_layer", &layer, py::arg("x"), py::arg("w"), py::arg("bias"), py::arg("residual"), py::arg("offsets"), py::arg("inner"), py::arg("act"));
+  m.def("expert_order", &make_order);
+  m.def("expert_gather", [](const Tensor& x, const OrderPtr& o) -> Tensor { return Gather::apply(x, o); });
+  m.def("expert_combine", [](const Tensor& rows, const std::optional<Tensor>& weight, const OrderPtr& o) -> Tensor { return combine(rows, weight, o); });
+}
+
+}  // namespace front

@@ -33,7 +33,8 @@ struct Core {
   F(eqlinear_pack) F(eqlinear_forward) F(eqlinear_dgrad) F(eqlinear_forward_packed) F(eqlinear_dgrad_packed)
   F(eqlinear_wgrad_scratch) F(eqlinear_wgrad_with) F(gemm_tf32x3_split) F(gemm_tf32x3_presplit)
   F(radial_chain_prepare) F(radial_chain_forward) F(radial_chain_backward) F(edge_geometry_forward) F(edge_geometry_backward)
-  F(silu) F(neighbors_work_bytes) F(neighbors_count) F(neighbors_fill) F(graph_partition) F(graph_partition_edges) F(last_cuda_error)
+  F(product_forward) F(product_dgrad) F(product_wgrad_scratch) F(product_wgrad) F(expert_plan_scratch) F(expert_plan) F(expert_gather) F(expert_combine)
+  F(expert_combine_backward) F(silu) F(neighbors_work_bytes) F(neighbors_count) F(neighbors_fill) F(graph_partition) F(graph_partition_edges) F(last_cuda_error)
 #undef F
 };
 extern Core core;
@@ -65,6 +66,9 @@ inline void* mptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr
 // Prepared (split / packed) forms of weights, see prepared.cpp
 std::optional<Tensor> prepared(const std::vector<Tensor>& weights, const std::string& tag, const std::function<Tensor()>& build);
 
+// g silu'(z), differentiable (layers.cpp)
+Tensor silu_gradient(const Tensor& g, const Tensor& z);
+
 // keeps a C++ object in an autograd node
 template <typename T> c10::IValue capsule(const c10::intrusive_ptr<T>& p) { return c10::IValue::make_capsule(p); }
 template <typename T> c10::intrusive_ptr<T> uncapsule(const c10::IValue& v) {
@@ -73,6 +77,7 @@ template <typename T> c10::intrusive_ptr<T> uncapsule(const c10::IValue& v) {
 
 void bind_prepared(py::module_& m);
 void bind_layers(py::module_& m);
+void bind_experts(py::module_& m);
 void bind_edges(py::module_& m);
 void bind_u1d(py::module_& m);
 

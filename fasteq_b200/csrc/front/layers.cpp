@@ -370,6 +370,8 @@ struct RadialChain : torch::autograd::Function<RadialChain> {
 
 }  // namespace
 
+Tensor silu_gradient(const Tensor& g, const Tensor& z) { return SiLUBackward::apply(g, z); }
+
 void bind_layers(py::module_& m) {
   py::class_<Geometry, Geom>(m, "Geometry")
       .def(py::init([](std::vector<std::array<int64_t, 4>> mapping, std::vector<double> coeff, int u, int v, int I, int J, py::object wgrad) {

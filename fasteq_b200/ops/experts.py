@@ -1,0 +1,106 @@
+"""Experts: a node (or any row) is given to one or several of a set of matrices, as ``fast_fctp`` gives it to its species' one.
+
+    plan = expert_plan(expert, num_experts)                       # who goes where: [tokens, slots] expert numbers, -1: to none
+    rows = expert_gather(x, plan)                                 # [tokens, ...] -> [tokens * slots, ...] in the experts' order
+    rows = expert_dense(rows, w1, plan, bias=b1, activation="silu")      # one launch for all experts, w1 [experts, N, K]
+    rows = expert_dense(rows, w2, plan, bias=b2)
+    y = expert_combine(rows, plan, weight)                        # [tokens, ...] = sum over slots of weight * row
+
+Everything stays on the device: the plan's offsets are read by the kernels, so the host waits for nothing and a step can be captured
+in a CUDA graph.  Sums run over slots and rows in a fixed order (no atomics): the same inputs give the same bits.  Entries given to no
+expert lie behind the experts' rows as zeros and take part in no sum and no gradient.  The weights are scalars of a row, so rows may hold
+components of irreps; ``expert_dense`` mixes channels, its rows' components ``[rows, components, K]`` share their expert's matrix.
+Float32 and float64, differentiable to every order.  CUDA tensors only.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional
+
+import torch
+
+from .. import _cabi, _front
+from .dense_act import act_code, check_operands
+
+__all__ = ["ExpertPlan", "expert_plan", "expert_gather", "expert_dense", "expert_combine", "expert_device_status"]
+
+MAX_EXPERTS = 1024
+
+
+class ExpertPlan:
+    """Order of the entries ``(token, slot)`` by expert.  ``position [tokens, slots]``: the entry's row; ``offsets [num_experts + 1]``: expert
+    ``e`` has rows ``offsets[e]`` to ``offsets[e + 1]``, those from ``offsets[-1]`` on have none (both int32, on the device)."""
+
+    def __init__(self, native):
+        self._native = native
+        self.position, self.offsets = native.position, native.offsets
+        self.tokens, self.slots = self.position.shape
+        self.rows, self.num_experts = self.tokens * self.slots, self.offsets.shape[0] - 1
+
+
+def expert_device_status() -> int:
+    """Reads and clears the status word of the plans (synchronises): 0, or 2 = an expert number was not below ``num_experts``."""
+    lib, v = _cabi.core(), C.c_int32(0)
+    _cabi.check(lib.fasteq_expert_device_status(C.byref(v)), lib, "fasteq_expert_device_status")
+    return int(v.value)
+
+
+def expert_plan(expert: torch.Tensor, num_experts: int) -> ExpertPlan:
+    """``expert [tokens, slots]`` (or ``[tokens]``: one slot), int32 or int64.  Negative numbers mean no expert; numbers from ``num_experts``
+    on are treated like them and reported by ``fasteq_b200.status.device_status``."""
+    if not expert.is_cuda:
+        raise RuntimeError("expert_plan: expert must be a CUDA tensor: fasteq_b200 has no CPU path")
+    if expert.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"expert_plan: expert must be int32 or int64, got {expert.dtype}")
+    if expert.dim() not in (1, 2) or (expert.dim() == 2 and expert.shape[1] < 1):
+        raise ValueError(f"expert_plan: expert must be [tokens] or [tokens, slots] with a slot at least, got {tuple(expert.shape)}")
+    if not 1 <= num_experts <= MAX_EXPERTS:
+        raise ValueError(f"expert_plan: 1 to {MAX_EXPERTS} experts are supported, got {num_experts}")
+    e = expert.unsqueeze(1) if expert.dim() == 1 else expert
+    return ExpertPlan(_front.lib().expert_order(e.contiguous(), int(num_experts)))
+
+
+def _check_rows(name: str, what: str, t: torch.Tensor, rows: int, plan: ExpertPlan) -> None:
+    if not isinstance(plan, ExpertPlan):
+        raise TypeError(f"{name}: plan must be an ExpertPlan, got {type(plan).__name__}")
+    if t.dim() < 1 or t.shape[0] != rows:
+        raise ValueError(f"{name}: {what} must have {rows} rows, got {tuple(t.shape)}")
+    if t.device != plan.offsets.device:
+        raise ValueError(f"{name}: {what} is on {t.device}, the plan on {plan.offsets.device}")
+
+
+def expert_gather(x: torch.Tensor, plan: ExpertPlan) -> torch.Tensor:
+    """``x [tokens, ...]`` to ``[tokens * slots, ...]`` in the experts' order (zeros for entries of no expert)."""
+    check_operands("expert_gather", x=x)
+    _check_rows("expert_gather", "x", x, plan.tokens if isinstance(plan, ExpertPlan) else -1, plan)
+    return _front.lib().expert_gather(x, plan._native)
+
+
+def expert_combine(rows: torch.Tensor, plan: ExpertPlan, weight: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``y[t] = sum_s weight[t, s] * rows[position[t, s]]``: ``rows [tokens * slots, ...]`` in the experts' order, ``weight [tokens, slots]``
+    (``[tokens]`` with one slot; ``None``: ones)."""
+    check_operands("expert_combine", rows=rows, weight=weight)
+    _check_rows("expert_combine", "rows", rows, plan.rows if isinstance(plan, ExpertPlan) else -1, plan)
+    if weight is not None:
+        if weight.dim() == 1 and plan.slots == 1:
+            weight = weight.unsqueeze(1)
+        if weight.shape != plan.position.shape:
+            raise ValueError(f"expert_combine: weight must be {tuple(plan.position.shape)}, got {tuple(weight.shape)}")
+    return _front.lib().expert_combine(rows, weight, plan._native)
+
+
+def expert_dense(rows: torch.Tensor, weight: torch.Tensor, plan: ExpertPlan, bias: Optional[torch.Tensor] = None,
+                 activation: Optional[str] = None) -> torch.Tensor:
+    """``act(rows[r] @ weight[e(r)].T + bias[e(r)])`` for rows in the experts' order, ``[tokens * slots, ..., K]``; ``weight [num_experts, N, K]``,
+    ``bias [num_experts, N]``, activations as in ``dense_act``.  Rows of no expert come out as zeros."""
+    code = act_code("expert_dense", activation)
+    check_operands("expert_dense", rows=rows, weight=weight, bias=bias)
+    _check_rows("expert_dense", "rows", rows, plan.rows if isinstance(plan, ExpertPlan) else -1, plan)
+    if rows.dim() < 2 or weight.dim() != 3 or weight.shape[0] != plan.num_experts or weight.shape[2] != rows.shape[-1]:
+        raise ValueError(f"expert_dense: rows [rows, ..., K] and weight [{plan.num_experts}, N, K] expected, got {tuple(rows.shape)} and {tuple(weight.shape)}")
+    if bias is not None and bias.shape != weight.shape[:2]:
+        raise ValueError(f"expert_dense: bias must be {tuple(weight.shape[:2])}, got {tuple(bias.shape)}")
+    inner = 1
+    for n in rows.shape[1:-1]:
+        inner *= n
+    return _front.lib().product_layer(rows, weight, bias, None, plan.offsets, max(inner, 1), code)

@@ -3,7 +3,7 @@
 Every kernel with a bounded wait or an index check records why it gave up or what it skipped in a status word
 instead of trapping (wait timed out, index outside its operand); results of that launch are then not to be used.
 The words live per generated module (tensor product, symmetric contraction) and per family in the core library
-(tcgen05 GEMMs and the radial chain, edge geometry).  Reading synchronises the device."""
+(tcgen05 GEMMs and the radial chain, edge geometry, experts).  Reading synchronises the device."""
 from __future__ import annotations
 
 from typing import Dict
@@ -20,6 +20,7 @@ def device_status() -> Dict[str, int]:
     from .ops import stc_uniform1d_jit as stc
     from .ops.dense import tensorcore_device_status
     from .ops.edge_geometry import edge_geometry_device_status
+    from .ops.experts import expert_device_status
     with u1d._lock:
         mods = list(u1d._MODULES.items())
     for (spec, direction, needs, tun), mod in mods:
@@ -30,7 +31,8 @@ def device_status() -> Dict[str, int]:
         code = mod.device_status()
         if code:
             out[f"stc {key[1:]}"] = code
-    for name, fn in (("tcgen05 gemm / radial chain", tensorcore_device_status), ("edge geometry", edge_geometry_device_status)):
+    for name, fn in (("tcgen05 gemm / radial chain", tensorcore_device_status), ("edge geometry", edge_geometry_device_status),
+                     ("experts", expert_device_status)):
         code = fn()
         if code:
             out[name] = code

@@ -435,6 +435,60 @@ int fasteq_readout_forward(int32_t dtype, const void* h, const void* w, const vo
 int fasteq_readout_backward(int32_t dtype, const void* g, const void* w, void* gh, int64_t n, int32_t c_count, int64_t d,
                             fasteq_stream_t stream);
 
+/* ------------------------------------------------------------------------- *
+ * Dense layers with an epilogue, one matrix for all rows or one per expert:
+ *   z[r, :] = x[r, :] W[e(r)]^T + bias[e(r)],   y[r, :] = act(z[r, :]) + residual[r, :],   x [rows, k], W [experts, n, k] (row-major)
+ * Without `offsets` (NULL) there is one matrix.  With them the rows are in the experts' order: entry i owns rows [i * inner, (i + 1) * inner),
+ * expert e the entries [offsets[e], offsets[e + 1]) (device [experts + 1], as fasteq_expert_plan writes them, read on the device: no host
+ * synchronisation), and rows behind offsets[experts] are written as zeros and take part in nothing.
+ * act: the codes of the gate (0 identity, 1 silu, 2 tanh, 3 sigmoid, 4 abs).  `slope` [rows, n] (forward, may be NULL) receives act'(z), which
+ * the gradients take (NULL where act is the identity): with gz = grad_y * slope
+ *   grad_x = gz W[e],   grad_w[e] = sum_{r of e} gz[r]^T x[r],   grad_bias[e] = sum_{r of e} gz[r].
+ * FP32 data: products of three bf16 parts per operand on the tensor cores, accumulated in FP32 (the accuracy of FP32 products), FP32 FMAs
+ * where those do not pay; FP64: FP64 throughout.  Sums are formed in a fixed order.  Any extents, any 4- / 8-byte aligned addresses.
+ * The reference leaves such layers to the model package.
+ * ------------------------------------------------------------------------- */
+#define FASTEQ_MAX_EXPERTS 1024
+typedef struct fasteq_product_problem {
+  int32_t dtype;                /* fasteq_dtype */
+  int32_t k, n;                 /* channels in and out */
+  int32_t experts, inner;       /* 1 .. FASTEQ_MAX_EXPERTS; rows of an entry */
+  int32_t act;
+  int64_t rows;
+} fasteq_product_problem;
+int fasteq_product_forward(const fasteq_product_problem* p /* host */, const void* x, const void* w, const void* bias /* or NULL */,
+                           const void* residual /* or NULL */, const int32_t* offsets /* or NULL */, void* y, void* slope /* or NULL */,
+                           fasteq_stream_t stream);
+int fasteq_product_dgrad(const fasteq_product_problem* p /* host */, const void* grad_y, const void* slope /* or NULL */, const void* w,
+                         const int32_t* offsets /* or NULL */, void* grad_x, fasteq_stream_t stream);
+/* Weight and bias gradient (grad_bias may be NULL).  scratch: 16-byte aligned device memory of the bytes `_scratch` names, not in use by other
+ * work on the device meanwhile. */
+int fasteq_product_wgrad_scratch(const fasteq_product_problem* p /* host */, int64_t* bytes /* host */);
+int fasteq_product_wgrad(const fasteq_product_problem* p /* host */, const void* x, const void* grad_y, const void* slope /* or NULL */,
+                         const int32_t* offsets /* or NULL */, void* grad_w, void* grad_bias /* or NULL */, void* scratch, int64_t scratch_bytes,
+                         fasteq_stream_t stream);
+
+/* Rows in the order of the experts they are given to, and back.  Entry i = token * slots + slot is given to expert[i] (index_bytes 4 or 8;
+ * negative: to none; >= experts: to none, and the status word below reads 2).  position[i]: the entry's row in a stable order by expert, entries of no
+ * expert last; offsets[e], e = 0 .. experts: the first row of expert e.  At most 1024 experts.  scratch: as `_scratch` says.
+ *   gather            rows[position[t, s], :] = x[t, :]   (zeros for no expert)
+ *   combine           y[t, :] = sum_s weight[t, s] rows[position[t, s], :]   (weight NULL: 1; entries of no expert count nothing)
+ *   combine_backward  grad_rows[position[t, s], :] = weight[t, s] grad_y[t, :],  grad_weight[t, s] = <rows[position[t, s], :], grad_y[t, :]>
+ *                     (zeros for no expert; either output may be NULL, weight too where grad_rows is)
+ * The reference groups nodes by species on the host (fasteq/ops/fctp.py:643-736). */
+int fasteq_expert_plan_scratch(int64_t entries, int32_t experts, int64_t* bytes /* host */);
+int fasteq_expert_plan(const void* expert, int32_t index_bytes, int64_t entries, int32_t experts, int32_t* position, int32_t* offsets,
+                       void* scratch, fasteq_stream_t stream);
+int fasteq_expert_gather(int32_t dtype, const void* x, const int32_t* position, const int32_t* offsets, int32_t experts, int64_t tokens,
+                         int32_t slots, int32_t width, void* rows, fasteq_stream_t stream);
+int fasteq_expert_combine(int32_t dtype, const void* rows, const void* weight /* or NULL */, const int32_t* position, const int32_t* offsets,
+                          int32_t experts, int64_t tokens, int32_t slots, int32_t width, void* y, fasteq_stream_t stream);
+int fasteq_expert_combine_backward(int32_t dtype, const void* rows, const void* weight, const void* grad_y, const int32_t* position,
+                                   const int32_t* offsets, int32_t experts, int64_t tokens, int32_t slots, int32_t width,
+                                   void* grad_rows /* or NULL */, void* grad_weight /* or NULL */, fasteq_stream_t stream);
+/* Reads and clears the status word of the expert order (synchronises): 0, or 2 = an expert number was out of range. */
+int fasteq_expert_device_status(int32_t* code /* host */);
+
 #ifdef __cplusplus
 }
 #endif
