@@ -178,7 +178,7 @@ def _own_route(s):
     plan = expert_plan(s["expert"], s["case"]["experts"])
     rows = expert_gather(s["x"], plan)
     y = expert_combine(s["y"], plan, s["weight"])
-    out = dict(offsets=plan.offsets, position=plan.position, rows=rows.detach(), out=y.detach())
+    out = dict(offsets=plan.offsets, position=plan.position.reshape(-1), rows=rows.detach(), out=y.detach())
     if s["case"]["grad"]:
         grads = torch.autograd.grad([rows, y], [s[n] for n in s["leaves"]], [s["grows"], s["g"]])
         out.update(zip(("g" + n for n in s["leaves"]), grads))
