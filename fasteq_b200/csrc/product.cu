@@ -9,6 +9,8 @@
 #include "fasteq_device.cuh"
 #include "launch.cuh"
 #include "product.cuh"
+#include "product_tc.cuh"
+#include "gemm_tf32x3.h"
 
 using namespace fasteq;
 using namespace fasteq::product;
@@ -201,11 +203,68 @@ int wgrad(const fasteq_product_problem* p, const void* x, const void* g, const v
 
 }  // namespace
 
+namespace {
+
+bool wide(int extent, std::initializer_list<const void*> pointers) {
+  uintptr_t all = 0;
+  for (const void* q : pointers) all |= reinterpret_cast<uintptr_t>(q);
+  return extent % 4 == 0 && (all & 15u) == 0;
+}
+
+// Units of the tensor-core kernel (at most), which counts them, and a CTA's blocks, in 32 bits.
+long long most_units(const fasteq_product_problem* p, int K, int N) {
+  const long long units = (p->rows / ptc::BM + p->experts) * ((N + ptc::BN - 1) / ptc::BN);
+  return units > 0x7fffffffLL || (units / 64 + 1) * ((K + ptc::KB - 1) / ptc::KB) > 0x3fffffffLL ? -1 : units;
+}
+
+template <bool FORWARD, bool SLOPE, int ACT>
+int launch_tc(const fasteq_product_problem* p, ptc::Args& a, int sms, const CUtensorMap& tmA, const CUtensorMap& tmSlope, cudaStream_t s) {
+  const int smem = ptc::Cfg<SLOPE>::smem(p->experts);
+  cudaError_t e = cudaFuncSetAttribute(ptc::product_tc_kernel<FORWARD, SLOPE, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess)
+    e = launch_dependent(ptc::product_tc_kernel<FORWARD, SLOPE, ACT>, (unsigned)std::min<long long>(sms, most_units(p, a.K, a.N)), ptc::NT, smem, s, a, tmA, tmSlope);
+  return e == cudaSuccess ? FASTEQ_OK : cuda_fail(e);
+}
+
+// K and N as the kernel sees them (grad_x: exchanged)
+template <bool FORWARD>
+int run_tc(const fasteq_product_problem* p, const void* A, const void* slope, const void* W, const void* bias, const void* residual,
+           const int32_t* offsets, void* C, void* slope_out, cudaStream_t s) {
+  ptc::Args a{};
+  a.groups = groups_of(p, offsets);
+  a.A = (const float*)A; a.slope = (const float*)slope; a.W = (const float*)W; a.bias = (const float*)bias; a.residual = (const float*)residual;
+  a.C = (float*)C; a.slope_out = (float*)slope_out;
+  a.K = FORWARD ? p->k : p->n; a.N = FORWARD ? p->n : p->k;
+  a.a_wide = wide(a.K, {A, slope}) && p->rows <= 0x7fffffffLL; a.w_wide = wide(p->k, {W}); a.c_wide = wide(a.N, {C, slope_out, bias, residual});
+  int sms = 0, dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e == cudaSuccess) e = tc::status_word(&a.status);
+  if (e != cudaSuccess) return cuda_fail(e);
+  CUtensorMap tmA{}, tmSlope{};
+  if (a.a_wide) {
+    int rc = tc::make_map(&tmA, a.A, (uint64_t)a.K, 1, (uint64_t)p->rows, (uint64_t)a.K, (uint64_t)a.K, ptc::KB, 1, ptc::BM);
+    if (rc == FASTEQ_OK && slope) rc = tc::make_map(&tmSlope, a.slope, (uint64_t)a.K, 1, (uint64_t)p->rows, (uint64_t)a.K, (uint64_t)a.K, ptc::KB, 1, ptc::BM);
+    if (rc != FASTEQ_OK) return rc;
+  }
+  if (!FORWARD) return slope ? launch_tc<false, true, kIdentity>(p, a, sms, tmA, tmSlope, s) : launch_tc<false, false, kIdentity>(p, a, sms, tmA, tmSlope, s);
+  switch (p->act) {
+    case kSilu: return launch_tc<true, false, kSilu>(p, a, sms, tmA, tmSlope, s);
+    case kTanh: return launch_tc<true, false, kTanh>(p, a, sms, tmA, tmSlope, s);
+    case kSigmoid: return launch_tc<true, false, kSigmoid>(p, a, sms, tmA, tmSlope, s);
+    case kAbs: return launch_tc<true, false, kAbs>(p, a, sms, tmA, tmSlope, s);
+    default: return launch_tc<true, false, kIdentity>(p, a, sms, tmA, tmSlope, s);
+  }
+}
+
+}  // namespace
+
 extern "C" int fasteq_product_forward(const fasteq_product_problem* p, const void* x, const void* w, const void* bias, const void* residual,
                                       const int32_t* offsets, void* y, void* slope, fasteq_stream_t stream) {
   if (const int rc = check(p, offsets)) return rc;
   if (p->rows == 0 || p->n == 0) return FASTEQ_OK;
   if (!y || (p->k > 0 && (!x || !w))) return FASTEQ_INVALID;
+  if (p->dtype == FASTEQ_F32 && p->k > 0 && most_units(p, p->k, p->n) > 0) return run_tc<true>(p, x, nullptr, w, bias, residual, offsets, y, slope, (cudaStream_t)stream);
   return p->dtype == FASTEQ_F32 ? forward<float>(p, x, w, bias, residual, offsets, y, slope, (cudaStream_t)stream)
                                 : forward<double>(p, x, w, bias, residual, offsets, y, slope, (cudaStream_t)stream);
 }
@@ -215,6 +274,8 @@ extern "C" int fasteq_product_dgrad(const fasteq_product_problem* p, const void*
   if (const int rc = check(p, offsets)) return rc;
   if (p->rows == 0 || p->k == 0) return FASTEQ_OK;
   if (!grad_x || (p->n > 0 && (!grad_y || !w))) return FASTEQ_INVALID;
+  if (p->dtype == FASTEQ_F32 && p->n > 0 && most_units(p, p->n, p->k) > 0)
+    return run_tc<false>(p, grad_y, slope, w, nullptr, nullptr, offsets, grad_x, nullptr, (cudaStream_t)stream);
   return p->dtype == FASTEQ_F32 ? dgrad<float>(p, grad_y, slope, w, offsets, grad_x, (cudaStream_t)stream)
                                 : dgrad<double>(p, grad_y, slope, w, offsets, grad_x, (cudaStream_t)stream);
 }

@@ -10,29 +10,50 @@ namespace product {
 
 enum Act : int { kIdentity = 0, kSilu = 1, kTanh = 2, kSigmoid = 3, kAbs = 4 };
 
+// exp(x) within two units of the last place: 2^t for the rounded t = x log2(e), times 1 + what the rounding left of the exponent (a
+// product in two parts, as in Cody and Waite's argument reduction).  A third of the instructions of expf.
+__device__ __forceinline__ float exponential(float x) {
+  constexpr float L = 1.44269502f, L_LOW = 1.92596303e-8f, LN2 = 0.693147181f;
+  const float t = x * L, left = fmaf(x, L_LOW, fmaf(x, L, -t));
+  float e;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(t));
+  return fabsf(t) < 200.f ? fmaf(e, left * LN2, e) : e;      // beyond: 0 or infinity, which `left` (infinite itself there, or not a number) must not touch
+}
+__device__ __forceinline__ double exponential(double x) { return exp(x); }
+__device__ __forceinline__ float reciprocal(float x) {
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ double reciprocal(double x) { return 1.0 / x; }
+
 // act(z) and act'(z)
-template <typename T> __device__ __forceinline__ T activate(int act, T z, T& slope) {
-  if (act == kSilu) {
-    const T e = T(1) + exp(-z), s = T(1) / e;
+template <int ACT, typename T> __device__ __forceinline__ T activate(T z, T& slope) {
+  if (ACT == kSilu) {
+    const T s = reciprocal(T(1) + exponential(-z));
     slope = s * (T(1) + z * (T(1) - s));
-    return z / e;                       // z s rounds once more
+    return z * s;
   }
-  if (act == kTanh) {
+  if (ACT == kTanh) {
     const T t = tanh(z);
     slope = T(1) - t * t;
     return t;
   }
-  if (act == kSigmoid) {
-    const T s = T(1) / (T(1) + exp(-z));
+  if (ACT == kSigmoid) {
+    const T s = reciprocal(T(1) + exponential(-z));
     slope = s * (T(1) - s);
     return s;
   }
-  if (act == kAbs) {
+  if (ACT == kAbs) {
     slope = T((z > T(0)) - (z < T(0)));
     return fabs(z);
   }
   slope = T(1);
   return z;
+}
+template <typename T> __device__ __forceinline__ T activate(int act, T z, T& slope) {
+  return act == kSilu ? activate<kSilu>(z, slope) : act == kTanh ? activate<kTanh>(z, slope) : act == kSigmoid ? activate<kSigmoid>(z, slope)
+       : act == kAbs ? activate<kAbs>(z, slope) : activate<kIdentity>(z, slope);
 }
 
 // Rows of group e: [first(e), first(e + 1)); group `experts` holds those of no expert.
