@@ -21,6 +21,12 @@ fasteq_product_problem problem(const Tensor& x, const Tensor& w, int64_t inner, 
 }
 const int32_t* offsets_of(const Tensor& offsets) { return offsets.defined() ? offsets.const_data_ptr<int32_t>() : nullptr; }
 
+Tensor scratch_of(const fasteq_product_problem& p, bool grad_x, const Tensor& like) {
+  int64_t need = 0;
+  check(core.product_scratch(&p, grad_x, &need), "fasteq_product_scratch", core.last_cuda_error);
+  return need ? at::empty({need}, like.options().dtype(at::kByte)) : Tensor();
+}
+
 Tensor run_forward(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& residual, const Tensor& offsets, int64_t inner, int64_t act,
                    Tensor* slope) {
   c10::cuda::CUDAGuard guard(x.device());
@@ -28,7 +34,9 @@ Tensor run_forward(const Tensor& x, const Tensor& w, const Tensor& bias, const T
   const auto p = problem(xc, wc, inner, act);
   Tensor y = at::empty({xc.size(0), wc.size(1)}, xc.options());
   if (slope) *slope = at::empty_like(y);
-  check(core.product_forward(&p, ptr(xc), ptr(wc), ptr(bc), ptr(rc), offsets_of(offsets), mptr(y), slope ? mptr(*slope) : nullptr, stream_of(xc)),
+  const Tensor scratch = scratch_of(p, false, xc);
+  check(core.product_forward(&p, ptr(xc), ptr(wc), ptr(bc), ptr(rc), offsets_of(offsets), mptr(y), slope ? mptr(*slope) : nullptr, mptr(scratch),
+                             scratch.defined() ? scratch.numel() : 0, stream_of(xc)),
         "fasteq_product_forward", core.last_cuda_error);
   return y;
 }
@@ -38,7 +46,9 @@ Tensor run_dgrad(const Tensor& g, const Tensor& slope, const Tensor& w, const Te
   const Tensor gc = g.contiguous(), wc = w.contiguous();
   const auto p = problem(gc, wc, inner, 0);
   Tensor gx = at::empty({gc.size(0), wc.size(2)}, gc.options());
-  check(core.product_dgrad(&p, ptr(gc), ptr(slope), ptr(wc), offsets_of(offsets), mptr(gx), stream_of(gc)), "fasteq_product_dgrad", core.last_cuda_error);
+  const Tensor scratch = scratch_of(p, true, gc);
+  check(core.product_dgrad(&p, ptr(gc), ptr(slope), ptr(wc), offsets_of(offsets), mptr(gx), mptr(scratch), scratch.defined() ? scratch.numel() : 0, stream_of(gc)),
+        "fasteq_product_dgrad", core.last_cuda_error);
   return gx;
 }
 

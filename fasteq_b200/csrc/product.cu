@@ -217,6 +217,14 @@ long long most_units(const fasteq_product_problem* p, int K, int N) {
   return units > 0x7fffffffLL || (units / 64 + 1) * ((K + ptc::KB - 1) / ptc::KB) > 0x3fffffffLL ? -1 : units;
 }
 
+// bytes of the weights split beforehand: none where a CTA keeps them
+int64_t split_bytes(const fasteq_product_problem* p, bool forward) {
+  const int K = forward ? p->k : p->n, N = forward ? p->n : p->k, n_kb = (K + ptc::KB - 1) / ptc::KB;
+  if (p->dtype != FASTEQ_F32 || K == 0 || N == 0 || p->rows == 0 || most_units(p, K, N) < 0) return 0;
+  const int slots = forward ? ptc::Cfg<false>::SLOTS : ptc::Cfg<true>::SLOTS;
+  return n_kb <= slots ? 0 : (int64_t)p->experts * ((N + ptc::BN - 1) / ptc::BN) * n_kb * ptc::B_BYTES;
+}
+
 template <bool FORWARD, bool SLOPE, int ACT>
 int launch_tc(const fasteq_product_problem* p, ptc::Args& a, int sms, const CUtensorMap& tmA, const CUtensorMap& tmSlope, cudaStream_t s) {
   const int smem = ptc::Cfg<SLOPE>::smem(p->experts);
@@ -229,7 +237,7 @@ int launch_tc(const fasteq_product_problem* p, ptc::Args& a, int sms, const CUte
 // K and N as the kernel sees them (grad_x: exchanged)
 template <bool FORWARD>
 int run_tc(const fasteq_product_problem* p, const void* A, const void* slope, const void* W, const void* bias, const void* residual,
-           const int32_t* offsets, void* C, void* slope_out, cudaStream_t s) {
+           const int32_t* offsets, void* C, void* slope_out, void* scratch, cudaStream_t s) {
   ptc::Args a{};
   a.groups = groups_of(p, offsets);
   a.A = (const float*)A; a.slope = (const float*)slope; a.W = (const float*)W; a.bias = (const float*)bias; a.residual = (const float*)residual;
@@ -241,6 +249,13 @@ int run_tc(const fasteq_product_problem* p, const void* A, const void* slope, co
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e == cudaSuccess) e = tc::status_word(&a.status);
   if (e != cudaSuccess) return cuda_fail(e);
+  if (split_bytes(p, FORWARD) > 0) {
+    const int n_tiles = (a.N + ptc::BN - 1) / ptc::BN, n_kb = (a.K + ptc::KB - 1) / ptc::KB;
+    e = launch_dependent(ptc::split_weights_kernel<FORWARD>, (unsigned)((int64_t)p->experts * n_tiles * n_kb), 256, 0, s, a.W, (unsigned char*)scratch, a.N, a.K,
+                         n_tiles, n_kb, a.w_wide);
+    if (e != cudaSuccess) return cuda_fail(e);
+    a.split = (const unsigned char*)scratch;
+  }
   CUtensorMap tmA{}, tmSlope{};
   if (a.a_wide) {
     int rc = tc::make_map(&tmA, a.A, (uint64_t)a.K, 1, (uint64_t)p->rows, (uint64_t)a.K, (uint64_t)a.K, ptc::KB, 1, ptc::BM);
@@ -259,23 +274,34 @@ int run_tc(const fasteq_product_problem* p, const void* A, const void* slope, co
 
 }  // namespace
 
+extern "C" int fasteq_product_scratch(const fasteq_product_problem* p, int32_t grad_x, int64_t* bytes) {
+  static const int32_t some = 0;
+  if (!bytes) return FASTEQ_INVALID;
+  if (const int rc = check(p, &some)) return rc;
+  *bytes = split_bytes(p, !grad_x);
+  return FASTEQ_OK;
+}
+
 extern "C" int fasteq_product_forward(const fasteq_product_problem* p, const void* x, const void* w, const void* bias, const void* residual,
-                                      const int32_t* offsets, void* y, void* slope, fasteq_stream_t stream) {
+                                      const int32_t* offsets, void* y, void* slope, void* scratch, int64_t scratch_bytes, fasteq_stream_t stream) {
   if (const int rc = check(p, offsets)) return rc;
   if (p->rows == 0 || p->n == 0) return FASTEQ_OK;
-  if (!y || (p->k > 0 && (!x || !w))) return FASTEQ_INVALID;
-  if (p->dtype == FASTEQ_F32 && p->k > 0 && most_units(p, p->k, p->n) > 0) return run_tc<true>(p, x, nullptr, w, bias, residual, offsets, y, slope, (cudaStream_t)stream);
+  const int64_t need = split_bytes(p, true);
+  if (!y || (p->k > 0 && (!x || !w)) || (need > 0 && (!scratch || scratch_bytes < need))) return FASTEQ_INVALID;
+  if (p->dtype == FASTEQ_F32 && p->k > 0 && most_units(p, p->k, p->n) > 0)
+    return run_tc<true>(p, x, nullptr, w, bias, residual, offsets, y, slope, scratch, (cudaStream_t)stream);
   return p->dtype == FASTEQ_F32 ? forward<float>(p, x, w, bias, residual, offsets, y, slope, (cudaStream_t)stream)
                                 : forward<double>(p, x, w, bias, residual, offsets, y, slope, (cudaStream_t)stream);
 }
 
 extern "C" int fasteq_product_dgrad(const fasteq_product_problem* p, const void* grad_y, const void* slope, const void* w, const int32_t* offsets,
-                                    void* grad_x, fasteq_stream_t stream) {
+                                    void* grad_x, void* scratch, int64_t scratch_bytes, fasteq_stream_t stream) {
   if (const int rc = check(p, offsets)) return rc;
   if (p->rows == 0 || p->k == 0) return FASTEQ_OK;
-  if (!grad_x || (p->n > 0 && (!grad_y || !w))) return FASTEQ_INVALID;
+  const int64_t need = split_bytes(p, false);
+  if (!grad_x || (p->n > 0 && (!grad_y || !w)) || (need > 0 && (!scratch || scratch_bytes < need))) return FASTEQ_INVALID;
   if (p->dtype == FASTEQ_F32 && p->n > 0 && most_units(p, p->n, p->k) > 0)
-    return run_tc<false>(p, grad_y, slope, w, nullptr, nullptr, offsets, grad_x, nullptr, (cudaStream_t)stream);
+    return run_tc<false>(p, grad_y, slope, w, nullptr, nullptr, offsets, grad_x, nullptr, scratch, (cudaStream_t)stream);
   return p->dtype == FASTEQ_F32 ? dgrad<float>(p, grad_y, slope, w, offsets, grad_x, (cudaStream_t)stream)
                                 : dgrad<double>(p, grad_y, slope, w, offsets, grad_x, (cudaStream_t)stream);
 }

@@ -8,12 +8,14 @@
 // additions cost it one rounding toward zero per 16 products.
 //
 // A persistent CTA per SM walks a share of the units (expert, 64 columns, 128 rows), rows innermost: the split weights stay in shared memory
-// as long as expert and columns do (k up to 32 x SLOTS; beyond that the blocks go through the slots as a ring).
+// as long as expert and columns do (k up to 32 x SLOTS).  Beyond that a kernel before this one splits the weights, and their blocks go through
+// the slots as a ring, a bulk copy each.
 //   warp 0       brings A's raw k-blocks to shared memory: TMA where K and the address allow it, else copies of four bytes (cp.async)
 //   warp 1       issues the MMAs
-//   warps 2-5    split raw blocks into tensor memory (thread = row = TMEM lane)
-//   warps 6-7    load, split and store the weights' k-blocks
-//   warps 8-15   add the three accumulators, turn the tile in shared memory, and write it with bias, activation and residual
+//   warps 2-3    load, split and store the weights' k-blocks, or bring the split ones
+//   warps 4-11   split raw blocks into tensor memory (thread = row = TMEM lane), four warps the even and four the odd ones
+//   warps 12-19  split the first weights, then add the three accumulators, turn the tile in shared memory, and write it with bias, activation and
+//                residual
 // Every 256 of k the accumulators are emptied (into C, for the sum to go on from there): see GAIN.
 // All waits are bounded; sums that are not finite (operands that are not, or beyond the split's range) are formed again in FP32.
 #pragma once
@@ -27,7 +29,7 @@ namespace ptc {
 using namespace tc;
 using product::Groups;
 
-constexpr int BM = 128, BN = 64, KB = 32, NT = 512;
+constexpr int BM = 128, BN = 64, KB = 32, NT = 640;
 constexpr int SEG = 256 / KB;              // k-blocks of an accumulation
 constexpr int A_BYTES = BM * KB * 4, B_PART = BN * KB * 2, B_BYTES = 3 * B_PART;
 constexpr uint32_t ACC_COLS = 3 * BN, A_COL0 = 2 * ACC_COLS, A_COLS = 3 * KB / 2;
@@ -51,6 +53,9 @@ __device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src, bool t
 // one arrival on the barrier once the thread's copies so far have landed
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, uint32_t n) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(n) : "memory");
 }
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
@@ -98,9 +103,88 @@ __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[16]) {
                  "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
 }
 
+// Values of a 64-column k-block of the weights for THREADS threads: forward, rows n = t / 8 + (THREADS / 8) i of W, four k from 4 (t % 8);
+// grad_x, column n = t % 64 of W, PER k from PER (t / 64)
+template <bool FORWARD, int THREADS>
+__device__ __forceinline__ void load_weights(const float* W, int n0, int N, int K, int kb, int t, bool wide, float (&v)[2048 / THREADS]) {
+  if (FORWARD) {
+    const int k = kb * KB + (t & 7) * 4;
+#pragma unroll
+    for (int i = 0; i < 512 / THREADS; ++i) {
+      const int n = n0 + (t >> 3) + (THREADS / 8) * i;
+      const float* src = W + (size_t)n * K + k;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (n < N) {
+        if (wide) { if (k < K) x = *reinterpret_cast<const float4*>(src); }
+        else {
+          if (k < K) x.x = src[0];
+          if (k + 1 < K) x.y = src[1];
+          if (k + 2 < K) x.z = src[2];
+          if (k + 3 < K) x.w = src[3];
+        }
+      }
+      v[4 * i] = x.x; v[4 * i + 1] = x.y; v[4 * i + 2] = x.z; v[4 * i + 3] = x.w;
+    }
+  } else {
+    constexpr int PER = 2048 / THREADS;
+    const int n = n0 + (t & 63), k = kb * KB + (t >> 6) * PER;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) v[i] = n < N && k + i < K ? W[(size_t)(k + i) * N + n] : 0.f;
+  }
+}
+// their parts at `st`: row n of a part 64 bytes, 16-byte chunk j at chunk position j ^ ((n >> 1) & 3)
+template <bool FORWARD, int THREADS> __device__ __forceinline__ void store_weights(unsigned char* st, int t, const float (&v)[2048 / THREADS]) {
+  if (FORWARD) {
+#pragma unroll
+    for (int i = 0; i < 512 / THREADS; ++i) {
+      const int n = (t >> 3) + (THREADS / 8) * i, at = n * 64 + ((((t & 7) >> 1) ^ ((n >> 1) & 3)) << 4) + (t & 1) * 8;
+      uint2 q[3];
+      wg::split_pair(make_float2(v[4 * i], v[4 * i + 1]), q[0].x, q[1].x, q[2].x);
+      wg::split_pair(make_float2(v[4 * i + 2], v[4 * i + 3]), q[0].y, q[1].y, q[2].y);
+#pragma unroll
+      for (int e = 0; e < 3; ++e) *reinterpret_cast<uint2*>(st + e * B_PART + at) = q[e];
+    }
+  } else {
+    constexpr int CHUNKS = 256 / THREADS;
+    const int n = t & 63;
+#pragma unroll
+    for (int h = 0; h < CHUNKS; ++h) {
+      uint32_t q[3][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) wg::split_pair(make_float2(v[8 * h + 2 * j], v[8 * h + 2 * j + 1]), q[0][j], q[1][j], q[2][j]);
+      const int at = n * 64 + ((((t >> 6) * CHUNKS + h) ^ ((n >> 1) & 3)) << 4);
+#pragma unroll
+      for (int e = 0; e < 3; ++e) *reinterpret_cast<uint4*>(st + e * B_PART + at) = make_uint4(q[e][0], q[e][1], q[e][2], q[e][3]);
+    }
+  }
+}
+
+// All weights split beforehand, [expert][64 columns][k-block] as they lie in shared memory: a block of 256 threads each
+template <bool FORWARD> __global__ void __launch_bounds__(256) split_weights_kernel(const float* W, unsigned char* out, int N, int K, int n_tiles, int n_kb, bool wide) {
+  wait_for_previous_kernel();
+  const int kb = blockIdx.x % n_kb, rest = blockIdx.x / n_kb, n = rest % n_tiles, e = rest / n_tiles;
+  float v[8];
+  load_weights<FORWARD, 256>(W + (size_t)e * N * K, n * BN, N, K, kb, threadIdx.x, wide, v);
+  store_weights<FORWARD, 256>(out + (size_t)blockIdx.x * B_BYTES, threadIdx.x, v);
+}
+
+// sum_k a[k] (d[k]) b[k * stride] with FP32's own products
+__device__ __noinline__ float sum_fp32(const float* a, const float* d, const float* b, int K, int stride) {
+  float v = 0.f;
+#pragma unroll 1
+  for (int k = 0; k < K; ++k) v = fmaf(d ? a[k] * d[k] : a[k], b[(size_t)k * stride], v);
+  return v;
+}
+
+template <int ACT> __device__ __noinline__ void wild(float4& v, float4& d) {
+  v.x = product::activate<ACT>(v.x, d.x); v.y = product::activate<ACT>(v.y, d.y);
+  v.z = product::activate<ACT>(v.z, d.z); v.w = product::activate<ACT>(v.w, d.w);
+}
+
 struct Args {
   Groups groups;
   const float *A, *slope, *W, *bias, *residual;
+  const unsigned char* split;         // the weights' blocks where they do not stay in shared memory
   float *C, *slope_out;
   int K, N;
   bool a_wide, w_wide, c_wide;        // 16-byte accesses of A (and slope), of W, of everything shaped like C (and bias)
@@ -131,7 +215,7 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&a_full[s], p.a_wide ? 1 : 32); mbar_init(&a_empty[s], 4); }
-    for (int s = 0; s < SLOTS; ++s) { mbar_init(&b_full[s], 2); mbar_init(&b_empty[s], 1); }
+    for (int s = 0; s < SLOTS; ++s) { mbar_init(&b_full[s], p.split ? 1 : 8); mbar_init(&b_empty[s], 1); }
     for (int s = 0; s < 2; ++s) { mbar_init(&s_full[s], 4); mbar_init(&s_empty[s], 1); mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 8); }
     mbar_fence_init();
   }
@@ -160,7 +244,7 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
   __syncthreads();
   const uint32_t tmem = *tmem_slot;
   const int n_tiles = (N + BN - 1) / BN, n_kb = (K + KB - 1) / KB;
-  const bool resident = n_kb <= SLOTS;
+  const bool resident = p.split == nullptr;        // n_kb <= SLOTS then
   const long long units = (long long)tiles[X] * n_tiles;
   const int u0 = (int)(units * blockIdx.x / gridDim.x), u1 = (int)(units * (blockIdx.x + 1) / gridDim.x);
 
@@ -238,15 +322,52 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
         if (ends) run += n_kb;
         w.next();
       }
-    } else if (warp < 6) {
+    } else if (warp < 4) {
+      // ------------------------------------------------------------------ the weights' parts
+      const int t = threadIdx.x - 64;
+      int fill = 0;
+      for (int u = u0; u < u1; ++u, w.next()) {
+        if (!resident) {
+          if (t == 0) {
+            const unsigned char* src = p.split + ((size_t)w.e * n_tiles + w.n) * n_kb * B_BYTES;
+            for (int kb = 0; kb < n_kb; ++kb, ++fill) {
+              const int slot = fill % SLOTS;
+              mbar_wait(&b_empty[slot], ((fill / SLOTS) & 1u) ^ 1u, status);
+              mbar_arrive_expect_tx(&b_full[slot], (uint32_t)B_BYTES);
+              bulk_g2s(smem + (size_t)slot * B_BYTES, src + (size_t)kb * B_BYTES, (uint32_t)B_BYTES, &b_full[slot]);
+            }
+          }
+          continue;
+        }
+        if (u == u0) fill += n_kb;                 // the first ones are split by the epilogue's warps
+        if (u == u0 || !w.run_begins(false)) continue;
+        const float* W = p.W + (size_t)w.e * N * K;
+        float v[32], ahead[32];
+        load_weights<FORWARD, 64>(W, w.n * BN, N, K, 0, t, p.w_wide, v);
+        for (int kb = 0; kb < n_kb; ++kb, ++fill) {
+          if (kb + 1 < n_kb) load_weights<FORWARD, 64>(W, w.n * BN, N, K, kb + 1, t, p.w_wide, ahead);
+          const int slot = fill % SLOTS;
+          mbar_wait(&b_empty[slot], ((fill / SLOTS) & 1u) ^ 1u, status);
+          store_weights<FORWARD, 64>(smem + (size_t)slot * B_BYTES, t, v);
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_n(&b_full[slot], 4);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = ahead[i];
+        }
+      }
+    } else if (warp < 12) {
       // ------------------------------------------------------------------ split A into tensor memory
-      const int row = (warp & 3) * 32 + lane;
-      const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + A_COL0;
+      const int row = (warp & 3) * 32 + lane, slot = (warp - 4) >> 2;
+      const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + A_COL0 + (uint32_t)(slot * A_COLS);
       const int total = (u1 - u0) * n_kb;
-      for (int it = 0; it < total; ++it) {
-        const int s = it % STAGES, slot = it & 1;
-        mbar_wait(&a_full[s], (it / STAGES) & 1u, status);
+      for (int it = slot; it < total; it += 2) {
+        const int s = it % STAGES;
+        // The slot first: with block it - 2 multiplied, the other warps have passed the stage's last phase (it - STAGES), and its parity
+        // cannot be taken for this block's.
         mbar_wait(&s_empty[slot], ((it >> 1) & 1u) ^ 1u, status);
+        mbar_wait(&a_full[s], (it / STAGES) & 1u, status);
+        __syncwarp();
         tc_fence_after();
         const unsigned char* st = a_raw + (size_t)s * C_::STAGE_BYTES + row * 128;
 #pragma unroll
@@ -264,7 +385,7 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
             wg::split_pair(make_float2(v.z, v.w), q[0][2 * j + 1], q[1][2 * j + 1], q[2][2 * j + 1]);
           }
 #pragma unroll
-          for (int e = 0; e < 3; ++e) wg::tmem_st_8(lanes + (uint32_t)(slot * A_COLS + e * (KB / 2) + ks * 8), q[e]);
+          for (int e = 0; e < 3; ++e) wg::tmem_st_8(lanes + (uint32_t)(e * (KB / 2) + ks * 8), q[e]);
         }
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         tc_fence_before();
@@ -272,80 +393,28 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
         __syncwarp();
         if (lane == 0) { mbar_arrive(&s_full[slot]); mbar_arrive(&a_empty[s]); }
       }
-    } else if (warp < 8) {
-      // ------------------------------------------------------------------ the weights' parts
-      // row n of a part: 64 bytes, 16-byte chunk j at chunk position j ^ ((n >> 1) & 3)
-      const int t = threadIdx.x - 192;
-      int fill = 0;
-      for (int u = u0; u < u1; ++u, w.next()) {
-        if (resident && !w.run_begins(u == u0)) continue;
-        const float* W = p.W + (size_t)w.e * N * K;
-        const int n0 = w.n * BN;
-        // 32 values a thread and block: forward, rows n = t / 8 + 8 i of W, four k from 4 (t % 8); grad_x, column n = t of W, all 32 k
-        auto load = [&](int kb, float (&v)[32]) {
-          if (FORWARD) {
-            const int k = kb * KB + (t & 7) * 4;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int n = n0 + (t >> 3) + 8 * i;
-              const float* src = W + (size_t)n * K + k;
-              float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-              if (n < N) {
-                if (p.w_wide) { if (k < K) x = *reinterpret_cast<const float4*>(src); }
-                else {
-                  if (k < K) x.x = src[0];
-                  if (k + 1 < K) x.y = src[1];
-                  if (k + 2 < K) x.z = src[2];
-                  if (k + 3 < K) x.w = src[3];
-                }
-              }
-              v[4 * i] = x.x; v[4 * i + 1] = x.y; v[4 * i + 2] = x.z; v[4 * i + 3] = x.w;
-            }
-          } else {
-            const int n = n0 + t, k = kb * KB;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = n < N && k + i < K ? W[(size_t)(k + i) * N + n] : 0.f;
-          }
-        };
-        float v[32], ahead[32];
-        load(0, v);
-        for (int kb = 0; kb < n_kb; ++kb, ++fill) {
-          if (kb + 1 < n_kb) load(kb + 1, ahead);
-          const int slot = fill % SLOTS;
-          mbar_wait(&b_empty[slot], ((fill / SLOTS) & 1u) ^ 1u, status);
-          unsigned char* st = smem + (size_t)slot * B_BYTES;
-          if (FORWARD) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int n = (t >> 3) + 8 * i, at = n * 64 + ((((t & 7) >> 1) ^ ((n >> 1) & 3)) << 4) + (t & 1) * 8;
-              uint2 q[3];
-              wg::split_pair(make_float2(v[4 * i], v[4 * i + 1]), q[0].x, q[1].x, q[2].x);
-              wg::split_pair(make_float2(v[4 * i + 2], v[4 * i + 3]), q[0].y, q[1].y, q[2].y);
-#pragma unroll
-              for (int e = 0; e < 3; ++e) *reinterpret_cast<uint2*>(st + e * B_PART + at) = q[e];
-            }
-          } else {
-#pragma unroll
-            for (int h = 0; h < 4; ++h) {
-              uint32_t q[3][4];
-#pragma unroll
-              for (int j = 0; j < 4; ++j) wg::split_pair(make_float2(v[8 * h + 2 * j], v[8 * h + 2 * j + 1]), q[0][j], q[1][j], q[2][j]);
-              const int at = t * 64 + ((h ^ ((t >> 1) & 3)) << 4);
-#pragma unroll
-              for (int e = 0; e < 3; ++e) *reinterpret_cast<uint4*>(st + e * B_PART + at) = make_uint4(q[e][0], q[e][1], q[e][2], q[e][3]);
-            }
-          }
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&b_full[slot]);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = ahead[i];
-        }
-      }
     } else {
       // ------------------------------------------------------------------ epilogue: 32 rows and 32 columns to a warp
-      const int quarter = warp & 3, half = (warp - 8) >> 2;
-      unsigned char* slab = slabs + (size_t)(warp - 8) * 4096;       // 16-byte chunk j of row r at j ^ (r & 7)
+      if (resident) {
+        const int t = threadIdx.x - 384;
+        const float* W = p.W + (size_t)w.e * N * K;
+        for (int k0 = 0; k0 < n_kb; k0 += 4) {
+          float v[4][8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (k0 + i < n_kb) load_weights<FORWARD, 256>(W, w.n * BN, N, K, k0 + i, t, p.w_wide, v[i]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (k0 + i >= n_kb) break;
+            store_weights<FORWARD, 256>(smem + (size_t)(k0 + i) * B_BYTES, t, v[i]);
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&b_full[k0 + i]);
+          }
+        }
+      }
+      const int quarter = warp & 3, half = (warp - 12) >> 2;
+      unsigned char* slab = slabs + (size_t)(warp - 12) * 4096;      // 16-byte chunk j of row r at j ^ (r & 7)
       const uint32_t cols = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 32);
       int lt = 0;
       for (int u = u0; u < u1; ++u, w.next()) {
@@ -354,26 +423,19 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
         const int rows = (int)(left < BM ? left : BM) - quarter * 32;      // of this warp
         const size_t row0 = (size_t)(begin + (long long)w.m * BM + quarter * 32);
         // wide: four columns, eight rows a thread; else one column, all rows
-        const int c = p.c_wide ? (lane & 7) * 4 : lane, n = nh + c, r0 = p.c_wide ? lane >> 3 : 0;
+        const int c = p.c_wide ? (lane & 7) * 4 : lane, n = nh + c;
         const bool column = n < N;
-        float4 bias = make_float4(0.f, 0.f, 0.f, 0.f), res[8];
+        float4 bias = make_float4(0.f, 0.f, 0.f, 0.f);
         if (FORWARD && p.bias && column) {
           const float* b = p.bias + (size_t)w.e * N + n;
           if (p.c_wide) bias = *reinterpret_cast<const float4*>(b); else bias.x = *b;
-        }
-        if (FORWARD && p.residual && p.c_wide) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            res[i] = column && r0 + 4 * i < rows ? *reinterpret_cast<const float4*>(p.residual + (row0 + r0 + 4 * i) * N + n) : make_float4(0.f, 0.f, 0.f, 0.f);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) res[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
         for (int k0 = 0; k0 < n_kb; k0 += SEG, ++lt) {
           const int buf = lt & 1;
           const bool last = k0 + SEG >= n_kb;
           const float gain = GAIN * (float)((min(K, (k0 + SEG) * KB) - k0 * KB + 15) / 16);
           mbar_wait(&acc_full[buf], (lt >> 1) & 1u, status);
+          __syncwarp();
           tc_fence_after();
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -387,52 +449,60 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
             tmem_ld_wait(z);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              float o[4];
+              float2 o[2];
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float large = __uint_as_float(x[4 * j + i]);
-                o[i] = (large + fmaf(large, gain, __uint_as_float(y[4 * j + i]) + __uint_as_float(z[4 * j + i]))) * wg::UNSCALE;
+              for (int i = 0; i < 2; ++i) {
+                const int q = 4 * j + 2 * i;
+                auto two = [&](const uint32_t (&r)[16]) { return make_float2(__uint_as_float(r[q]), __uint_as_float(r[q + 1])); };
+                o[i] = vmul(vadd(two(x), vfma(two(x), make_float2(gain, gain), vadd(two(y), two(z)))), make_float2(wg::UNSCALE, wg::UNSCALE));
               }
-              *reinterpret_cast<float4*>(slab + lane * 128 + (((h * 4 + j) ^ (lane & 7)) << 4)) = make_float4(o[0], o[1], o[2], o[3]);
+              *reinterpret_cast<float4*>(slab + lane * 128 + (((h * 4 + j) ^ (lane & 7)) << 4)) = make_float4(o[0].x, o[0].y, o[1].x, o[1].y);
             }
           }
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&acc_empty[buf]);
-          // value (row r, column m) of the layer, from its sum
-          auto value = [&](float v, int r, int m, float bias, float residual, float& slope) {
-            if (!(fabsf(v) <= 3.402823466e38f)) {
-              const float* a = p.A + (row0 + r) * K;
-              const float* d = SLOPE ? p.slope + (row0 + r) * K : nullptr;
-              const float* b = p.W + (size_t)w.e * N * K + (FORWARD ? (size_t)m * K : (size_t)m);
-              v = 0.f;
-#pragma unroll 1
-              for (int k = 0; k < K; ++k) v = fmaf(SLOPE ? a[k] * d[k] : a[k], b[FORWARD ? (size_t)k : (size_t)k * N], v);
-            }
-            slope = 1.f;
-            if (!FORWARD) return v;
-            v = product::activate<ACT>(v + bias, slope);
-            return v + residual;
+          // a sum that is not finite, again in FP32
+          auto again = [&](float v, int r, int m) {
+            if (fabsf(v) <= 3.402823466e38f) return v;
+            return sum_fp32(p.A + (row0 + r) * K, SLOPE ? p.slope + (row0 + r) * K : nullptr,
+                            p.W + (size_t)w.e * N * K + (FORWARD ? (size_t)m * K : (size_t)m), K, FORWARD ? 1 : N);
           };
           if (column && p.c_wide) {
-#pragma unroll
+            const float* from = reinterpret_cast<const float*>(slab + (lane >> 3) * 128);
+#pragma unroll 4
             for (int i = 0; i < 8; ++i) {
-              const int r = r0 + i * 4;
-              if (r >= rows) continue;
+              const int r = (lane >> 3) + i * 4;
+              if (r >= rows) break;
               const size_t o = (row0 + r) * N + n;
-              float4 s = *reinterpret_cast<const float4*>(slab + r * 128 + (((lane & 7) ^ (r & 7)) << 4)), v = s, d;
+              float4 v = *reinterpret_cast<const float4*>(from + i * 128 + (((lane & 7) ^ (r & 7)) << 2));
               if (k0 > 0) {
                 const float4 before = *reinterpret_cast<const float4*>(p.C + o);
-                v.x = s.x += before.x; v.y = s.y += before.y; v.z = s.z += before.z; v.w = s.w += before.w;
+                v.x += before.x; v.y += before.y; v.z += before.z; v.w += before.w;
               }
               if (last) {
-                v.x = value(s.x, r, n, bias.x, res[i].x, d.x);
-                v.y = value(s.y, r, n + 1, bias.y, res[i].y, d.y);
-                v.z = value(s.z, r, n + 2, bias.z, res[i].z, d.z);
-                v.w = value(s.w, r, n + 3, bias.w, res[i].w, d.w);
+                const float2 z0 = make_float2(v.x + bias.x, v.y + bias.y), z1 = make_float2(v.z + bias.z, v.w + bias.w);
+                float4 d;
+                // larger than kTame, infinite or not a number: in magnitude bits
+                auto bits = [](float x) { return __float_as_uint(x) & 0x7fffffffu; };
+                constexpr float most = ACT == product::kIdentity || ACT == product::kAbs ? 3.402823466e38f : product::kTame;
+                if (max(max(bits(z0.x), bits(z0.y)), max(bits(z1.x), bits(z1.y))) <= __float_as_uint(most)) {
+                  float2 d0, d1;
+                  const float2 y0 = FORWARD ? product::activate_tame<ACT>(z0, p.slope_out != nullptr, d0) : z0;
+                  const float2 y1 = FORWARD ? product::activate_tame<ACT>(z1, p.slope_out != nullptr, d1) : z1;
+                  v = make_float4(y0.x, y0.y, y1.x, y1.y);
+                  d = make_float4(d0.x, d0.y, d1.x, d1.y);
+                } else {
+                  v.x = again(v.x, r, n) + bias.x; v.y = again(v.y, r, n + 1) + bias.y; v.z = again(v.z, r, n + 2) + bias.z; v.w = again(v.w, r, n + 3) + bias.w;
+                  if (FORWARD) wild<ACT>(v, d);
+                }
+                if (FORWARD && p.residual) {
+                  const float4 res = *reinterpret_cast<const float4*>(p.residual + o);
+                  v.x += res.x; v.y += res.y; v.z += res.z; v.w += res.w;
+                }
+                if (FORWARD && p.slope_out) *reinterpret_cast<float4*>(p.slope_out + o) = d;
               }
               *reinterpret_cast<float4*>(p.C + o) = v;
-              if (FORWARD && last && p.slope_out) *reinterpret_cast<float4*>(p.slope_out + o) = d;
             }
           } else if (column) {
 #pragma unroll 4
@@ -441,9 +511,15 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
               const size_t o = (row0 + r) * N + n;
               float d, v = *reinterpret_cast<const float*>(slab + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
               if (k0 > 0) v += p.C[o];
-              if (last) v = value(v, r, n, bias.x, FORWARD && p.residual ? p.residual[o] : 0.f, d);
+              if (last) {
+                const float res = FORWARD && p.residual ? p.residual[o] : 0.f;
+                v = again(v, r, n);
+                if (FORWARD) {
+                  v = product::activate<ACT>(v + bias.x, d) + res;
+                  if (p.slope_out) p.slope_out[o] = d;
+                }
+              }
               p.C[o] = v;
-              if (FORWARD && last && p.slope_out) p.slope_out[o] = d;
             }
           }
           __syncwarp();

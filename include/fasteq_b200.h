@@ -456,13 +456,15 @@ typedef struct fasteq_product_problem {
   int32_t act;
   int64_t rows;
 } fasteq_product_problem;
+/* scratch: 16-byte aligned device memory of the bytes `_scratch` names (grad_x: for `_dgrad`; may be 0, NULL then), not in use by other work on the
+ * device meanwhile. */
+int fasteq_product_scratch(const fasteq_product_problem* p /* host */, int32_t grad_x, int64_t* bytes /* host */);
 int fasteq_product_forward(const fasteq_product_problem* p /* host */, const void* x, const void* w, const void* bias /* or NULL */,
                            const void* residual /* or NULL */, const int32_t* offsets /* or NULL */, void* y, void* slope /* or NULL */,
-                           fasteq_stream_t stream);
+                           void* scratch, int64_t scratch_bytes, fasteq_stream_t stream);
 int fasteq_product_dgrad(const fasteq_product_problem* p /* host */, const void* grad_y, const void* slope /* or NULL */, const void* w,
-                         const int32_t* offsets /* or NULL */, void* grad_x, fasteq_stream_t stream);
-/* Weight and bias gradient (grad_bias may be NULL).  scratch: 16-byte aligned device memory of the bytes `_scratch` names, not in use by other
- * work on the device meanwhile. */
+                         const int32_t* offsets /* or NULL */, void* grad_x, void* scratch, int64_t scratch_bytes, fasteq_stream_t stream);
+/* Weight and bias gradient (grad_bias may be NULL), with a scratch of its own. */
 int fasteq_product_wgrad_scratch(const fasteq_product_problem* p /* host */, int64_t* bytes /* host */);
 int fasteq_product_wgrad(const fasteq_product_problem* p /* host */, const void* x, const void* grad_y, const void* slope /* or NULL */,
                          const int32_t* offsets /* or NULL */, void* grad_w, void* grad_bias /* or NULL */, void* scratch, int64_t scratch_bytes,

@@ -40,14 +40,19 @@ def _core():
 def test_forward_problems(change, status):
     lib = _core()
     p = Problem(**{**GOOD, **change})
-    assert lib.fasteq_product_forward(C.byref(p), None, None, None, None, None, None, None, None) == status
+    assert lib.fasteq_product_forward(C.byref(p), None, None, None, None, None, None, None, None, I64(0), None) == status
 
 
 def test_other_entries_refuse_null_pointers_and_sizes():
     lib = _core()
     p, one = Problem(**GOOD), C.c_int64(0)
-    assert lib.fasteq_product_forward(None, None, None, None, None, None, None, None, None) == INVALID
-    assert lib.fasteq_product_dgrad(C.byref(p), None, None, None, None, None, None) == INVALID
+    assert lib.fasteq_product_forward(None, None, None, None, None, None, None, None, None, I64(0), None) == INVALID
+    assert lib.fasteq_product_dgrad(C.byref(p), None, None, None, None, None, None, I64(0), None) == INVALID
+    assert lib.fasteq_product_scratch(C.byref(p), I32(0), None) == INVALID and lib.fasteq_product_scratch(C.byref(p), I32(1), C.byref(one)) == OK
+    long = Problem(**{**GOOD, "k": 2048})
+    assert lib.fasteq_product_scratch(C.byref(long), I32(0), C.byref(one)) == OK and one.value > 0
+    some = C.create_string_buffer(64)
+    assert lib.fasteq_product_forward(C.byref(long), some, some, None, None, None, some, None, some, I64(16), None) == INVALID
     assert lib.fasteq_product_wgrad_scratch(C.byref(p), C.byref(one)) == OK and one.value > 0
     assert lib.fasteq_product_wgrad_scratch(C.byref(p), None) == INVALID
     assert lib.fasteq_product_wgrad(C.byref(p), None, None, None, None, None, None, None, I64(0), None) == INVALID
