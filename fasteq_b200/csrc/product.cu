@@ -221,16 +221,17 @@ long long most_units(const fasteq_product_problem* p, int K, int N) {
 int64_t split_bytes(const fasteq_product_problem* p, bool forward) {
   const int K = forward ? p->k : p->n, N = forward ? p->n : p->k, n_kb = (K + ptc::KB - 1) / ptc::KB;
   if (p->dtype != FASTEQ_F32 || K == 0 || N == 0 || p->rows == 0 || most_units(p, K, N) < 0) return 0;
-  const int slots = forward ? ptc::Cfg<false>::SLOTS : ptc::Cfg<true>::SLOTS;
-  return n_kb <= slots ? 0 : (int64_t)p->experts * ((N + ptc::BN - 1) / ptc::BN) * n_kb * ptc::B_BYTES;
+  const int slots = forward ? ptc::Cfg<false>::slots(p->experts) : ptc::Cfg<true>::slots(p->experts);
+  return n_kb <= std::min(slots, ptc::Cfg<false>::slots(p->experts)) ? 0 : (int64_t)p->experts * ((N + ptc::BN - 1) / ptc::BN) * n_kb * ptc::B_BYTES;
 }
 
 template <bool FORWARD, bool SLOPE, int ACT>
-int launch_tc(const fasteq_product_problem* p, ptc::Args& a, int sms, const CUtensorMap& tmA, const CUtensorMap& tmSlope, cudaStream_t s) {
-  const int smem = ptc::Cfg<SLOPE>::smem(p->experts);
+int launch_tc(const fasteq_product_problem* p, ptc::Args& a, int sms, const CUtensorMap (&tm)[4], cudaStream_t s) {
+  a.slots = ptc::Cfg<SLOPE>::slots(p->experts);
+  const int smem = ptc::Cfg<SLOPE>::smem(a.slots, p->experts);
   cudaError_t e = cudaFuncSetAttribute(ptc::product_tc_kernel<FORWARD, SLOPE, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e == cudaSuccess)
-    e = launch_dependent(ptc::product_tc_kernel<FORWARD, SLOPE, ACT>, (unsigned)std::min<long long>(sms, most_units(p, a.K, a.N)), ptc::NT, smem, s, a, tmA, tmSlope);
+    e = launch_dependent(ptc::product_tc_kernel<FORWARD, SLOPE, ACT>, (unsigned)std::min<long long>(sms, most_units(p, a.K, a.N)), ptc::NT, smem, s, a, tm[0], tm[1], tm[2], tm[3]);
   return e == cudaSuccess ? FASTEQ_OK : cuda_fail(e);
 }
 
@@ -243,7 +244,7 @@ int run_tc(const fasteq_product_problem* p, const void* A, const void* slope, co
   a.A = (const float*)A; a.slope = (const float*)slope; a.W = (const float*)W; a.bias = (const float*)bias; a.residual = (const float*)residual;
   a.C = (float*)C; a.slope_out = (float*)slope_out;
   a.K = FORWARD ? p->k : p->n; a.N = FORWARD ? p->n : p->k;
-  a.a_wide = wide(a.K, {A, slope}) && p->rows <= 0x7fffffffLL; a.w_wide = wide(p->k, {W}); a.c_wide = wide(a.N, {C, slope_out, bias, residual});
+  a.a_wide = wide(a.K, {A, slope}) && p->rows <= 0x7fffffffLL; a.w_wide = wide(p->k, {W}); a.c_wide = wide(a.N, {C, slope_out, bias, residual}) && p->rows <= 0x7fffffffLL;
   int sms = 0, dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
@@ -256,19 +257,21 @@ int run_tc(const fasteq_product_problem* p, const void* A, const void* slope, co
     if (e != cudaSuccess) return cuda_fail(e);
     a.split = (const unsigned char*)scratch;
   }
-  CUtensorMap tmA{}, tmSlope{};
-  if (a.a_wide) {
-    int rc = tc::make_map(&tmA, a.A, (uint64_t)a.K, 1, (uint64_t)p->rows, (uint64_t)a.K, (uint64_t)a.K, ptc::KB, 1, ptc::BM);
-    if (rc == FASTEQ_OK && slope) rc = tc::make_map(&tmSlope, a.slope, (uint64_t)a.K, 1, (uint64_t)p->rows, (uint64_t)a.K, (uint64_t)a.K, ptc::KB, 1, ptc::BM);
-    if (rc != FASTEQ_OK) return rc;
-  }
-  if (!FORWARD) return slope ? launch_tc<false, true, kIdentity>(p, a, sms, tmA, tmSlope, s) : launch_tc<false, false, kIdentity>(p, a, sms, tmA, tmSlope, s);
+  CUtensorMap tm[4] = {};               // A, its slope; C, its slope
+  int rc = FASTEQ_OK;
+  auto map = [&](int i, const float* base, int columns, uint32_t box_rows) {
+    if (rc == FASTEQ_OK && base) rc = tc::make_map(&tm[i], base, (uint64_t)columns, 1, (uint64_t)p->rows, (uint64_t)columns, (uint64_t)columns, 32, 1, box_rows);
+  };
+  if (a.a_wide) { map(0, a.A, a.K, ptc::BM); map(1, a.slope, a.K, ptc::BM); }
+  if (a.c_wide) { map(2, a.C, a.N, 32); map(3, a.slope_out, a.N, 32); }
+  if (rc != FASTEQ_OK) return rc;
+  if (!FORWARD) return slope ? launch_tc<false, true, kIdentity>(p, a, sms, tm, s) : launch_tc<false, false, kIdentity>(p, a, sms, tm, s);
   switch (p->act) {
-    case kSilu: return launch_tc<true, false, kSilu>(p, a, sms, tmA, tmSlope, s);
-    case kTanh: return launch_tc<true, false, kTanh>(p, a, sms, tmA, tmSlope, s);
-    case kSigmoid: return launch_tc<true, false, kSigmoid>(p, a, sms, tmA, tmSlope, s);
-    case kAbs: return launch_tc<true, false, kAbs>(p, a, sms, tmA, tmSlope, s);
-    default: return launch_tc<true, false, kIdentity>(p, a, sms, tmA, tmSlope, s);
+    case kSilu: return launch_tc<true, false, kSilu>(p, a, sms, tm, s);
+    case kTanh: return launch_tc<true, false, kTanh>(p, a, sms, tm, s);
+    case kSigmoid: return launch_tc<true, false, kSigmoid>(p, a, sms, tm, s);
+    case kAbs: return launch_tc<true, false, kAbs>(p, a, sms, tm, s);
+    default: return launch_tc<true, false, kIdentity>(p, a, sms, tm, s);
   }
 }
 

@@ -10,40 +10,32 @@ namespace product {
 
 enum Act : int { kIdentity = 0, kSilu = 1, kTanh = 2, kSigmoid = 3, kAbs = 4 };
 
-// exp(x) within two units of the last place: 2^t for the rounded t = x log2(e), times 1 + what the rounding left of the exponent (a
-// product in two parts, as in Cody and Waite's argument reduction); below 2^-126 it is 0.
-constexpr float kLog2e = 1.44269502f, kLog2eLow = 1.92596303e-8f, kLn2 = 0.693147181f;
+// 2^t within two units of the last place (0 below 2^-126), and 1 / x within one (0 from 2^126 on)
 __device__ __forceinline__ float power_of_two(float t) {
   float e;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
   return e;
 }
-__device__ __forceinline__ float exponential(float x) {
-  const float t = x * kLog2e, left = fmaf(x, kLog2eLow, fmaf(x, kLog2e, -t)), e = power_of_two(t);
-  return fabsf(t) < 200.f ? fmaf(e, left * kLn2, e) : e;      // beyond: 0 or infinity, which `left` (infinite itself there, or not a number) must not touch
-}
-__device__ __forceinline__ double exponential(double x) { return exp(x); }
-// within a unit of the last place; 0 from 2^126 on
 __device__ __forceinline__ float reciprocal(float x) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-__device__ __forceinline__ double reciprocal(double x) { return 1.0 / x; }
-// 1 / (1 + exp(-z)) of two values of at most kTame in magnitude, or not numbers
-constexpr float kTame = 80.f;
-__device__ __forceinline__ float2 sigmoid_tame(float2 z) {
-  const float2 l = make_float2(-kLog2e, -kLog2e), low = make_float2(-kLog2eLow, -kLog2eLow), ln2 = make_float2(kLn2, kLn2), one = make_float2(1.f, 1.f);
-  const float2 t = vmul(z, l), minus_t = make_float2(-t.x, -t.y);
-  const float2 left = vmul(vfma(z, low, vfma(z, l, minus_t)), ln2), e = make_float2(power_of_two(t.x), power_of_two(t.y));
-  const float2 d = vadd(vfma(e, left, e), one);
+constexpr float kLog2e = 1.44269502f;
+// 1 / (1 + exp(-z)).  In FP32 the exponent -z log2(e) is rounded once, which moves the exponential by |z| half steps, as z's own rounding
+// did before; infinities come out as 0 and 1.
+__device__ __forceinline__ float sigmoid(float z) { return reciprocal(1.f + power_of_two(z * -kLog2e)); }
+__device__ __forceinline__ double sigmoid(double z) { return 1.0 / (1.0 + exp(-z)); }
+__device__ __forceinline__ float2 sigmoid(float2 z) {
+  const float2 t = vmul(z, make_float2(-kLog2e, -kLog2e));
+  const float2 d = vadd(make_float2(power_of_two(t.x), power_of_two(t.y)), make_float2(1.f, 1.f));
   return make_float2(reciprocal(d.x), reciprocal(d.y));
 }
 
 // act(z) and act'(z)
 template <int ACT, typename T> __device__ __forceinline__ T activate(T z, T& slope) {
   if (ACT == kSilu) {
-    const T s = reciprocal(T(1) + exponential(-z));
+    const T s = sigmoid(z);
     slope = s * (T(1) + z * (T(1) - s));
     return z * s;
   }
@@ -53,7 +45,7 @@ template <int ACT, typename T> __device__ __forceinline__ T activate(T z, T& slo
     return t;
   }
   if (ACT == kSigmoid) {
-    const T s = reciprocal(T(1) + exponential(-z));
+    const T s = sigmoid(z);
     slope = s * (T(1) - s);
     return s;
   }
@@ -64,11 +56,14 @@ template <int ACT, typename T> __device__ __forceinline__ T activate(T z, T& slo
   slope = T(1);
   return z;
 }
-// Two values of at most kTame in magnitude, or not numbers; the slope where it is asked for.
-template <int ACT> __device__ __forceinline__ float2 activate_tame(float2 z, bool with_slope, float2& slope) {
+// two values; the slope where it is asked for
+template <int ACT> __device__ __forceinline__ float2 activate(float2 z, bool with_slope, float2& slope) {
   if (ACT == kSilu || ACT == kSigmoid) {
-    const float2 s = sigmoid_tame(z), one = make_float2(1.f, 1.f), rest = make_float2(1.f - s.x, 1.f - s.y);
-    if (with_slope) slope = ACT == kSilu ? vmul(s, vfma(z, rest, one)) : vmul(s, rest);
+    const float2 s = sigmoid(z), one = make_float2(1.f, 1.f);
+    if (with_slope) {
+      const float2 rest = make_float2(1.f - s.x, 1.f - s.y);
+      slope = ACT == kSilu ? vmul(s, vfma(z, rest, one)) : vmul(s, rest);
+    }
     return ACT == kSilu ? vmul(z, s) : s;
   }
   float2 y;

@@ -2,20 +2,19 @@
 //   C[r, n] = epilogue(sum_k A[r, k] (slope[r, k]) B[e(r)][k, n]),   B = W^T (forward) or W (grad_x)
 //
 // Each FP32 operand v is three bf16 parts v = v1 + v2 + v3 (exact: 8 + 8 + 8 significand bits, see wgrad_bf16x6.cuh for the range), and
-// v1 w1 + (v1 w2 + v2 w1) + (v1 w3 + v2 w2 + v3 w1) leaves out terms of 2^-27 v w.  The weights' parts of a 32-wide k-block lie stacked in
-// shared memory, [w1; w2; w3] = 192 rows of 64 columns' tiles, so that a K = 16 step is three MMAs, v1 x 192, v2 x 128, v3 x 64, which leave
-// the three magnitudes in accumulators of their own: only the first is as large as the result, and the tensor core's truncating
-// additions cost it one rounding toward zero per 16 products.
+// v1 w1 + (v1 w2 + v2 w1 + v1 w3 + v2 w2 + v3 w1) leaves out terms of 2^-27 v w.  The weights' parts of a 32-wide k-block lie stacked in
+// shared memory, [w1; w2; w3], so that a K = 16 step is five MMAs, v1 x [w1; w2] and four of 64 columns.  The first product has an
+// accumulator of its own and the small ones another: only the first is as large as the result, and the tensor core's truncating additions
+// cost it one rounding toward zero per 16 products.
 //
 // A persistent CTA per SM walks a share of the units (expert, 64 columns, 128 rows), rows innermost: the split weights stay in shared memory
-// as long as expert and columns do (k up to 32 x SLOTS).  Beyond that a kernel before this one splits the weights, and their blocks go through
+// as long as expert and columns do (k up to 32 x slots).  Beyond that a kernel before this one splits the weights, and their blocks go through
 // the slots as a ring, a bulk copy each.
 //   warp 0       brings A's raw k-blocks to shared memory: TMA where K and the address allow it, else copies of four bytes (cp.async)
 //   warp 1       issues the MMAs
 //   warps 2-3    load, split and store the weights' k-blocks, or bring the split ones
 //   warps 4-11   split raw blocks into tensor memory (thread = row = TMEM lane), four warps the even and four the odd ones
-//   warps 12-19  split the first weights, then add the three accumulators, turn the tile in shared memory, and write it with bias, activation and
-//                residual
+//   warps 12-19  split the first weights, then add the two accumulators, bias, activation and residual, and store tiles of 32 x 32 by TMA
 // Every 256 of k the accumulators are emptied (into C, for the sum to go on from there): see GAIN.
 // All waits are bounded; sums that are not finite (operands that are not, or beyond the split's range) are formed again in FP32.
 #pragma once
@@ -32,19 +31,23 @@ using product::Groups;
 constexpr int BM = 128, BN = 64, KB = 32, NT = 640;
 constexpr int SEG = 256 / KB;              // k-blocks of an accumulation
 constexpr int A_BYTES = BM * KB * 4, B_PART = BN * KB * 2, B_BYTES = 3 * B_PART;
-constexpr uint32_t ACC_COLS = 3 * BN, A_COL0 = 2 * ACC_COLS, A_COLS = 3 * KB / 2;
+constexpr uint32_t ACC_COLS = 2 * BN, A_COL0 = 2 * ACC_COLS, A_COLS = 3 * KB / 2;
+constexpr int A_SLOTS = 4;                 // of tensor memory: 2 x 128 columns of accumulators, 4 x 48 of A's parts
 // What a K = 16 step's truncation costs on average, of the sum: measured 0.18 to 0.21 x 2^-24 with operands of both signs, 0.27 to 0.40 with those of
 // one.  Given back with the small parts.  Errors (2-norm, 1e-8; torch's FP32 products, this without the gain, this) at k = 64, 128, 256: both signs
 // 14.5, 7.1, 5.1; 20.3, 12.1, 7.9; 28.8, 22.9, 14.4; one sign 12.2, 9.1, 5.0; 17.5, 17.9, 8.6; 24.7, 38.8, 15.3.
 constexpr float GAIN = 0.27f / 16777216.f;
 
 template <bool SLOPE> struct Cfg {
-  static constexpr int STAGES = SLOPE ? 3 : 4, STAGE_BYTES = SLOPE ? 2 * A_BYTES : A_BYTES;
-  static constexpr int SLOTS = SLOPE ? 7 : 10, SLABS = 8 * 4096;
-  static constexpr int BARRIERS = 2 * STAGES + 2 * 2 + 2 * SLOTS + 2 * 2;
-  static constexpr int FIXED = 1024 + SLOTS * B_BYTES + STAGES * STAGE_BYTES + SLABS + BARRIERS * 8 + 16;
-  static constexpr int smem(int experts) { return FIXED + (experts + 1) * 4; }
-  static_assert(FIXED + 1025 * 4 <= 227 * 1024, "shared memory of one CTA");
+  // Even: a stage then always belongs to the same set of split warps, which sees each of its phases (a set that saw every other one could take
+  // the parity of a phase long past for its own).
+  static constexpr int STAGES = SLOPE ? 2 : 4, STAGE_BYTES = SLOPE ? 2 * A_BYTES : A_BYTES;
+  static constexpr int SLABS = SLOPE ? 8 * 4096 : 8 * 8192;       // forward: values and slopes
+  static constexpr int MOST_SLOTS = 16;
+  static constexpr int BARRIERS = 2 * STAGES + 2 * A_SLOTS + 2 * MOST_SLOTS + 2 * 2;
+  static constexpr int smem(int slots, int experts) { return 1024 + slots * B_BYTES + STAGES * STAGE_BYTES + SLABS + BARRIERS * 8 + 8 * 128 + 16 + (experts + 1) * 4; }
+  // as many of the weights' blocks as an SM holds: 8 forward, 10 for grad_x, one less with more than about 150 experts
+  static constexpr int slots(int experts) { return (227 * 1024 - smem(0, experts)) / B_BYTES < MOST_SLOTS ? (227 * 1024 - smem(0, experts)) / B_BYTES : MOST_SLOTS; }
 };
 
 __device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src, bool there) {
@@ -168,17 +171,9 @@ template <bool FORWARD> __global__ void __launch_bounds__(256) split_weights_ker
   store_weights<FORWARD, 256>(out + (size_t)blockIdx.x * B_BYTES, threadIdx.x, v);
 }
 
-// sum_k a[k] (d[k]) b[k * stride] with FP32's own products
-__device__ __noinline__ float sum_fp32(const float* a, const float* d, const float* b, int K, int stride) {
-  float v = 0.f;
-#pragma unroll 1
-  for (int k = 0; k < K; ++k) v = fmaf(d ? a[k] * d[k] : a[k], b[(size_t)k * stride], v);
-  return v;
-}
-
-template <int ACT> __device__ __noinline__ void wild(float4& v, float4& d) {
-  v.x = product::activate<ACT>(v.x, d.x); v.y = product::activate<ACT>(v.y, d.y);
-  v.z = product::activate<ACT>(v.z, d.z); v.w = product::activate<ACT>(v.w, d.w);
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, int column, int row, const void* src) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(column), "r"(0), "r"(row), "r"(smem_u32(src))
+               : "memory");
 }
 
 struct Args {
@@ -186,37 +181,115 @@ struct Args {
   const float *A, *slope, *W, *bias, *residual;
   const unsigned char* split;         // the weights' blocks where they do not stay in shared memory
   float *C, *slope_out;
-  int K, N;
+  int K, N, slots;                    // slots of the weights' blocks
   bool a_wide, w_wide, c_wide;        // 16-byte accesses of A (and slope), of W, of everything shaped like C (and bias)
   int* status;
 };
 
+// a sum of row r (of all) and column n of expert e that is not finite, again with FP32's own products
+template <bool FORWARD, bool SLOPE> __device__ __noinline__ float again(const Args& p, int e, size_t r, int n, float v) {
+  if (fabsf(v) <= 3.402823466e38f) return v;
+  const float *a = p.A + r * p.K, *d = SLOPE ? p.slope + r * p.K : nullptr, *b = p.W + (size_t)e * p.N * p.K + (FORWARD ? (size_t)n * p.K : (size_t)n);
+  v = 0.f;
+#pragma unroll 1
+  for (int k = 0; k < p.K; ++k) v = fmaf(SLOPE ? a[k] * d[k] : a[k], b[FORWARD ? (size_t)k : (size_t)k * p.N], v);
+  return v;
+}
+// 16-byte chunk j of row r in a slab of 32 rows and 32 columns (what a TMA store with 128-byte swizzle takes)
+__device__ __forceinline__ int slab_at(int r, int j) { return r * 128 + ((j ^ (r & 7)) << 4); }
+
+// Values of 16 columns of this thread's row whose sums, in the slab, are not all finite.  Apart from the kernel and with nothing handed back:
+// values whose addresses a call takes would live in memory for good.
+template <bool FORWARD, bool SLOPE, int ACT>
+__device__ __noinline__ void wild_row(const Args& p, int e, size_t row, int n, int h, unsigned char* slab, unsigned char* slopes) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  for (int j = 0; j < 16 && n + j < p.N; ++j) {
+    const int at = slab_at(lane, h * 4 + (j >> 2)) + (j & 3) * 4;
+    float d = 1.f, v = again<FORWARD, SLOPE>(p, e, row, n + j, *reinterpret_cast<const float*>(slab + at));
+    if (FORWARD) {
+      v = product::activate<ACT>(p.bias ? v + p.bias[(size_t)e * p.N + n + j] : v, d);
+      if (p.residual) v += p.residual[row * p.N + n + j];
+      if (ACT != product::kIdentity && p.slope_out) *reinterpret_cast<float*>(slopes + at) = d;
+    }
+    *reinterpret_cast<float*>(slab + at) = v;
+  }
+}
+
+// 16 values from `src`, of which `count` are there
+__device__ __forceinline__ void load_16(const float* src, int count, bool wide, float2 (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (wide) { if (4 * i < count) x = *reinterpret_cast<const float4*>(src + 4 * i); }
+    else {
+      if (4 * i < count) x.x = src[4 * i];
+      if (4 * i + 1 < count) x.y = src[4 * i + 1];
+      if (4 * i + 2 < count) x.z = src[4 * i + 2];
+      if (4 * i + 3 < count) x.w = src[4 * i + 3];
+    }
+    v[2 * i] = make_float2(x.x, x.y);
+    v[2 * i + 1] = make_float2(x.z, x.w);
+  }
+}
+__device__ __forceinline__ void store_16(float* dst, int count, bool wide, const float2 (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (wide) { if (4 * i < count) *reinterpret_cast<float4*>(dst + 4 * i) = make_float4(v[2 * i].x, v[2 * i].y, v[2 * i + 1].x, v[2 * i + 1].y); }
+    else {
+      if (4 * i < count) dst[4 * i] = v[2 * i].x;
+      if (4 * i + 1 < count) dst[4 * i + 1] = v[2 * i].y;
+      if (4 * i + 2 < count) dst[4 * i + 2] = v[2 * i + 1].x;
+      if (4 * i + 3 < count) dst[4 * i + 3] = v[2 * i + 1].y;
+    }
+  }
+}
+// A slab's rows, without TMA: where the tile ends inside the tensor (another expert's rows follow), or its rows are not 16-byte aligned.
+__device__ __forceinline__ void store_slab(float* C, size_t row0, int rows, int n0, int N, bool wide, const unsigned char* slab) {
+  const int lane = threadIdx.x & 31;
+  if (wide) {
+    const int n = n0 + (lane & 7) * 4;
+#pragma unroll 2
+    for (int r = lane >> 3; r < 32; r += 4)
+      if (r < rows && n < N) *reinterpret_cast<float4*>(C + (row0 + r) * N + n) = *reinterpret_cast<const float4*>(slab + slab_at(r, lane & 7));
+  } else {
+    const int n = n0 + lane;
+#pragma unroll 4
+    for (int r = 0; r < 32; ++r)
+      if (r < rows && n < N) C[(row0 + r) * N + n] = *reinterpret_cast<const float*>(slab + slab_at(r, lane >> 2) + (lane & 3) * 4);
+  }
+}
+
 template <bool FORWARD, bool SLOPE, int ACT>
 __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap tmA,
-                                                           const __grid_constant__ CUtensorMap tmSlope) {
+                                                           const __grid_constant__ CUtensorMap tmSlope, const __grid_constant__ CUtensorMap tmC,
+                                                           const __grid_constant__ CUtensorMap tmD) {
   using C_ = Cfg<SLOPE>;
-  constexpr int STAGES = C_::STAGES, SLOTS = C_::SLOTS;
+  constexpr int STAGES = C_::STAGES;
+  const int slots = p.slots;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  unsigned char* a_raw = smem + SLOTS * B_BYTES;
+  unsigned char* a_raw = smem + (size_t)slots * B_BYTES;
   unsigned char* slabs = a_raw + STAGES * C_::STAGE_BYTES;
   uint64_t* a_full = reinterpret_cast<uint64_t*>(slabs + C_::SLABS);     // [STAGES] a raw k-block has landed
   uint64_t* a_empty = a_full + STAGES;                                   // [STAGES] it has been split
-  uint64_t* s_full = a_empty + STAGES;                                   // [2] its parts are in tensor memory
-  uint64_t* s_empty = s_full + 2;                                        // [2] the MMAs have read them
-  uint64_t* b_full = s_empty + 2;                                        // [SLOTS]
-  uint64_t* b_empty = b_full + SLOTS;                                    // [SLOTS]
-  uint64_t* acc_full = b_empty + SLOTS;                                  // [2]
+  uint64_t* s_full = a_empty + STAGES;                                   // [A_SLOTS] its parts are in tensor memory
+  uint64_t* s_empty = s_full + A_SLOTS;                                  // [A_SLOTS] the MMAs have read them
+  uint64_t* b_full = s_empty + A_SLOTS;                                        // [slots]
+  uint64_t* b_empty = b_full + C_::MOST_SLOTS;                           // [slots]
+  uint64_t* acc_full = b_empty + C_::MOST_SLOTS;                                  // [2]
   uint64_t* acc_empty = acc_full + 2;                                    // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  float* biases = reinterpret_cast<float*>(acc_empty + 2);               // [8][32] of the epilogue's warps
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(biases + 8 * 32);
   int* tiles = reinterpret_cast<int*>(tmem_slot + 4);                    // [experts + 1]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, K = p.K, N = p.N, X = p.groups.experts;
   int* status = p.status;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&a_full[s], p.a_wide ? 1 : 32); mbar_init(&a_empty[s], 4); }
-    for (int s = 0; s < SLOTS; ++s) { mbar_init(&b_full[s], p.split ? 1 : 8); mbar_init(&b_empty[s], 1); }
-    for (int s = 0; s < 2; ++s) { mbar_init(&s_full[s], 4); mbar_init(&s_empty[s], 1); mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 8); }
+    for (int s = 0; s < slots; ++s) { mbar_init(&b_full[s], p.split ? 1 : 8); mbar_init(&b_empty[s], 1); }
+    for (int s = 0; s < A_SLOTS; ++s) { mbar_init(&s_full[s], 4); mbar_init(&s_empty[s], 1); }
+    for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 8); }
     mbar_fence_init();
   }
   if (warp == 1) tmem_alloc(tmem_slot, 512);
@@ -244,7 +317,7 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
   __syncthreads();
   const uint32_t tmem = *tmem_slot;
   const int n_tiles = (N + BN - 1) / BN, n_kb = (K + KB - 1) / KB;
-  const bool resident = p.split == nullptr;        // n_kb <= SLOTS then
+  const bool resident = p.split == nullptr;        // n_kb <= slots then
   const long long units = (long long)tiles[X] * n_tiles;
   const int u0 = (int)(units * blockIdx.x / gridDim.x), u1 = (int)(units * (blockIdx.x + 1) / gridDim.x);
 
@@ -289,65 +362,70 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
       cp_async_wait_all();
     } else if (warp == 1) {
       // ------------------------------------------------------------------ MMAs (whole warp, one elected lane)
-      const uint32_t idesc1 = wg::idesc_bf16_m128(3 * BN), idesc2 = wg::idesc_bf16_m128(2 * BN), idesc3 = wg::idesc_bf16_m128(BN);
+      const uint32_t idesc2 = wg::idesc_bf16_m128(2 * BN), idesc1 = wg::idesc_bf16_m128(BN);
       const uint32_t tm = uniform(tmem);
       const uint64_t desc0 = wg::desc_sw64(uniform(smem_u32(smem)));
-      int it = 0, lt = 0, run = 0;         // lt: accumulations, run: number of the run's first block
+      int it = 0, lt = 0, run = 0, run_phase = 0;         // lt: accumulations; run, run_phase: slot of the run's first block and its parity
       for (int u = u0; u < u1; ++u) {
         const bool ends = !resident || uniform((uint32_t)w.run_ends(u + 1 == u1));
+        int bs = run;
+        uint32_t bp = run_phase;
         for (int k0 = 0; k0 < n_kb; k0 += SEG, ++lt) {
           const int buf = lt & 1, k1 = min(n_kb, k0 + SEG);
           mbar_wait(&acc_empty[buf], ((lt >> 1) & 1u) ^ 1u, status);
           const uint32_t d = tm + (uint32_t)buf * ACC_COLS;
           for (int kb = k0; kb < k1; ++kb, ++it) {
-            const int fill = run + kb, bs = fill % SLOTS, slot = it & 1;
-            mbar_wait(&b_full[bs], (fill / SLOTS) & 1u, status);
-            mbar_wait(&s_full[slot], (it >> 1) & 1u, status);
+            const int slot = it % A_SLOTS;
+            mbar_wait(&b_full[bs], bp, status);
+            mbar_wait(&s_full[slot], (it / A_SLOTS) & 1u, status);
             __syncwarp();
             tc_fence_after();
             const uint32_t a = tm + A_COL0 + (uint32_t)(slot * A_COLS);
             const uint64_t b = desc_at(desc0, (uint32_t)(bs * B_BYTES));
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
-              const uint64_t bk = desc_at(b, (uint32_t)(ks * 32));
-              warp_mma_bf16_a_tmem(d, a + (uint32_t)(ks * 8), bk, idesc1, kb > k0 || ks ? 1u : 0u);
-              warp_mma_bf16_a_tmem(d + BN, a + (uint32_t)(KB / 2 + ks * 8), bk, idesc2, 1u);
-              warp_mma_bf16_a_tmem(d + 2 * BN, a + (uint32_t)(KB + ks * 8), bk, idesc3, 1u);
+              const uint64_t w1 = desc_at(b, (uint32_t)(ks * 32)), w2 = desc_at(w1, B_PART), w3 = desc_at(w1, 2 * B_PART);
+              const uint32_t v1 = a + (uint32_t)(ks * 8), v2 = v1 + KB / 2, v3 = v1 + KB;
+              warp_mma_bf16_a_tmem(d, v1, w1, idesc2, kb > k0 || ks ? 1u : 0u);
+              warp_mma_bf16_a_tmem(d + BN, v1, w3, idesc1, 1u);
+              warp_mma_bf16_a_tmem(d + BN, v2, w1, idesc1, 1u);
+              warp_mma_bf16_a_tmem(d + BN, v2, w2, idesc1, 1u);
+              warp_mma_bf16_a_tmem(d + BN, v3, w1, idesc1, 1u);
             }
             warp_mma_commit(&s_empty[slot]);
             if (ends) warp_mma_commit(&b_empty[bs]);
+            if (++bs == slots) { bs = 0; bp ^= 1u; }
           }
           warp_mma_commit(&acc_full[buf]);
         }
-        if (ends) run += n_kb;
+        if (ends) { run = bs; run_phase = bp; }
         w.next();
       }
     } else if (warp < 4) {
       // ------------------------------------------------------------------ the weights' parts
       const int t = threadIdx.x - 64;
-      int fill = 0;
+      int slot = resident ? n_kb % slots : 0;        // the first ones are split by the epilogue's warps
+      uint32_t phase = resident && n_kb == slots ? 1u : 0u;
+      auto next = [&] { if (++slot == slots) { slot = 0; phase ^= 1u; } };
       for (int u = u0; u < u1; ++u, w.next()) {
         if (!resident) {
           if (t == 0) {
             const unsigned char* src = p.split + ((size_t)w.e * n_tiles + w.n) * n_kb * B_BYTES;
-            for (int kb = 0; kb < n_kb; ++kb, ++fill) {
-              const int slot = fill % SLOTS;
-              mbar_wait(&b_empty[slot], ((fill / SLOTS) & 1u) ^ 1u, status);
+            for (int kb = 0; kb < n_kb; ++kb, next()) {
+              mbar_wait(&b_empty[slot], phase ^ 1u, status);
               mbar_arrive_expect_tx(&b_full[slot], (uint32_t)B_BYTES);
               bulk_g2s(smem + (size_t)slot * B_BYTES, src + (size_t)kb * B_BYTES, (uint32_t)B_BYTES, &b_full[slot]);
             }
           }
           continue;
         }
-        if (u == u0) fill += n_kb;                 // the first ones are split by the epilogue's warps
         if (u == u0 || !w.run_begins(false)) continue;
         const float* W = p.W + (size_t)w.e * N * K;
         float v[32], ahead[32];
         load_weights<FORWARD, 64>(W, w.n * BN, N, K, 0, t, p.w_wide, v);
-        for (int kb = 0; kb < n_kb; ++kb, ++fill) {
+        for (int kb = 0; kb < n_kb; ++kb, next()) {
           if (kb + 1 < n_kb) load_weights<FORWARD, 64>(W, w.n * BN, N, K, kb + 1, t, p.w_wide, ahead);
-          const int slot = fill % SLOTS;
-          mbar_wait(&b_empty[slot], ((fill / SLOTS) & 1u) ^ 1u, status);
+          mbar_wait(&b_empty[slot], phase ^ 1u, status);
           store_weights<FORWARD, 64>(smem + (size_t)slot * B_BYTES, t, v);
           fence_async_smem();
           __syncwarp();
@@ -358,15 +436,13 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
       }
     } else if (warp < 12) {
       // ------------------------------------------------------------------ split A into tensor memory
-      const int row = (warp & 3) * 32 + lane, slot = (warp - 4) >> 2;
-      const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + A_COL0 + (uint32_t)(slot * A_COLS);
+      const int row = (warp & 3) * 32 + lane, set = (warp - 4) >> 2;
+      const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + A_COL0;
       const int total = (u1 - u0) * n_kb;
-      for (int it = slot; it < total; it += 2) {
-        const int s = it % STAGES;
-        // The slot first: with block it - 2 multiplied, the other warps have passed the stage's last phase (it - STAGES), and its parity
-        // cannot be taken for this block's.
-        mbar_wait(&s_empty[slot], ((it >> 1) & 1u) ^ 1u, status);
+      for (int it = set; it < total; it += 2) {
+        const int s = it % STAGES, slot = it % A_SLOTS;
         mbar_wait(&a_full[s], (it / STAGES) & 1u, status);
+        mbar_wait(&s_empty[slot], ((it / A_SLOTS) & 1u) ^ 1u, status);
         __syncwarp();
         tc_fence_after();
         const unsigned char* st = a_raw + (size_t)s * C_::STAGE_BYTES + row * 128;
@@ -385,7 +461,7 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
             wg::split_pair(make_float2(v.z, v.w), q[0][2 * j + 1], q[1][2 * j + 1], q[2][2 * j + 1]);
           }
 #pragma unroll
-          for (int e = 0; e < 3; ++e) wg::tmem_st_8(lanes + (uint32_t)(e * (KB / 2) + ks * 8), q[e]);
+          for (int e = 0; e < 3; ++e) wg::tmem_st_8(lanes + (uint32_t)(slot * A_COLS + e * (KB / 2) + ks * 8), q[e]);
         }
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         tc_fence_before();
@@ -394,7 +470,7 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
         if (lane == 0) { mbar_arrive(&s_full[slot]); mbar_arrive(&a_empty[s]); }
       }
     } else {
-      // ------------------------------------------------------------------ epilogue: 32 rows and 32 columns to a warp
+      // ------------------------------------------------------------------ epilogue: thread = row = TMEM lane, 16 columns at a time, 32 to a slab
       if (resident) {
         const int t = threadIdx.x - 384;
         const float* W = p.W + (size_t)w.e * N * K;
@@ -414,117 +490,118 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
         }
       }
       const int quarter = warp & 3, half = (warp - 12) >> 2;
-      unsigned char* slab = slabs + (size_t)(warp - 12) * 4096;      // 16-byte chunk j of row r at j ^ (r & 7)
+      unsigned char* slab = slabs + (size_t)(warp - 12) * (SLOPE ? 4096 : 8192);
+      unsigned char* slopes = slab + 4096;
+      float* bias = biases + (warp - 12) * 32;
       const uint32_t cols = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 32);
       int lt = 0;
       for (int u = u0; u < u1; ++u, w.next()) {
-        const int nh = w.n * BN + half * 32;
         const long long begin = p.groups.first(w.e), left = p.groups.first(w.e + 1) - begin - (long long)w.m * BM;
-        const int rows = (int)(left < BM ? left : BM) - quarter * 32;      // of this warp
+        const int rows = (int)(left < BM ? left : BM) - quarter * 32, n0 = w.n * BN + half * 32;      // of this warp
         const size_t row0 = (size_t)(begin + (long long)w.m * BM + quarter * 32);
-        // wide: four columns, eight rows a thread; else one column, all rows
-        const int c = p.c_wide ? (lane & 7) * 4 : lane, n = nh + c;
-        const bool column = n < N;
-        float4 bias = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (FORWARD && p.bias && column) {
-          const float* b = p.bias + (size_t)w.e * N + n;
-          if (p.c_wide) bias = *reinterpret_cast<const float4*>(b); else bias.x = *b;
-        }
+        const bool mine = lane < rows;
+        if (FORWARD && w.run_begins(u == u0)) bias[lane] = p.bias && n0 + lane < N ? p.bias[(size_t)w.e * N + n0 + lane] : 0.f;
         for (int k0 = 0; k0 < n_kb; k0 += SEG, ++lt) {
           const int buf = lt & 1;
-          const bool last = k0 + SEG >= n_kb;
           const float gain = GAIN * (float)((min(K, (k0 + SEG) * KB) - k0 * KB + 15) / 16);
+          if (lane == 0) bulk_wait_read<0>();      // the slabs' last stores have read them
           mbar_wait(&acc_full[buf], (lt >> 1) & 1u, status);
-          __syncwarp();
-          tc_fence_after();
-#pragma unroll
+          // One copy of this code for both halves, and the warp together all through it: it is bound by the instructions of two warps to a
+          // scheduler, which wait for their code where it is long.
+#pragma unroll 1
           for (int h = 0; h < 2; ++h) {
-            uint32_t x[16], y[16], z[16];
+            __syncwarp();
+            tc_fence_after();
+            uint32_t x[16], y[16];
             const uint32_t at = cols + (uint32_t)buf * ACC_COLS + (uint32_t)(h * 16);
             tmem_ld_16_begin(at, x);
             tmem_ld_16_begin(at + BN, y);
-            tmem_ld_16_begin(at + 2 * BN, z);
             tmem_ld_wait(x);
             tmem_ld_wait(y);
-            tmem_ld_wait(z);
+            float2 v[8], sum = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              float2 o[2];
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const int q = 4 * j + 2 * i;
-                auto two = [&](const uint32_t (&r)[16]) { return make_float2(__uint_as_float(r[q]), __uint_as_float(r[q + 1])); };
-                o[i] = vmul(vadd(two(x), vfma(two(x), make_float2(gain, gain), vadd(two(y), two(z)))), make_float2(wg::UNSCALE, wg::UNSCALE));
-              }
-              *reinterpret_cast<float4*>(slab + lane * 128 + (((h * 4 + j) ^ (lane & 7)) << 4)) = make_float4(o[0].x, o[0].y, o[1].x, o[1].y);
+            for (int i = 0; i < 8; ++i) {
+              const float2 large = make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
+              v[i] = vadd(large, vfma(large, make_float2(gain, gain), make_float2(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1]))));
             }
+            float scale = wg::UNSCALE;
+            if (n_kb > SEG) {                        // the sum so far, which this thread left where its result goes
+              float* C = p.C + (row0 + lane) * N + n0 + h * 16;
+              if (k0 > 0) {
+                float2 before[8];
+                load_16(C, mine ? N - n0 - h * 16 : 0, p.c_wide, before);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = vfma(v[i], make_float2(scale, scale), before[i]);
+                scale = 1.f;
+              }
+              if (k0 + SEG < n_kb) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = vmul(v[i], make_float2(scale, scale));
+                store_16(C, mine ? N - n0 - h * 16 : 0, p.c_wide, v);
+                continue;
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum = vadd(sum, v[i]);
+            if (__any_sync(0xffffffffu, mine && !(fabsf(sum.x + sum.y) <= 3.402823466e38f))) {      // a sum may not be finite
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<float4*>(slab + slab_at(lane, h * 4 + j)) = make_float4(v[2 * j].x * scale, v[2 * j].y * scale, v[2 * j + 1].x * scale, v[2 * j + 1].y * scale);
+              if (mine) wild_row<FORWARD, SLOPE, ACT>(p, w.e, row0 + lane, n0 + h * 16, h, slab, slopes);
+              continue;
+            }
+            if (FORWARD) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float4 b = *reinterpret_cast<const float4*>(bias + h * 16 + 4 * j);
+                v[2 * j] = vfma(v[2 * j], make_float2(scale, scale), make_float2(b.x, b.y));
+                v[2 * j + 1] = vfma(v[2 * j + 1], make_float2(scale, scale), make_float2(b.z, b.w));
+              }
+              if (ACT != product::kIdentity) {
+                float2 d[8];
+                const bool keep = p.slope_out != nullptr;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = product::activate<ACT>(v[i], keep, d[i]);
+                if (keep) {
+#pragma unroll
+                  for (int j = 0; j < 4; ++j)
+                    *reinterpret_cast<float4*>(slopes + slab_at(lane, h * 4 + j)) = make_float4(d[2 * j].x, d[2 * j].y, d[2 * j + 1].x, d[2 * j + 1].y);
+                }
+              }
+              if (p.residual) {
+                float2 res[8];
+                load_16(p.residual + (row0 + lane) * N + n0 + h * 16, mine ? N - n0 - h * 16 : 0, p.c_wide, res);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = vadd(v[i], res[i]);
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[i] = vmul(v[i], make_float2(scale, scale));
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              *reinterpret_cast<float4*>(slab + slab_at(lane, h * 4 + j)) = make_float4(v[2 * j].x, v[2 * j].y, v[2 * j + 1].x, v[2 * j + 1].y);
           }
           tc_fence_before();
+          fence_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(&acc_empty[buf]);
-          // a sum that is not finite, again in FP32
-          auto again = [&](float v, int r, int m) {
-            if (fabsf(v) <= 3.402823466e38f) return v;
-            return sum_fp32(p.A + (row0 + r) * K, SLOPE ? p.slope + (row0 + r) * K : nullptr,
-                            p.W + (size_t)w.e * N * K + (FORWARD ? (size_t)m * K : (size_t)m), K, FORWARD ? 1 : N);
-          };
-          if (column && p.c_wide) {
-            const float* from = reinterpret_cast<const float*>(slab + (lane >> 3) * 128);
-#pragma unroll 4
-            for (int i = 0; i < 8; ++i) {
-              const int r = (lane >> 3) + i * 4;
-              if (r >= rows) break;
-              const size_t o = (row0 + r) * N + n;
-              float4 v = *reinterpret_cast<const float4*>(from + i * 128 + (((lane & 7) ^ (r & 7)) << 2));
-              if (k0 > 0) {
-                const float4 before = *reinterpret_cast<const float4*>(p.C + o);
-                v.x += before.x; v.y += before.y; v.z += before.z; v.w += before.w;
-              }
-              if (last) {
-                const float2 z0 = make_float2(v.x + bias.x, v.y + bias.y), z1 = make_float2(v.z + bias.z, v.w + bias.w);
-                float4 d;
-                // larger than kTame, infinite or not a number: in magnitude bits
-                auto bits = [](float x) { return __float_as_uint(x) & 0x7fffffffu; };
-                constexpr float most = ACT == product::kIdentity || ACT == product::kAbs ? 3.402823466e38f : product::kTame;
-                if (max(max(bits(z0.x), bits(z0.y)), max(bits(z1.x), bits(z1.y))) <= __float_as_uint(most)) {
-                  float2 d0, d1;
-                  const float2 y0 = FORWARD ? product::activate_tame<ACT>(z0, p.slope_out != nullptr, d0) : z0;
-                  const float2 y1 = FORWARD ? product::activate_tame<ACT>(z1, p.slope_out != nullptr, d1) : z1;
-                  v = make_float4(y0.x, y0.y, y1.x, y1.y);
-                  d = make_float4(d0.x, d0.y, d1.x, d1.y);
-                } else {
-                  v.x = again(v.x, r, n) + bias.x; v.y = again(v.y, r, n + 1) + bias.y; v.z = again(v.z, r, n + 2) + bias.z; v.w = again(v.w, r, n + 3) + bias.w;
-                  if (FORWARD) wild<ACT>(v, d);
-                }
-                if (FORWARD && p.residual) {
-                  const float4 res = *reinterpret_cast<const float4*>(p.residual + o);
-                  v.x += res.x; v.y += res.y; v.z += res.z; v.w += res.w;
-                }
-                if (FORWARD && p.slope_out) *reinterpret_cast<float4*>(p.slope_out + o) = d;
-              }
-              *reinterpret_cast<float4*>(p.C + o) = v;
+          if (k0 + SEG < n_kb) continue;
+          const bool keep = FORWARD && ACT != product::kIdentity && p.slope_out;
+          if (p.c_wide && (rows >= 32 || row0 + rows == (size_t)p.groups.rows)) {
+            if (lane == 0 && rows > 0 && n0 < N) {
+              tma_store_3d(&tmC, n0, (int)row0, slab);
+              if (keep) tma_store_3d(&tmD, n0, (int)row0, slopes);
+              bulk_commit();
             }
-          } else if (column) {
-#pragma unroll 4
-            for (int r = 0; r < 32; ++r) {
-              if (r >= rows) break;
-              const size_t o = (row0 + r) * N + n;
-              float d, v = *reinterpret_cast<const float*>(slab + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
-              if (k0 > 0) v += p.C[o];
-              if (last) {
-                const float res = FORWARD && p.residual ? p.residual[o] : 0.f;
-                v = again(v, r, n);
-                if (FORWARD) {
-                  v = product::activate<ACT>(v + bias.x, d) + res;
-                  if (p.slope_out) p.slope_out[o] = d;
-                }
-              }
-              p.C[o] = v;
-            }
+          } else {
+            store_slab(p.C, row0, rows, n0, N, p.c_wide, slab);
+            if (keep) store_slab(p.slope_out, row0, rows, n0, N, p.c_wide, slopes);
           }
           __syncwarp();
         }
       }
+      if (lane == 0) bulk_wait_all<0>();
     }
   }
   // rows of no expert
@@ -532,7 +609,7 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
     const size_t first = (size_t)p.groups.first(X) * N, end = (size_t)p.groups.rows * N;
     for (size_t i = first + (size_t)blockIdx.x * NT + threadIdx.x; i < end; i += (size_t)gridDim.x * NT) {
       p.C[i] = 0.f;
-      if (FORWARD && p.slope_out) p.slope_out[i] = 0.f;
+      if (FORWARD && ACT != product::kIdentity && p.slope_out) p.slope_out[i] = 0.f;
     }
   }
   tc_fence_before();
