@@ -21,51 +21,51 @@ fasteq_product_problem problem(const Tensor& x, const Tensor& w, int64_t inner, 
 }
 const int32_t* offsets_of(const Tensor& offsets) { return offsets.defined() ? offsets.const_data_ptr<int32_t>() : nullptr; }
 
-Tensor scratch_of(const fasteq_product_problem& p, bool grad_x, const Tensor& like) {
+Tensor scratch_of(const fasteq_product_problem& p, bool backward, const Tensor& like) {
   int64_t need = 0;
-  check(core.product_scratch(&p, grad_x, &need), "fasteq_product_scratch", core.last_cuda_error);
+  check(core.product_scratch(&p, backward, &need), "fasteq_product_scratch", core.last_cuda_error);
   return need ? at::empty({need}, like.options().dtype(at::kByte)) : Tensor();
 }
+int64_t bytes_of(const Tensor& t) { return t.defined() ? t.numel() : 0; }
+// dense, and at an address the tensor-core kernels take
+Tensor dense_rows(const Tensor& t) {
+  if (!t.defined()) return t;
+  const Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.const_data_ptr()) % 16 ? c.clone() : c;
+}
 
+// slope: receives act'(z) as the kernels keep it
 Tensor run_forward(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& residual, const Tensor& offsets, int64_t inner, int64_t act,
                    Tensor* slope) {
   c10::cuda::CUDAGuard guard(x.device());
-  const Tensor xc = x.contiguous(), wc = w.contiguous(), bc = defined_contiguous(bias), rc = defined_contiguous(residual);
+  const Tensor xc = dense_rows(x), wc = w.contiguous(), bc = defined_contiguous(bias), rc = defined_contiguous(residual);
   const auto p = problem(xc, wc, inner, act);
-  Tensor y = at::empty({xc.size(0), wc.size(1)}, xc.options());
-  if (slope) *slope = at::empty_like(y);
+  const int64_t rows = xc.size(0), n = wc.size(1);
+  Tensor y = at::empty({rows, n}, xc.options());
+  if (slope) *slope = at::empty({rows, p.dtype == FASTEQ_F32 ? (n + 3) & ~(int64_t)3 : n}, xc.options());
   const Tensor scratch = scratch_of(p, false, xc);
   check(core.product_forward(&p, ptr(xc), ptr(wc), ptr(bc), ptr(rc), offsets_of(offsets), mptr(y), slope ? mptr(*slope) : nullptr, mptr(scratch),
-                             scratch.defined() ? scratch.numel() : 0, stream_of(xc)),
+                             bytes_of(scratch), stream_of(xc)),
         "fasteq_product_forward", core.last_cuda_error);
   return y;
 }
 
-Tensor run_dgrad(const Tensor& g, const Tensor& slope, const Tensor& w, const Tensor& offsets, int64_t inner) {
+// The gradients that are asked for, the others undefined.  w [experts, N, K] (only its extents without gx), x may be undefined without gw
+variable_list run_backward(const Tensor& x, at::IntArrayRef shape, const Tensor& w, const Tensor& g, const Tensor& slope, const Tensor& offsets, int64_t inner,
+                           bool need_x, bool need_w, bool need_b) {
   c10::cuda::CUDAGuard guard(g.device());
-  const Tensor gc = g.contiguous(), wc = w.contiguous();
-  const auto p = problem(gc, wc, inner, 0);
-  Tensor gx = at::empty({gc.size(0), wc.size(2)}, gc.options());
+  const Tensor gc = dense_rows(g), xc = dense_rows(x), wc = defined_contiguous(w);
+  fasteq_product_problem p{};
+  p.dtype = gc.scalar_type() == at::kDouble ? FASTEQ_F64 : FASTEQ_F32;
+  p.experts = (int32_t)shape[0]; p.n = (int32_t)shape[1]; p.k = (int32_t)shape[2]; p.inner = (int32_t)inner; p.rows = gc.size(0);
+  Tensor gx = need_x ? at::empty({gc.size(0), shape[2]}, gc.options()) : Tensor();
+  Tensor gw = need_w || need_b ? at::empty(shape, gc.options()) : Tensor();
+  Tensor gb = need_b ? at::empty({shape[0], shape[1]}, gc.options()) : Tensor();
   const Tensor scratch = scratch_of(p, true, gc);
-  check(core.product_dgrad(&p, ptr(gc), ptr(slope), ptr(wc), offsets_of(offsets), mptr(gx), mptr(scratch), scratch.defined() ? scratch.numel() : 0, stream_of(gc)),
-        "fasteq_product_dgrad", core.last_cuda_error);
-  return gx;
-}
-
-// `shape`: the weights'
-Tensor run_wgrad(const Tensor& x, const Tensor& g, const Tensor& slope, const Tensor& offsets, int64_t inner, at::IntArrayRef shape, Tensor* grad_bias) {
-  c10::cuda::CUDAGuard guard(g.device());
-  const Tensor gc = g.contiguous(), xc = x.contiguous();
-  Tensor gw = at::empty(shape, gc.options());
-  const auto p = problem(xc, gw, inner, 0);
-  if (grad_bias) *grad_bias = at::empty({shape[0], shape[1]}, gc.options());
-  int64_t need = 0;
-  check(core.product_wgrad_scratch(&p, &need), "fasteq_product_wgrad_scratch", core.last_cuda_error);
-  Tensor scratch = at::empty({std::max<int64_t>(need, 16)}, gc.options().dtype(at::kByte));
-  check(core.product_wgrad(&p, ptr(xc), ptr(gc), ptr(slope), offsets_of(offsets), mptr(gw), grad_bias ? mptr(*grad_bias) : nullptr, scratch.data_ptr(),
-                           scratch.numel(), stream_of(gc)),
-        "fasteq_product_wgrad", core.last_cuda_error);
-  return gw;
+  check(core.product_backward(&p, ptr(xc), ptr(wc), ptr(gc), ptr(slope), offsets_of(offsets), mptr(gx), mptr(gw), mptr(gb), mptr(scratch), bytes_of(scratch),
+                              stream_of(gc)),
+        "fasteq_product_backward", core.last_cuda_error);
+  return {gx, need_w ? gw : Tensor(), gb};
 }
 
 Tensor product(const Tensor& x, const Tensor& w, const Tensor& offsets, int64_t inner);
@@ -80,8 +80,8 @@ struct Bilinear : torch::autograd::Function<Bilinear> {
     ctx->saved_data["i"] = inner; ctx->saved_data["w"] = which;
     const Tensor o = offsets.value_or(Tensor());
     if (which == 0) return run_forward(a, b, Tensor(), Tensor(), o, inner, kIdentity, nullptr);
-    if (which == 1) return run_dgrad(a, Tensor(), b, o, inner);
-    return run_wgrad(b, a, Tensor(), o, inner, shape, nullptr);
+    if (which == 1) return run_backward(Tensor(), b.sizes(), b, a, Tensor(), o, inner, true, false, false)[0];
+    return run_backward(b, shape, Tensor(), a, Tensor(), o, inner, false, true, false)[1];
   }
   static variable_list backward(AutogradContext* ctx, variable_list go) {
     const auto saved = ctx->get_saved_variables();
@@ -145,11 +145,8 @@ struct Layer : torch::autograd::Function<Layer> {
       if (need_w) gw = product_w(gz, x, o, inner, w.sizes());
       if (need_b) gb = product_w(gz, ones, o, inner, {b.size(0), b.size(1), 1}).squeeze(2);
     } else {
-      if (need_x) gx = run_dgrad(g, slope, w, o, inner);
-      if (need_w || need_b) {
-        gw = run_wgrad(x, g, slope, o, inner, w.sizes(), need_b ? &gb : nullptr);
-        if (!need_w) gw = Tensor();
-      }
+      auto d = run_backward(x, w.sizes(), w, g, slope, o, inner, need_x, need_w, need_b);
+      gx = d[0]; gw = d[1]; gb = d[2];
     }
     return {gx, gw, gb, gr, Tensor(), Tensor(), Tensor(), Tensor()};
   }

@@ -29,7 +29,7 @@ PYBIND11_MODULE(fasteq_front, m) {
     F(eqlinear_pack) F(eqlinear_forward) F(eqlinear_dgrad) F(eqlinear_forward_packed) F(eqlinear_dgrad_packed)
     F(eqlinear_wgrad_scratch) F(eqlinear_wgrad_with) F(gemm_tf32x3_split) F(gemm_tf32x3_presplit)
     F(radial_chain_prepare) F(radial_chain_forward) F(radial_chain_backward) F(edge_geometry_forward) F(edge_geometry_backward)
-    F(product_scratch) F(product_forward) F(product_dgrad) F(product_wgrad_scratch) F(product_wgrad) F(expert_plan_scratch) F(expert_plan) F(expert_gather) F(expert_combine)
+    F(product_scratch) F(product_forward) F(product_backward) F(expert_plan_scratch) F(expert_plan) F(expert_gather) F(expert_combine)
     F(expert_combine_backward) F(silu) F(neighbors_work_bytes) F(neighbors_count) F(neighbors_fill) F(graph_partition) F(graph_partition_edges) F(last_cuda_error)
 #undef F
     raised = failure.release().ptr();

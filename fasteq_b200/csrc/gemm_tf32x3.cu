@@ -971,6 +971,11 @@ int make_map_rows(CUtensorMap* m, const float* base, int width, int rows, long l
                     {(cuuint32_t)box_width, 1u, (cuuint32_t)box_batch}, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
+int make_map_pitched(CUtensorMap* m, const float* base, int width, int pitch, long long rows, uint32_t box_width, uint32_t box_rows) {
+  return encode_map(m, base, {(cuuint64_t)width, 1, (cuuint64_t)rows}, {(cuuint64_t)pitch * 4, (cuuint64_t)pitch * 4}, {box_width, 1, box_rows},
+                    CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
 bool supported(long long M, int a_rows, int K, int P, int N, int c_rows, const void* A, const void* Bt, const void* C) {
   if (M < 1 || K < 4 || N < 4 || (K % 4) || (N % 4)) return false;                 // 16-byte global strides
   if (M > 0x7fffffffLL) return false;

@@ -23,6 +23,8 @@ int make_map(CUtensorMap* m, const float* base, uint64_t d0, uint64_t d1, uint64
              uint64_t stride2_elems, uint32_t b0, uint32_t b1, uint32_t b2);
 // FP32 rows [batch][rows][width], box [box_batch][1][box_width] unswizzled, zero fill
 int make_map_rows(CUtensorMap* m, const float* base, int width, int rows, long long batch, int box_width, int box_batch);
+// FP32 rows [rows][width], `pitch` columns apart, box [box_rows][1][box_width] unswizzled, zero fill
+int make_map_pitched(CUtensorMap* m, const float* base, int width, int pitch, long long rows, uint32_t box_width, uint32_t box_rows);
 }  // namespace tc
 namespace chain {
 int device_status(int* code);   // status word of the radial-chain kernels (read and cleared)

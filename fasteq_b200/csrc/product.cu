@@ -10,6 +10,7 @@
 #include "launch.cuh"
 #include "product.cuh"
 #include "product_tc.cuh"
+#include "product_wgrad_tc.cuh"
 #include "gemm_tf32x3.h"
 
 using namespace fasteq;
@@ -23,7 +24,7 @@ constexpr int TILE = 64, BK = 16, PITCH = TILE + 4, THREADS = 256;
 // else W [K, N] (grad_x: K the layer's outputs, N its inputs).
 template <typename T, bool FORWARD>
 __global__ void __launch_bounds__(THREADS) product_kernel(Groups groups, const T* A, const T* slope, const T* W, const T* bias, const T* residual,
-                                                          int K, int N, int act, T* C, T* slope_out) {
+                                                          int K, int N, int ldd, int act, T* C, T* slope_out) {
   __shared__ __align__(16) T sa[BK][PITCH], sw[BK][PITCH];
   wait_for_previous_kernel();
   long long m0;
@@ -40,7 +41,7 @@ __global__ void __launch_bounds__(THREADS) product_kernel(Groups groups, const T
         const int k = t % 16, m = t / 16 + 16 * i;
         const long long at = (m0 + m) * K + k0 + k;
         T v = T(0);
-        if (m < m_rows && k0 + k < K) v = slope ? A[at] * slope[at] : A[at];
+        if (m < m_rows && k0 + k < K) v = slope ? A[at] * slope[(m0 + m) * ldd + k0 + k] : A[at];
         sa[k][m] = v;
         if (FORWARD) {
           sw[k][m] = n0 + m < N && k0 + k < K ? w[(size_t)(n0 + m) * K + k0 + k] : T(0);
@@ -78,39 +79,37 @@ __global__ void __launch_bounds__(THREADS) product_kernel(Groups groups, const T
         d = T(0);
       }
       C[at] = v;
-      if (FORWARD && slope_out) slope_out[at] = d;
+      if (FORWARD && slope_out) slope_out[(size_t)(m0 + tm + i) * ldd + n] = d;
     }
   }
 }
 
 // ------------------------------------------------------------------------------------------------ weight gradient
-// A chunk of an expert's rows and a tile of its matrix per CTA; the partial sums [chunk][N * K | N] are added by a second kernel in order.
-constexpr int CHUNK_ROWS = 512;
-
+// A chunk of `size` of an expert's rows and a tile of its matrix per CTA.  An expert of one chunk has its sums then; the partial sums [slot][N * K | N]
+// of the others a second kernel adds in order.
 template <typename T>
-__global__ void __launch_bounds__(THREADS) product_wgrad_kernel(Groups groups, const T* X, const T* G, const T* slope, int K, int N, T* partial) {
+__global__ void __launch_bounds__(THREADS) product_wgrad_kernel(Groups groups, const T* X, const T* G, const T* slope, int K, int N, int ldd, int size, T* gw,
+                                                                T* gb, T* partial) {
   __shared__ __align__(16) T sg[BK][PITCH], sx[BK][PITCH];
   wait_for_previous_kernel();
-  long long m0;
-  int m_rows;
-  tile_of<CHUNK_ROWS>(groups, groups.experts, blockIdx.x, &m0, &m_rows);
-  if (m_rows == 0) return;
+  const Chunk c = chunk_of(groups, groups.experts, size, blockIdx.x);
+  if (c.rows == 0) return;
   const int tiles_k = max(1, (K + TILE - 1) / TILE), n0 = ((int)blockIdx.y / tiles_k) * TILE, k0 = ((int)blockIdx.y % tiles_k) * TILE;
   const int t = threadIdx.x, tn = (t / 16) * 4, tk = (t % 16) * 4;
   T sum[4][4] = {}, column = T(0);
-  for (int r0 = 0; r0 < m_rows; r0 += BK) {
+  for (int r0 = 0; r0 < c.rows; r0 += BK) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int c = t % 64, r = t / 64 + 4 * i;
-      const bool there = r0 + r < m_rows;
-      const long long row = m0 + r0 + r;
+      const int col = t % 64, r = t / 64 + 4 * i;
+      const bool there = r0 + r < c.rows;
+      const long long row = c.m0 + r0 + r;
       T g = T(0);
-      if (there && n0 + c < N) {
-        const long long at = row * N + n0 + c;
-        g = slope ? G[at] * slope[at] : G[at];
+      if (there && n0 + col < N) {
+        const long long at = row * N + n0 + col;
+        g = slope ? G[at] * slope[row * ldd + n0 + col] : G[at];
       }
-      sg[r][c] = g;
-      sx[r][c] = there && k0 + c < K ? X[row * K + k0 + c] : T(0);
+      sg[r][col] = g;
+      sx[r][col] = there && k0 + col < K ? X[row * K + k0 + col] : T(0);
     }
     __syncthreads();
 #pragma unroll
@@ -126,33 +125,40 @@ __global__ void __launch_bounds__(THREADS) product_wgrad_kernel(Groups groups, c
     }
     __syncthreads();
   }
-  T* dst = partial + (size_t)blockIdx.x * ((size_t)N * K + N);
+  const size_t nk = (size_t)N * K;
+  const bool only = c.count == 1;
+  T* dst = only ? gw + (size_t)c.e * nk : partial + (size_t)partial_slot(c, size) * (nk + N);
   for (int i = 0; i < 4; ++i)
     for (int j = 0; j < 4; ++j)
       if (n0 + tn + i < N && k0 + tk + j < K) dst[(size_t)(n0 + tn + i) * K + k0 + tk + j] = sum[i][j];
-  if (k0 == 0 && t < TILE && n0 + t < N) dst[(size_t)N * K + n0 + t] = column;
+  if (k0 == 0 && t < TILE && n0 + t < N && (gb || !only)) (only ? gb + (size_t)c.e * N : dst + nk)[n0 + t] = column;
 }
 
-// 32 values of an expert to a CTA, eight threads to each, which take every eighth chunk and are added in order
-template <typename T>
-__global__ void __launch_bounds__(256) product_reduce_kernel(Groups groups, const T* partial, int K, int N, T* gw, T* gb) {
+// Experts of no or of several chunks: 32 values at a time to a CTA, eight threads to each, which take every eighth chunk and are added in order.
+template <typename T> __global__ void __launch_bounds__(256) product_reduce_kernel(Groups groups, const T* partial, int K, int N, int size, T* gw, T* gb) {
   __shared__ T part[8][33];
   wait_for_previous_kernel();
   const int e = blockIdx.y;
-  const size_t nk = (size_t)N * K, all = nk + N, i = (size_t)blockIdx.x * 32 + threadIdx.x;
-  const long long begin = groups.first(e), end = groups.first(e + 1), c0 = begin / CHUNK_ROWS + e, n = (end - begin + CHUNK_ROWS - 1) / CHUNK_ROWS;
-  T s = T(0);
-  if (i < all) {
+  const size_t nk = (size_t)N * K, all = nk + N;
+  const long long begin = groups.first(e), n = (groups.first(e + 1) - begin + size - 1) / size;
+  if (n == 1) return;
+  const T* from = partial + (size_t)(2 * begin / size) * all;
+  for (size_t i0 = (size_t)blockIdx.x * 32; i0 < all; i0 += (size_t)gridDim.x * 32) {
+    const size_t i = i0 + threadIdx.x;
+    T s = T(0);
+    if (i < all) {
 #pragma unroll 4
-    for (long long c = threadIdx.y; c < n; c += 8) s += partial[(size_t)(c0 + c) * all + i];
-  }
-  part[threadIdx.y][threadIdx.x] = s;
-  __syncthreads();
-  if (threadIdx.y == 0 && i < all) {
+      for (long long c = threadIdx.y; c < n; c += 8) s += from[(size_t)c * all + i];
+    }
+    part[threadIdx.y][threadIdx.x] = s;
+    __syncthreads();
+    if (threadIdx.y == 0 && i < all) {
 #pragma unroll
-    for (int j = 1; j < 8; ++j) s += part[j][threadIdx.x];
-    if (i < nk) gw[(size_t)e * nk + i] = s;
-    else if (gb) gb[(size_t)e * N + (i - nk)] = s;
+      for (int j = 1; j < 8; ++j) s += part[j][threadIdx.x];
+      if (i < nk) gw[(size_t)e * nk + i] = s;
+      else if (gb) gb[(size_t)e * N + (i - nk)] = s;
+    }
+    __syncthreads();
   }
 }
 
@@ -167,44 +173,52 @@ int check(const fasteq_product_problem* p, const int32_t* offsets) {
 }
 Groups groups_of(const fasteq_product_problem* p, const int32_t* offsets) { return Groups{offsets, p->experts, p->inner, (long long)p->rows}; }
 
+// columns between the rows of what the forward leaves for the gradients (TMA wants multiples of 16 bytes)
+int slope_pitch(const fasteq_product_problem* p) { return p->dtype == FASTEQ_F32 ? (p->n + 3) & ~3 : p->n; }
+
 template <typename T>
 int forward(const fasteq_product_problem* p, const void* x, const void* w, const void* bias, const void* residual, const int32_t* offsets, void* y,
             void* slope, cudaStream_t s) {
   const dim3 grid((unsigned)tile_numbers<TILE>(p->rows, p->experts + 1), (unsigned)((p->n + TILE - 1) / TILE));
   const cudaError_t e = launch_dependent(product_kernel<T, true>, grid, THREADS, 0, s, groups_of(p, offsets), (const T*)x, (const T*)nullptr, (const T*)w,
-                                         (const T*)bias, (const T*)residual, p->k, p->n, p->act, (T*)y, (T*)slope);
+                                         (const T*)bias, (const T*)residual, p->k, p->n, slope_pitch(p), p->act, (T*)y, (T*)slope);
   return e == cudaSuccess ? FASTEQ_OK : cuda_fail(e);
 }
 template <typename T>
 int dgrad(const fasteq_product_problem* p, const void* g, const void* slope, const void* w, const int32_t* offsets, void* gx, cudaStream_t s) {
   const dim3 grid((unsigned)tile_numbers<TILE>(p->rows, p->experts + 1), (unsigned)((p->k + TILE - 1) / TILE));
   const cudaError_t e = launch_dependent(product_kernel<T, false>, grid, THREADS, 0, s, groups_of(p, offsets), (const T*)g, (const T*)slope, (const T*)w,
-                                         (const T*)nullptr, (const T*)nullptr, p->n, p->k, 0, (T*)gx, (T*)nullptr);
+                                         (const T*)nullptr, (const T*)nullptr, p->n, p->k, slope_pitch(p), 0, (T*)gx, (T*)nullptr);
   return e == cudaSuccess ? FASTEQ_OK : cuda_fail(e);
 }
+// Rows of a chunk: as many as give every SM `per_sm` tiles of rows x matrix.  At least 256: below that a chunk's start and its sums' way out
+// take longer than its rows.
+int chunk_rows(const fasteq_product_problem* p, int tile_n, int tile_k, int per_sm) {
+  const long long tiles = (long long)((p->n + tile_n - 1) / tile_n) * std::max(1, (p->k + tile_k - 1) / tile_k);
+  const long long rows = (p->rows * tiles + 148 * per_sm - 1) / (148 * per_sm);
+  return (int)std::min<long long>(1 << 24, std::max<long long>(256, (rows + 31) / 32 * 32));
+}
+int chunk_rows(const fasteq_product_problem* p, bool tensor_cores) { return tensor_cores ? chunk_rows(p, pwg::TM, pwg::TN, 1) : chunk_rows(p, TILE, TILE, 4); }
+
+template <typename T> int reduce(const fasteq_product_problem* p, const Groups& groups, int size, void* gw, void* gb, void* scratch, cudaStream_t s) {
+  if (p->experts == 1 && p->rows <= size && !groups.offsets) return FASTEQ_OK;
+  const size_t blocks = ((size_t)p->n * p->k + p->n + 31) / 32;
+  const cudaError_t e = launch_dependent(product_reduce_kernel<T>, dim3((unsigned)std::min<size_t>(blocks, std::max(1, 4096 / p->experts)), (unsigned)p->experts), dim3(32, 8),
+                                         0, s, groups, (const T*)scratch, p->k, p->n, size, (T*)gw, (T*)gb);
+  return e == cudaSuccess ? FASTEQ_OK : cuda_fail(e);
+}
+
 template <typename T>
-int wgrad(const fasteq_product_problem* p, const void* x, const void* g, const void* slope, const int32_t* offsets, void* gw, void* gb, void* scratch,
+int wgrad(const fasteq_product_problem* p, int size, const void* x, const void* g, const void* slope, const int32_t* offsets, void* gw, void* gb, void* scratch,
           cudaStream_t s) {
   const Groups groups = groups_of(p, offsets);
   const int tiles = ((p->n + TILE - 1) / TILE) * std::max(1, (p->k + TILE - 1) / TILE);
-  cudaError_t e = cudaSuccess;
-  if (p->rows == 0) {
-    if (p->k > 0) e = cudaMemsetAsync(gw, 0, (size_t)p->experts * p->n * p->k * sizeof(T), s);
-    if (e == cudaSuccess && gb) e = cudaMemsetAsync(gb, 0, (size_t)p->experts * p->n * sizeof(T), s);
-    return e == cudaSuccess ? FASTEQ_OK : cuda_fail(e);
-  }
-  e = launch_dependent(product_wgrad_kernel<T>, dim3((unsigned)tile_numbers<CHUNK_ROWS>(p->rows, p->experts), (unsigned)tiles), THREADS, 0, s, groups, (const T*)x,
-                       (const T*)g, (const T*)slope, p->k, p->n, (T*)scratch);
-  if (e == cudaSuccess)
-    e = launch_dependent(product_reduce_kernel<T>, dim3((unsigned)(((size_t)p->n * p->k + p->n + 31) / 32), (unsigned)p->experts), dim3(32, 8), 0, s, groups,
-                         (const T*)scratch, p->k, p->n, (T*)gw, (T*)gb);
-  return e == cudaSuccess ? FASTEQ_OK : cuda_fail(e);
+  const cudaError_t e = launch_dependent(product_wgrad_kernel<T>, dim3((unsigned)(p->rows / size + p->experts), (unsigned)tiles), THREADS, 0, s, groups, (const T*)x,
+                                         (const T*)g, (const T*)slope, p->k, p->n, slope_pitch(p), size, (T*)gw, (T*)gb, (T*)scratch);
+  return e == cudaSuccess ? reduce<T>(p, groups, size, gw, gb, scratch, s) : cuda_fail(e);
 }
 
-}  // namespace
-
-namespace {
-
+// ------------------------------------------------------------------------------------------------ tensor cores
 bool wide(int extent, std::initializer_list<const void*> pointers) {
   uintptr_t all = 0;
   for (const void* q : pointers) all |= reinterpret_cast<uintptr_t>(q);
@@ -216,13 +230,55 @@ long long most_units(const fasteq_product_problem* p, int K, int N) {
   const long long units = (p->rows / ptc::BM + p->experts) * ((N + ptc::BN - 1) / ptc::BN);
   return units > 0x7fffffffLL || (units / 64 + 1) * ((K + ptc::KB - 1) / ptc::KB) > 0x3fffffffLL ? -1 : units;
 }
+bool on_tensor_cores(const fasteq_product_problem* p) {
+  return p->dtype == FASTEQ_F32 && p->k > 0 && p->n > 0 && p->rows > 0 && p->rows <= 0x7fffffffLL && most_units(p, p->k, p->n) > 0 && most_units(p, p->n, p->k) > 0;
+}
 
-// bytes of the weights split beforehand: none where a CTA keeps them
-int64_t split_bytes(const fasteq_product_problem* p, bool forward) {
-  const int K = forward ? p->k : p->n, N = forward ? p->n : p->k, n_kb = (K + ptc::KB - 1) / ptc::KB;
-  if (p->dtype != FASTEQ_F32 || K == 0 || N == 0 || p->rows == 0 || most_units(p, K, N) < 0) return 0;
-  const int slots = forward ? ptc::Cfg<false>::slots(p->experts) : ptc::Cfg<true>::slots(p->experts);
-  return n_kb <= std::min(slots, ptc::Cfg<false>::slots(p->experts)) ? 0 : (int64_t)p->experts * ((N + ptc::BN - 1) / ptc::BN) * n_kb * ptc::B_BYTES;
+// dst [rows, (columns + 3) & ~3] = src [rows, columns] (times slope), for rows that TMA cannot take as they lie
+__global__ void __launch_bounds__(256) align_rows_kernel(const float* src, const float* slope, int columns, int ldd, long long rows, float* dst) {
+  const int c = threadIdx.x * 4, pitch = (columns + 3) & ~3;
+  wait_for_previous_kernel();
+  for (long long r = (long long)blockIdx.x * blockDim.y + threadIdx.y; r < rows; r += (long long)gridDim.x * blockDim.y)
+    for (int k = c; k < pitch; k += blockDim.x * 4) {
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = k + i < columns ? src[r * columns + k + i] : 0.f;
+        if (slope && k + i < columns) v[i] *= slope[r * ldd + k + i];
+      }
+      *reinterpret_cast<float4*>(dst + r * pitch + k) = make_float4(v[0], v[1], v[2], v[3]);
+    }
+}
+cudaError_t align_rows(const void* src, const void* slope, int columns, int ldd, long long rows, void* dst, cudaStream_t s) {
+  int tx = 1;
+  while (tx * 4 < columns && tx < 32) tx *= 2;
+  const dim3 block((unsigned)tx, (unsigned)(256 / tx));
+  return launch_dependent(align_rows_kernel, (unsigned)std::min<long long>((rows + block.y - 1) / block.y, 148 * 32), block, 0, s, (const float*)src,
+                          (const float*)slope, columns, ldd, rows, (float*)dst);
+}
+
+// A call's scratch: the aligned copies, the weights split beforehand (none where a CTA keeps them), the weight gradient's partial sums.
+struct Scratch {
+  int64_t x = 0, g = 0, split = 0, partial = 0;
+  int64_t total() const { return x + g + split + partial; }
+};
+int64_t round16(int64_t v) { return (v + 15) & ~(int64_t)15; }
+Scratch scratch_of(const fasteq_product_problem* p, bool backward) {
+  Scratch r;
+  const bool tensor = on_tensor_cores(p);
+  const int64_t size = p->dtype == FASTEQ_F32 ? 4 : 8;
+  if (tensor) {
+    const int K = backward ? p->n : p->k, N = backward ? p->k : p->n, n_kb = (K + ptc::KB - 1) / ptc::KB;
+    const int slots = std::min(ptc::Cfg<false>::slots(p->experts), ptc::Cfg<true>::slots(p->experts));
+    if (p->k % 4) r.x = round16(p->rows * ((p->k + 3) & ~3) * size);
+    if (backward && p->n % 4) r.g = round16(p->rows * ((p->n + 3) & ~3) * size);
+    if (n_kb > slots) r.split = (int64_t)p->experts * ((N + ptc::BN - 1) / ptc::BN) * n_kb * ptc::B_BYTES;
+  }
+  if (backward && p->rows > 0) {
+    const int rows = chunk_rows(p, tensor);
+    if (p->rows > rows) r.partial = partial_slots(p->rows, rows) * ((int64_t)p->n * p->k + p->n) * size;
+  }
+  return r;
 }
 
 template <bool FORWARD, bool SLOPE, int ACT>
@@ -231,39 +287,41 @@ int launch_tc(const fasteq_product_problem* p, ptc::Args& a, int sms, const CUte
   const int smem = ptc::Cfg<SLOPE>::smem(a.slots, p->experts);
   cudaError_t e = cudaFuncSetAttribute(ptc::product_tc_kernel<FORWARD, SLOPE, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e == cudaSuccess)
-    e = launch_dependent(ptc::product_tc_kernel<FORWARD, SLOPE, ACT>, (unsigned)std::min<long long>(sms, most_units(p, a.K, a.N)), ptc::NT, smem, s, a, tm[0], tm[1], tm[2], tm[3]);
+    e = launch_dependent(ptc::product_tc_kernel<FORWARD, SLOPE, ACT>, (unsigned)std::min<long long>(sms, most_units(p, a.K, a.N)), ptc::NT, smem, s, a, tm[0], tm[1],
+                         tm[2], tm[3]);
   return e == cudaSuccess ? FASTEQ_OK : cuda_fail(e);
 }
 
-// K and N as the kernel sees them (grad_x: exchanged)
+// K and N as the kernel sees them (grad_x: exchanged); A and slope with rows of lda and ldd, 16-byte aligned
 template <bool FORWARD>
-int run_tc(const fasteq_product_problem* p, const void* A, const void* slope, const void* W, const void* bias, const void* residual,
-           const int32_t* offsets, void* C, void* slope_out, void* scratch, cudaStream_t s) {
+int run_tc(const fasteq_product_problem* p, const void* A, int lda, const void* slope, const void* W, const void* bias, const void* residual,
+           const int32_t* offsets, void* C, void* slope_out, void* split, cudaStream_t s) {
   ptc::Args a{};
   a.groups = groups_of(p, offsets);
   a.A = (const float*)A; a.slope = (const float*)slope; a.W = (const float*)W; a.bias = (const float*)bias; a.residual = (const float*)residual;
   a.C = (float*)C; a.slope_out = (float*)slope_out;
-  a.K = FORWARD ? p->k : p->n; a.N = FORWARD ? p->n : p->k;
-  a.a_wide = wide(a.K, {A, slope}) && p->rows <= 0x7fffffffLL; a.w_wide = wide(p->k, {W}); a.c_wide = wide(a.N, {C, slope_out, bias, residual}) && p->rows <= 0x7fffffffLL;
+  a.K = FORWARD ? p->k : p->n; a.N = FORWARD ? p->n : p->k; a.lda = lda; a.ldd = slope_pitch(p);
+  a.w_wide = wide(p->k, {W}); a.c_wide = wide(a.N, {C, residual});
   int sms = 0, dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e == cudaSuccess) e = tc::status_word(&a.status);
-  if (e != cudaSuccess) return cuda_fail(e);
-  if (split_bytes(p, FORWARD) > 0) {
+  if (e == cudaSuccess && split) {
     const int n_tiles = (a.N + ptc::BN - 1) / ptc::BN, n_kb = (a.K + ptc::KB - 1) / ptc::KB;
-    e = launch_dependent(ptc::split_weights_kernel<FORWARD>, (unsigned)((int64_t)p->experts * n_tiles * n_kb), 256, 0, s, a.W, (unsigned char*)scratch, a.N, a.K,
-                         n_tiles, n_kb, a.w_wide);
-    if (e != cudaSuccess) return cuda_fail(e);
-    a.split = (const unsigned char*)scratch;
+    e = launch_dependent(ptc::split_weights_kernel<FORWARD>, (unsigned)((int64_t)p->experts * n_tiles * n_kb), 256, 0, s, a.W, (unsigned char*)split, a.N, a.K, n_tiles,
+                         n_kb, a.w_wide);
+    a.split = (const unsigned char*)split;
   }
+  if (e != cudaSuccess) return cuda_fail(e);
   CUtensorMap tm[4] = {};               // A, its slope; C, its slope
   int rc = FASTEQ_OK;
-  auto map = [&](int i, const float* base, int columns, uint32_t box_rows) {
-    if (rc == FASTEQ_OK && base) rc = tc::make_map(&tm[i], base, (uint64_t)columns, 1, (uint64_t)p->rows, (uint64_t)columns, (uint64_t)columns, 32, 1, box_rows);
+  auto map = [&](int i, const float* base, int columns, int pitch, uint32_t box_rows) {
+    if (rc == FASTEQ_OK && base) rc = tc::make_map(&tm[i], base, (uint64_t)columns, 1, (uint64_t)p->rows, (uint64_t)pitch, (uint64_t)pitch, 32, 1, box_rows);
   };
-  if (a.a_wide) { map(0, a.A, a.K, ptc::BM); map(1, a.slope, a.K, ptc::BM); }
-  if (a.c_wide) { map(2, a.C, a.N, 32); map(3, a.slope_out, a.N, 32); }
+  map(0, a.A, a.K, a.lda, ptc::BM);
+  map(1, a.slope, a.K, a.ldd, ptc::BM);
+  if (a.c_wide) map(2, a.C, a.N, a.N, 32);
+  map(3, a.slope_out, a.N, a.ldd, 32);
   if (rc != FASTEQ_OK) return rc;
   if (!FORWARD) return slope ? launch_tc<false, true, kIdentity>(p, a, sms, tm, s) : launch_tc<false, false, kIdentity>(p, a, sms, tm, s);
   switch (p->act) {
@@ -275,13 +333,39 @@ int run_tc(const fasteq_product_problem* p, const void* A, const void* slope, co
   }
 }
 
+template <bool SLOPE>
+int wgrad_tc(const fasteq_product_problem* p, const void* x, int ldx, const void* g, int ldg, const void* slope, const int32_t* offsets, void* gw, void* gb,
+             void* partial, cudaStream_t s) {
+  pwg::ArgsW a{};
+  a.groups = groups_of(p, offsets);
+  a.x = (const float*)x; a.g = (const float*)g; a.slope = (const float*)slope;
+  a.gw = (float*)gw; a.gb = (float*)gb; a.partial = (float*)partial;
+  a.K = p->k; a.N = p->n; a.ldx = ldx; a.ldg = ldg; a.ldd = slope_pitch(p); a.size = chunk_rows(p, true);
+  a.tiles_k = (p->k + pwg::TN - 1) / pwg::TN;
+  a.tiles = a.tiles_k * ((p->n + pwg::TM - 1) / pwg::TM);
+  a.wide = wide(p->k, {gw}) && p->n % 4 == 0;
+  CUtensorMap tm[3] = {};
+  int rc = FASTEQ_OK;
+  auto map = [&](int i, const float* base, int columns, int pitch, uint32_t box) {
+    if (rc == FASTEQ_OK && base) rc = tc::make_map_pitched(&tm[i], base, columns, pitch, p->rows, box, pwg::ROWS);
+  };
+  map(0, a.g, p->n, ldg, pwg::TM); map(1, a.slope, p->n, a.ldd, pwg::TM); map(2, a.x, p->k, ldx, pwg::TN);
+  if (rc != FASTEQ_OK) return rc;
+  cudaError_t e = tc::status_word(&a.status);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(pwg::product_wgrad_tc_kernel<SLOPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, pwg::CfgW<SLOPE>::SMEM);
+  if (e == cudaSuccess)
+    e = launch_dependent(pwg::product_wgrad_tc_kernel<SLOPE>, (unsigned)((p->rows / a.size + p->experts) * a.tiles), pwg::NTW, pwg::CfgW<SLOPE>::SMEM, s, a, tm[0], tm[1],
+                         tm[2]);
+  return e == cudaSuccess ? reduce<float>(p, a.groups, a.size, gw, gb, partial, s) : cuda_fail(e);
+}
+
 }  // namespace
 
-extern "C" int fasteq_product_scratch(const fasteq_product_problem* p, int32_t grad_x, int64_t* bytes) {
+extern "C" int fasteq_product_scratch(const fasteq_product_problem* p, int32_t backward, int64_t* bytes) {
   static const int32_t some = 0;
   if (!bytes) return FASTEQ_INVALID;
   if (const int rc = check(p, &some)) return rc;
-  *bytes = split_bytes(p, !grad_x);
+  *bytes = scratch_of(p, backward != 0).total();
   return FASTEQ_OK;
 }
 
@@ -289,41 +373,65 @@ extern "C" int fasteq_product_forward(const fasteq_product_problem* p, const voi
                                       const int32_t* offsets, void* y, void* slope, void* scratch, int64_t scratch_bytes, fasteq_stream_t stream) {
   if (const int rc = check(p, offsets)) return rc;
   if (p->rows == 0 || p->n == 0) return FASTEQ_OK;
-  const int64_t need = split_bytes(p, true);
-  if (!y || (p->k > 0 && (!x || !w)) || (need > 0 && (!scratch || scratch_bytes < need))) return FASTEQ_INVALID;
-  if (p->dtype == FASTEQ_F32 && p->k > 0 && most_units(p, p->k, p->n) > 0)
-    return run_tc<true>(p, x, nullptr, w, bias, residual, offsets, y, slope, scratch, (cudaStream_t)stream);
-  return p->dtype == FASTEQ_F32 ? forward<float>(p, x, w, bias, residual, offsets, y, slope, (cudaStream_t)stream)
-                                : forward<double>(p, x, w, bias, residual, offsets, y, slope, (cudaStream_t)stream);
+  const Scratch need = scratch_of(p, false);
+  if (!y || (p->k > 0 && (!x || !w)) || (need.total() > 0 && (!scratch || scratch_bytes < need.total()))) return FASTEQ_INVALID;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (on_tensor_cores(p) && (need.x || wide(0, {x})) && wide(0, {slope, scratch})) {
+    char* at = (char*)scratch;
+    if (need.x) {
+      const cudaError_t e = align_rows(x, nullptr, p->k, 0, p->rows, at, s);
+      if (e != cudaSuccess) return cuda_fail(e);
+      x = at;
+      at += need.x;
+    }
+    return run_tc<true>(p, x, (p->k + 3) & ~3, nullptr, w, bias, residual, offsets, y, slope, need.split ? at : nullptr, s);
+  }
+  return p->dtype == FASTEQ_F32 ? forward<float>(p, x, w, bias, residual, offsets, y, slope, s) : forward<double>(p, x, w, bias, residual, offsets, y, slope, s);
 }
 
-extern "C" int fasteq_product_dgrad(const fasteq_product_problem* p, const void* grad_y, const void* slope, const void* w, const int32_t* offsets,
-                                    void* grad_x, void* scratch, int64_t scratch_bytes, fasteq_stream_t stream) {
+extern "C" int fasteq_product_backward(const fasteq_product_problem* p, const void* x, const void* w, const void* grad_y, const void* slope,
+                                       const int32_t* offsets, void* grad_x, void* grad_w, void* grad_bias, void* scratch, int64_t scratch_bytes,
+                                       fasteq_stream_t stream) {
   if (const int rc = check(p, offsets)) return rc;
-  if (p->rows == 0 || p->k == 0) return FASTEQ_OK;
-  const int64_t need = split_bytes(p, false);
-  if (!grad_x || (p->n > 0 && (!grad_y || !w)) || (need > 0 && (!scratch || scratch_bytes < need))) return FASTEQ_INVALID;
-  if (p->dtype == FASTEQ_F32 && p->n > 0 && most_units(p, p->n, p->k) > 0)
-    return run_tc<false>(p, grad_y, slope, w, nullptr, nullptr, offsets, grad_x, nullptr, scratch, (cudaStream_t)stream);
-  return p->dtype == FASTEQ_F32 ? dgrad<float>(p, grad_y, slope, w, offsets, grad_x, (cudaStream_t)stream)
-                                : dgrad<double>(p, grad_y, slope, w, offsets, grad_x, (cudaStream_t)stream);
-}
-
-extern "C" int fasteq_product_wgrad_scratch(const fasteq_product_problem* p, int64_t* bytes) {
-  static const int32_t some = 0;
-  if (!bytes) return FASTEQ_INVALID;
-  if (const int rc = check(p, &some)) return rc;
-  *bytes = tile_numbers<CHUNK_ROWS>(p->rows, p->experts) * ((int64_t)p->n * p->k + p->n) * (p->dtype == FASTEQ_F32 ? 4 : 8);
-  return FASTEQ_OK;
-}
-
-extern "C" int fasteq_product_wgrad(const fasteq_product_problem* p, const void* x, const void* grad_y, const void* slope, const int32_t* offsets,
-                                    void* grad_w, void* grad_bias, void* scratch, int64_t scratch_bytes, fasteq_stream_t stream) {
-  if (const int rc = check(p, offsets)) return rc;
-  int64_t need = 0;
-  if (const int rc = fasteq_product_wgrad_scratch(p, &need)) return rc;
-  if (p->n == 0) return FASTEQ_OK;
-  if ((p->k > 0 && !grad_w) || (need > 0 && (!scratch || scratch_bytes < need)) || (p->rows > 0 && (!grad_y || (p->k > 0 && !x)))) return FASTEQ_INVALID;
-  return p->dtype == FASTEQ_F32 ? wgrad<float>(p, x, grad_y, slope, offsets, grad_w, grad_bias, scratch, (cudaStream_t)stream)
-                                : wgrad<double>(p, x, grad_y, slope, offsets, grad_w, grad_bias, scratch, (cudaStream_t)stream);
+  if (!grad_x && !grad_w && !grad_bias) return FASTEQ_OK;
+  if (grad_bias && !grad_w && p->k > 0) return FASTEQ_INVALID;
+  const bool sums = grad_w || grad_bias, there = p->rows > 0 && p->n > 0;
+  const Scratch need = scratch_of(p, true);
+  if (need.total() > 0 && (!scratch || scratch_bytes < need.total())) return FASTEQ_INVALID;
+  if (there && (!grad_y || (grad_x && p->k > 0 && !w) || (sums && p->k > 0 && !x))) return FASTEQ_INVALID;
+  cudaStream_t s = (cudaStream_t)stream;
+  const size_t size = p->dtype == FASTEQ_F32 ? 4 : 8;
+  cudaError_t e = cudaSuccess;
+  if (!there) {                           // no rows, or no columns to sum over
+    if (grad_x && p->rows > 0 && p->k > 0) e = cudaMemsetAsync(grad_x, 0, (size_t)p->rows * p->k * size, s);
+    if (e == cudaSuccess && grad_w && p->n > 0 && p->k > 0) e = cudaMemsetAsync(grad_w, 0, (size_t)p->experts * p->n * p->k * size, s);
+    if (e == cudaSuccess && grad_bias && p->n > 0) e = cudaMemsetAsync(grad_bias, 0, (size_t)p->experts * p->n * size, s);
+    return e == cudaSuccess ? FASTEQ_OK : cuda_fail(e);
+  }
+  char *x_at = (char*)scratch, *g_at = x_at + need.x, *split_at = g_at + need.g, *partial_at = split_at + need.split;
+  int rc = FASTEQ_OK;
+  if (on_tensor_cores(p) && (need.g || wide(0, {grad_y})) && (need.x || !sums || wide(0, {x})) && wide(0, {slope, scratch})) {
+    const int ldg = (p->n + 3) & ~3, ldx = (p->k + 3) & ~3;
+    if (need.g) {                         // with the slope multiplied in, then
+      e = align_rows(grad_y, slope, p->n, ldg, p->rows, g_at, s);
+      grad_y = g_at;
+      slope = nullptr;
+    }
+    if (sums && need.x && e == cudaSuccess) {
+      e = align_rows(x, nullptr, p->k, 0, p->rows, x_at, s);
+      x = x_at;
+    }
+    if (e != cudaSuccess) return cuda_fail(e);
+    if (grad_x) rc = run_tc<false>(p, grad_y, ldg, slope, w, nullptr, nullptr, offsets, grad_x, nullptr, need.split ? split_at : nullptr, s);
+    if (rc == FASTEQ_OK && sums)
+      rc = slope ? wgrad_tc<true>(p, x, ldx, grad_y, ldg, slope, offsets, grad_w, grad_bias, partial_at, s)
+                 : wgrad_tc<false>(p, x, ldx, grad_y, ldg, slope, offsets, grad_w, grad_bias, partial_at, s);
+    return rc;
+  }
+  const bool f32 = p->dtype == FASTEQ_F32;
+  const int rows = chunk_rows(p, on_tensor_cores(p));      // as the scratch was counted with
+  if (grad_x && p->k > 0) rc = f32 ? dgrad<float>(p, grad_y, slope, w, offsets, grad_x, s) : dgrad<double>(p, grad_y, slope, w, offsets, grad_x, s);
+  if (rc == FASTEQ_OK && sums)
+    rc = f32 ? wgrad<float>(p, rows, x, grad_y, slope, offsets, grad_w, grad_bias, partial_at, s) : wgrad<double>(p, rows, x, grad_y, slope, offsets, grad_w, grad_bias, partial_at, s);
+  return rc;
 }

@@ -106,5 +106,29 @@ template <int SIZE> __device__ __forceinline__ int tile_of(const Groups& g, int 
   return lo;
 }
 
+// The same with a size known at run time, found by a warp together (two loads a lane for up to 1024 groups): for the chunks of the weight gradient.
+struct Chunk {
+  int e, rows;                          // group, rows (0: an empty number)
+  long long m0, begin, count;           // first row; the group's first row and number of chunks
+};
+__device__ __forceinline__ Chunk chunk_of(const Groups& g, int n_groups, int size, long long b) {
+  const int lane = threadIdx.x & 31, step = (n_groups + 31) / 32;
+  auto begins = [&](int e) { return e < n_groups && g.first(e) / size + e <= b; };
+  int e = (__popc(__ballot_sync(0xffffffffu, begins(lane * step))) - 1) * step;
+  if (step > 1) e += __popc(__ballot_sync(0xffffffffu, lane < step && begins(e + lane))) - 1;
+  Chunk c;
+  c.e = e;
+  c.begin = g.first(e);
+  const long long end = g.first(e + 1), left = end - c.begin - (b - (c.begin / size + e)) * size;
+  c.count = (end - c.begin + size - 1) / size;
+  c.m0 = end - left;
+  c.rows = left <= 0 ? 0 : left < size ? (int)left : size;
+  return c;
+}
+// Where a chunk's partial sums go, of chunks(rows, size): groups of several chunks have more than their share of 2 rows / size, so that
+// counting those from 2 begin / size leaves each its own.  A group of one chunk needs none, its sums are the result.
+__host__ __device__ inline long long partial_slots(long long rows, int size) { return 2 * rows / size + 1; }
+__device__ __forceinline__ long long partial_slot(const Chunk& c, int size) { return 2 * c.begin / size + (c.m0 - c.begin) / size; }
+
 }  // namespace product
 }  // namespace fasteq

@@ -10,7 +10,7 @@
 // A persistent CTA per SM walks a share of the units (expert, 64 columns, 128 rows), rows innermost: the split weights stay in shared memory
 // as long as expert and columns do (k up to 32 x slots).  Beyond that a kernel before this one splits the weights, and their blocks go through
 // the slots as a ring, a bulk copy each.
-//   warp 0       brings A's raw k-blocks to shared memory: TMA where K and the address allow it, else copies of four bytes (cp.async)
+//   warp 0       brings A's raw k-blocks to shared memory (TMA; rows that are not 16-byte aligned a kernel before this one copies apart)
 //   warp 1       issues the MMAs
 //   warps 2-3    load, split and store the weights' k-blocks, or bring the split ones
 //   warps 4-11   split raw blocks into tensor memory (thread = row = TMEM lane), four warps the even and four the odd ones
@@ -50,17 +50,9 @@ template <bool SLOPE> struct Cfg {
   static constexpr int slots(int experts) { return (227 * 1024 - smem(0, experts)) / B_BYTES < MOST_SLOTS ? (227 * 1024 - smem(0, experts)) / B_BYTES : MOST_SLOTS; }
 };
 
-__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src, bool there) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
-}
-// one arrival on the barrier once the thread's copies so far have landed
-__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
 __device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, uint32_t n) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(n) : "memory");
 }
-__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // A CTA's walk over its units.  tiles: exclusive prefix sums of the experts' row tiles, [experts + 1].
 struct Walk {
@@ -181,15 +173,15 @@ struct Args {
   const float *A, *slope, *W, *bias, *residual;
   const unsigned char* split;         // the weights' blocks where they do not stay in shared memory
   float *C, *slope_out;
-  int K, N, slots;                    // slots of the weights' blocks
-  bool a_wide, w_wide, c_wide;        // 16-byte accesses of A (and slope), of W, of everything shaped like C (and bias)
+  int K, N, lda, ldd, slots;          // columns between A's rows and between slope's, slots of the weights' blocks
+  bool w_wide, c_wide;                // 16-byte accesses of W, of C and the residual
   int* status;
 };
 
 // a sum of row r (of all) and column n of expert e that is not finite, again with FP32's own products
 template <bool FORWARD, bool SLOPE> __device__ __noinline__ float again(const Args& p, int e, size_t r, int n, float v) {
   if (fabsf(v) <= 3.402823466e38f) return v;
-  const float *a = p.A + r * p.K, *d = SLOPE ? p.slope + r * p.K : nullptr, *b = p.W + (size_t)e * p.N * p.K + (FORWARD ? (size_t)n * p.K : (size_t)n);
+  const float *a = p.A + r * p.lda, *d = SLOPE ? p.slope + r * p.ldd : nullptr, *b = p.W + (size_t)e * p.N * p.K + (FORWARD ? (size_t)n * p.K : (size_t)n);
   v = 0.f;
 #pragma unroll 1
   for (int k = 0; k < p.K; ++k) v = fmaf(SLOPE ? a[k] * d[k] : a[k], b[FORWARD ? (size_t)k : (size_t)k * p.N], v);
@@ -245,18 +237,18 @@ __device__ __forceinline__ void store_16(float* dst, int count, bool wide, const
   }
 }
 // A slab's rows, without TMA: where the tile ends inside the tensor (another expert's rows follow), or its rows are not 16-byte aligned.
-__device__ __forceinline__ void store_slab(float* C, size_t row0, int rows, int n0, int N, bool wide, const unsigned char* slab) {
+__device__ __forceinline__ void store_slab(float* C, size_t row0, int rows, int n0, int N, int pitch, bool wide, const unsigned char* slab) {
   const int lane = threadIdx.x & 31;
   if (wide) {
     const int n = n0 + (lane & 7) * 4;
 #pragma unroll 2
     for (int r = lane >> 3; r < 32; r += 4)
-      if (r < rows && n < N) *reinterpret_cast<float4*>(C + (row0 + r) * N + n) = *reinterpret_cast<const float4*>(slab + slab_at(r, lane & 7));
+      if (r < rows && n < N) *reinterpret_cast<float4*>(C + (row0 + r) * pitch + n) = *reinterpret_cast<const float4*>(slab + slab_at(r, lane & 7));
   } else {
     const int n = n0 + lane;
 #pragma unroll 4
     for (int r = 0; r < 32; ++r)
-      if (r < rows && n < N) C[(row0 + r) * N + n] = *reinterpret_cast<const float*>(slab + slab_at(r, lane >> 2) + (lane & 3) * 4);
+      if (r < rows && n < N) C[(row0 + r) * pitch + n] = *reinterpret_cast<const float*>(slab + slab_at(r, lane >> 2) + (lane & 3) * 4);
   }
 }
 
@@ -286,7 +278,7 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
   int* status = p.status;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) { mbar_init(&a_full[s], p.a_wide ? 1 : 32); mbar_init(&a_empty[s], 4); }
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&a_full[s], 1); mbar_init(&a_empty[s], 4); }
     for (int s = 0; s < slots; ++s) { mbar_init(&b_full[s], p.split ? 1 : 8); mbar_init(&b_empty[s], 1); }
     for (int s = 0; s < A_SLOTS; ++s) { mbar_init(&s_full[s], 4); mbar_init(&s_empty[s], 1); }
     for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 8); }
@@ -329,37 +321,19 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
       // results are not written
       int it = 0;
       for (int u = u0; u < u1; ++u, w.next()) {
-        const long long begin = p.groups.first(w.e), left = p.groups.first(w.e + 1) - begin - (long long)w.m * BM;
-        const long long row0 = begin + (long long)w.m * BM;
+        const long long row0 = p.groups.first(w.e) + (long long)w.m * BM;
         for (int kb = 0; kb < n_kb; ++kb, ++it) {
           const int s = it % STAGES;
           unsigned char* st = a_raw + (size_t)s * C_::STAGE_BYTES;
           mbar_wait(&a_empty[s], ((it / STAGES) & 1u) ^ 1u, status);
-          if (p.a_wide) {
-            if (lane == 0) {
-              mbar_arrive_expect_tx(&a_full[s], (uint32_t)C_::STAGE_BYTES);
-              tma_load_3d(st, &tmA, kb * KB, 0, (int)row0, &a_full[s]);
-              if (SLOPE) tma_load_3d(st + A_BYTES, &tmSlope, kb * KB, 0, (int)row0, &a_full[s]);
-            }
-            __syncwarp();
-          } else {
-            const int rows = left < BM ? (int)left : BM, k = kb * KB + lane;
-#pragma unroll
-            for (int side = 0; side < (SLOPE ? 2 : 1); ++side) {
-              const float* src = side ? p.slope : p.A;
-              const float* a = src + (size_t)row0 * K + k;
-              const uint32_t d = smem_u32(st) + side * A_BYTES + (lane & 3) * 4;
-#pragma unroll 8
-              for (int r = 0; r < BM; ++r) {
-                const bool there = r < rows && k < K;
-                cp_async_4(d + r * 128 + (((lane >> 2) ^ (r & 7)) << 4), there ? a + (size_t)r * K : src, there);
-              }
-            }
-            cp_async_arrive(&a_full[s]);
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&a_full[s], (uint32_t)C_::STAGE_BYTES);
+            tma_load_3d(st, &tmA, kb * KB, 0, (int)row0, &a_full[s]);
+            if (SLOPE) tma_load_3d(st + A_BYTES, &tmSlope, kb * KB, 0, (int)row0, &a_full[s]);
           }
+          __syncwarp();
         }
       }
-      cp_async_wait_all();
     } else if (warp == 1) {
       // ------------------------------------------------------------------ MMAs (whole warp, one elected lane)
       const uint32_t idesc2 = wg::idesc_bf16_m128(2 * BN), idesc1 = wg::idesc_bf16_m128(BN);
@@ -595,8 +569,8 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
               bulk_commit();
             }
           } else {
-            store_slab(p.C, row0, rows, n0, N, p.c_wide, slab);
-            if (keep) store_slab(p.slope_out, row0, rows, n0, N, p.c_wide, slopes);
+            store_slab(p.C, row0, rows, n0, N, N, p.c_wide, slab);
+            if (keep) store_slab(p.slope_out, row0, rows, n0, N, p.ldd, true, slopes);
           }
           __syncwarp();
         }
@@ -607,10 +581,7 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
   // rows of no expert
   if (p.groups.offsets) {
     const size_t first = (size_t)p.groups.first(X) * N, end = (size_t)p.groups.rows * N;
-    for (size_t i = first + (size_t)blockIdx.x * NT + threadIdx.x; i < end; i += (size_t)gridDim.x * NT) {
-      p.C[i] = 0.f;
-      if (FORWARD && ACT != product::kIdentity && p.slope_out) p.slope_out[i] = 0.f;
-    }
+    for (size_t i = first + (size_t)blockIdx.x * NT + threadIdx.x; i < end; i += (size_t)gridDim.x * NT) p.C[i] = 0.f;
   }
   tc_fence_before();
   __syncthreads();

@@ -441,12 +441,13 @@ int fasteq_readout_backward(int32_t dtype, const void* g, const void* w, void* g
  * Without `offsets` (NULL) there is one matrix.  With them the rows are in the experts' order: entry i owns rows [i * inner, (i + 1) * inner),
  * expert e the entries [offsets[e], offsets[e + 1]) (device [experts + 1], as fasteq_expert_plan writes them, read on the device: no host
  * synchronisation), and rows behind offsets[experts] are written as zeros and take part in nothing.
- * act: the codes of the gate (0 identity, 1 silu, 2 tanh, 3 sigmoid, 4 abs).  `slope` [rows, n] (forward, may be NULL) receives act'(z), which
- * the gradients take (NULL where act is the identity): with gz = grad_y * slope
+ * act: the codes of the gate (0 identity, 1 silu, 2 tanh, 3 sigmoid, 4 abs).  `slope` (forward, may be NULL; not touched where act is the
+ * identity) receives act'(z) for the gradients, which take NULL where it is the identity: [rows, n], FP32 rows (n + 3) & ~3 values apart and 16-byte
+ * aligned.  With gz = grad_y * slope
  *   grad_x = gz W[e],   grad_w[e] = sum_{r of e} gz[r]^T x[r],   grad_bias[e] = sum_{r of e} gz[r].
- * FP32 data: products of three bf16 parts per operand on the tensor cores, accumulated in FP32 (the accuracy of FP32 products), FP32 FMAs
- * where those do not pay; FP64: FP64 throughout.  Sums are formed in a fixed order.  Any extents, any 4- / 8-byte aligned addresses.
- * The reference leaves such layers to the model package.
+ * FP32 data: products of three bf16 parts per operand on the tensor cores, accumulated in FP32 (the accuracy of FP32 products); FP64: FP64
+ * throughout.  Sums are formed in a fixed order.  Any extents, any 4- / 8-byte aligned addresses (FP32 ones that are not 16-byte aligned
+ * take FP32 multiply-adds).  The reference leaves such layers to the model package.
  * ------------------------------------------------------------------------- */
 #define FASTEQ_MAX_EXPERTS 1024
 typedef struct fasteq_product_problem {
@@ -456,19 +457,16 @@ typedef struct fasteq_product_problem {
   int32_t act;
   int64_t rows;
 } fasteq_product_problem;
-/* scratch: 16-byte aligned device memory of the bytes `_scratch` names (grad_x: for `_dgrad`; may be 0, NULL then), not in use by other work on the
- * device meanwhile. */
-int fasteq_product_scratch(const fasteq_product_problem* p /* host */, int32_t grad_x, int64_t* bytes /* host */);
+/* scratch: 16-byte aligned device memory of the bytes `_scratch` names for the forward (backward 0) or the gradients (1) of the problem; may be
+ * 0, NULL then; not in use by other work on the device meanwhile. */
+int fasteq_product_scratch(const fasteq_product_problem* p /* host */, int32_t backward, int64_t* bytes /* host */);
 int fasteq_product_forward(const fasteq_product_problem* p /* host */, const void* x, const void* w, const void* bias /* or NULL */,
                            const void* residual /* or NULL */, const int32_t* offsets /* or NULL */, void* y, void* slope /* or NULL */,
                            void* scratch, int64_t scratch_bytes, fasteq_stream_t stream);
-int fasteq_product_dgrad(const fasteq_product_problem* p /* host */, const void* grad_y, const void* slope /* or NULL */, const void* w,
-                         const int32_t* offsets /* or NULL */, void* grad_x, void* scratch, int64_t scratch_bytes, fasteq_stream_t stream);
-/* Weight and bias gradient (grad_bias may be NULL), with a scratch of its own. */
-int fasteq_product_wgrad_scratch(const fasteq_product_problem* p /* host */, int64_t* bytes /* host */);
-int fasteq_product_wgrad(const fasteq_product_problem* p /* host */, const void* x, const void* grad_y, const void* slope /* or NULL */,
-                         const int32_t* offsets /* or NULL */, void* grad_w, void* grad_bias /* or NULL */, void* scratch, int64_t scratch_bytes,
-                         fasteq_stream_t stream);
+/* Any of the gradients may be NULL; grad_bias goes with grad_w.  w is read for grad_x, x for the others. */
+int fasteq_product_backward(const fasteq_product_problem* p /* host */, const void* x, const void* w, const void* grad_y,
+                            const void* slope /* or NULL */, const int32_t* offsets /* or NULL */, void* grad_x, void* grad_w, void* grad_bias,
+                            void* scratch, int64_t scratch_bytes, fasteq_stream_t stream);
 
 /* Rows in the order of the experts they are given to, and back.  Entry i = token * slots + slot is given to expert[i] (index_bytes 4 or 8;
  * negative: to none; >= experts: to none, and the status word below reads 2).  position[i]: the entry's row in a stable order by expert, entries of no

@@ -47,17 +47,20 @@ def test_other_entries_refuse_null_pointers_and_sizes():
     lib = _core()
     p, one = Problem(**GOOD), C.c_int64(0)
     assert lib.fasteq_product_forward(None, None, None, None, None, None, None, None, None, I64(0), None) == INVALID
-    assert lib.fasteq_product_dgrad(C.byref(p), None, None, None, None, None, None, I64(0), None) == INVALID
-    assert lib.fasteq_product_scratch(C.byref(p), I32(0), None) == INVALID and lib.fasteq_product_scratch(C.byref(p), I32(1), C.byref(one)) == OK
-    long = Problem(**{**GOOD, "k": 2048})
-    assert lib.fasteq_product_scratch(C.byref(long), I32(0), C.byref(one)) == OK and one.value > 0
+    none = (None,) * 8
+    assert lib.fasteq_product_backward(C.byref(p), *none, None, I64(0), None) == OK              # no gradient is asked for
     some = C.create_string_buffer(64)
+    assert lib.fasteq_product_backward(C.byref(p), None, None, None, None, None, some, None, None, None, I64(0), None) == INVALID
+    assert lib.fasteq_product_backward(C.byref(p), some, some, some, None, None, None, None, some, None, I64(0), None) == INVALID      # bias without weights
+    assert lib.fasteq_product_scratch(C.byref(p), I32(0), None) == INVALID
+    for change, backward, there in ((dict(), 0, False), (dict(), 1, False), (dict(k=2048), 0, True), (dict(k=7), 0, True), (dict(n=7), 0, False), (dict(n=7), 1, True),
+                                    (dict(rows=100_000), 1, True), (dict(rows=100_000, dtype=1), 0, False), (dict(rows=0, k=7), 1, False)):
+        q = Problem(**{**GOOD, **change})
+        assert lib.fasteq_product_scratch(C.byref(q), I32(backward), C.byref(one)) == OK and (one.value > 0) == there, change
+    long = Problem(**{**GOOD, "k": 2048})
     assert lib.fasteq_product_forward(C.byref(long), some, some, None, None, None, some, None, some, I64(16), None) == INVALID
-    assert lib.fasteq_product_wgrad_scratch(C.byref(p), C.byref(one)) == OK and one.value > 0
-    assert lib.fasteq_product_wgrad_scratch(C.byref(p), None) == INVALID
-    assert lib.fasteq_product_wgrad(C.byref(p), None, None, None, None, None, None, None, I64(0), None) == INVALID
     many = Problem(**{**GOOD, "experts": 1025})
-    assert lib.fasteq_product_wgrad_scratch(C.byref(many), C.byref(one)) == UNSUPPORTED
+    assert lib.fasteq_product_scratch(C.byref(many), I32(1), C.byref(one)) == UNSUPPORTED
     assert lib.fasteq_expert_plan_scratch(I64(-1), I32(3), C.byref(one)) == INVALID
     assert lib.fasteq_expert_plan_scratch(I64(5), I32(1025), C.byref(one)) == UNSUPPORTED
     assert lib.fasteq_expert_plan_scratch(I64(2 ** 31), I32(3), C.byref(one)) == UNSUPPORTED
