@@ -11,6 +11,7 @@
 #include "product.cuh"
 #include "product_tc.cuh"
 #include "product_wgrad_tc.cuh"
+#include "product_f64.cuh"
 #include "gemm_tf32x3.h"
 
 using namespace fasteq;
@@ -134,29 +135,37 @@ __global__ void __launch_bounds__(THREADS) product_wgrad_kernel(Groups groups, c
   if (k0 == 0 && t < TILE && n0 + t < N && (gb || !only)) (only ? gb + (size_t)c.e * N : dst + nk)[n0 + t] = column;
 }
 
-// Experts of no or of several chunks: 32 values at a time to a CTA, eight threads to each, which take every eighth chunk and are added in order.
-template <typename T> __global__ void __launch_bounds__(256) product_reduce_kernel(Groups groups, const T* partial, int K, int N, int size, T* gw, T* gb) {
-  __shared__ T part[8][33];
+// Experts of no or of several chunks: 32 packs of V values at a time to a CTA, eight threads to each, which take every eighth chunk and are added in
+// order.
+template <typename T, int V> __global__ void __launch_bounds__(256) product_reduce_kernel(Groups groups, const T* partial, int K, int N, int size, T* gw, T* gb) {
+  struct alignas(sizeof(T) * V) Pack { T v[V]; };
+  __shared__ Pack part[8][32];
   wait_for_previous_kernel();
   const int e = blockIdx.y;
   const size_t nk = (size_t)N * K, all = nk + N;
   const long long begin = groups.first(e), n = (groups.first(e + 1) - begin + size - 1) / size;
   if (n == 1) return;
   const T* from = partial + (size_t)(2 * begin / size) * all;
-  for (size_t i0 = (size_t)blockIdx.x * 32; i0 < all; i0 += (size_t)gridDim.x * 32) {
-    const size_t i = i0 + threadIdx.x;
-    T s = T(0);
+  for (size_t i0 = (size_t)blockIdx.x * 32 * V; i0 < all; i0 += (size_t)gridDim.x * 32 * V) {
+    const size_t i = i0 + threadIdx.x * V;
+    Pack s{};
     if (i < all) {
 #pragma unroll 4
-      for (long long c = threadIdx.y; c < n; c += 8) s += from[(size_t)c * all + i];
+      for (long long c = threadIdx.y; c < n; c += 8) {
+        const Pack v = *reinterpret_cast<const Pack*>(from + (size_t)c * all + i);
+#pragma unroll
+        for (int k = 0; k < V; ++k) s.v[k] += v.v[k];
+      }
     }
     part[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
     if (threadIdx.y == 0 && i < all) {
 #pragma unroll
-      for (int j = 1; j < 8; ++j) s += part[j][threadIdx.x];
-      if (i < nk) gw[(size_t)e * nk + i] = s;
-      else if (gb) gb[(size_t)e * N + (i - nk)] = s;
+      for (int j = 1; j < 8; ++j)
+#pragma unroll
+        for (int k = 0; k < V; ++k) s.v[k] += part[j][threadIdx.x].v[k];
+      if (i < nk) *reinterpret_cast<Pack*>(gw + (size_t)e * nk + i) = s;
+      else if (gb) *reinterpret_cast<Pack*>(gb + (size_t)e * N + (i - nk)) = s;
     }
     __syncthreads();
   }
@@ -191,21 +200,61 @@ int dgrad(const fasteq_product_problem* p, const void* g, const void* slope, con
                                          (const T*)nullptr, (const T*)nullptr, p->n, p->k, slope_pitch(p), 0, (T*)gx, (T*)nullptr);
   return e == cudaSuccess ? FASTEQ_OK : cuda_fail(e);
 }
-// Rows of a chunk: as many as give every SM `per_sm` tiles of rows x matrix.  At least 256: below that a chunk's start and its sums' way out
-// take longer than its rows.
-int chunk_rows(const fasteq_product_problem* p, int tile_n, int tile_k, int per_sm) {
-  const long long tiles = (long long)((p->n + tile_n - 1) / tile_n) * std::max(1, (p->k + tile_k - 1) / tile_k);
-  const long long rows = (p->rows * tiles + 148 * per_sm - 1) / (148 * per_sm);
-  return (int)std::min<long long>(1 << 24, std::max<long long>(256, (rows + 31) / 32 * 32));
+// CTAs of a launch over tiles of rows and columns
+bool in_32_bits(const fasteq_product_problem* p, int tile) {
+  const long long columns = (std::max(p->k, p->n) + tile - 1) / tile, rows = p->rows / tile + p->experts + 1;
+  return rows * columns <= 0x7fffffffLL && columns * columns * (p->rows / 256 + p->experts) <= 0x7fffffffLL;
 }
-int chunk_rows(const fasteq_product_problem* p, bool tensor_cores) { return tensor_cores ? chunk_rows(p, pwg::TM, pwg::TN, 1) : chunk_rows(p, TILE, TILE, 4); }
+bool even(int extent, std::initializer_list<const void*> pointers) {
+  uintptr_t all = 0;
+  for (const void* q : pointers) all |= reinterpret_cast<uintptr_t>(q);
+  return extent % 2 == 0 && (all & 15u) == 0;
+}
+template <bool FORWARD, bool SLOPE>
+int product_f64(const fasteq_product_problem* p, const void* A, const void* slope, const void* w, const void* bias, const void* residual, const int32_t* offsets, void* C,
+                void* slope_out, cudaStream_t s) {
+  const int K = FORWARD ? p->k : p->n, N = FORWARD ? p->n : p->k, tiles_n = (N + pf64::TILE - 1) / pf64::TILE;
+  cudaError_t e = cudaFuncSetAttribute(pf64::product_f64_kernel<FORWARD, SLOPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, pf64::smem_bytes<SLOPE>());
+  if (e == cudaSuccess)
+    e = launch_dependent(pf64::product_f64_kernel<FORWARD, SLOPE>, (unsigned)(tile_numbers<pf64::TILE>(p->rows, p->experts + 1) * tiles_n), pf64::NT,
+                         pf64::smem_bytes<SLOPE>(), s, groups_of(p, offsets), (const double*)A, (const double*)slope, (const double*)w, (const double*)bias,
+                         (const double*)residual, K, N, p->act, tiles_n, even(K, {A, slope}), even(p->k, {w}), (double*)C, (double*)slope_out);
+  return e == cudaSuccess ? FASTEQ_OK : cuda_fail(e);
+}
+
+// Rows of a chunk: as many as give every SM `per_sm` tiles of rows x matrix, in one wave.  Every expert may add a chunk to those; many experts take
+// half of the places at most.  At least 256 rows: below that a chunk's start and its sums' way out take longer than its rows.
+int chunk_rows(const fasteq_product_problem* p, int tile_n, int tile_k, int per_sm) {
+  const long long tiles = (long long)((p->n + tile_n - 1) / tile_n) * std::max(1, (p->k + tile_k - 1) / tile_k), places = std::max<long long>(1, 148 * per_sm / tiles);
+  const long long chunks = std::max<long long>(std::max<long long>(places - (p->experts > 1 ? p->experts : 0), places / 2), 1);
+  const long long rows = ((p->rows + chunks - 1) / chunks + 31) / 32 * 32;
+  return (int)std::min<long long>(1 << 24, std::max<long long>(256, rows));
+}
+int chunk_rows(const fasteq_product_problem* p, bool tensor_cores) { return tensor_cores ? chunk_rows(p, pwg::TM, pwg::TN, 1) : chunk_rows(p, TILE, TILE, 3); }
 
 template <typename T> int reduce(const fasteq_product_problem* p, const Groups& groups, int size, void* gw, void* gb, void* scratch, cudaStream_t s) {
   if (p->experts == 1 && p->rows <= size && !groups.offsets) return FASTEQ_OK;
-  const size_t blocks = ((size_t)p->n * p->k + p->n + 31) / 32;
-  const cudaError_t e = launch_dependent(product_reduce_kernel<T>, dim3((unsigned)std::min<size_t>(blocks, std::max(1, 4096 / p->experts)), (unsigned)p->experts), dim3(32, 8),
-                                         0, s, groups, (const T*)scratch, p->k, p->n, size, (T*)gw, (T*)gb);
+  constexpr int V = 16 / sizeof(T);
+  const uintptr_t all = reinterpret_cast<uintptr_t>(gw) | reinterpret_cast<uintptr_t>(gb) | reinterpret_cast<uintptr_t>(scratch);
+  const bool wide = p->n % V == 0 && all % 16 == 0;
+  const size_t blocks = ((size_t)p->n * p->k + p->n + 32 * (wide ? V : 1) - 1) / (32 * (wide ? V : 1));
+  const cudaError_t e = launch_dependent(wide ? product_reduce_kernel<T, V> : product_reduce_kernel<T, 1>,
+                                         dim3((unsigned)std::min<size_t>(blocks, std::max(1, 4096 / p->experts)), (unsigned)p->experts), dim3(32, 8), 0, s, groups,
+                                         (const T*)scratch, p->k, p->n, size, (T*)gw, (T*)gb);
   return e == cudaSuccess ? FASTEQ_OK : cuda_fail(e);
+}
+
+template <bool SLOPE>
+int wgrad_f64(const fasteq_product_problem* p, int size, const void* x, const void* g, const void* slope, const int32_t* offsets, void* gw, void* gb, void* scratch,
+              cudaStream_t s) {
+  const Groups groups = groups_of(p, offsets);
+  const int tiles_k = (p->k + pf64::TILE - 1) / pf64::TILE, tiles = tiles_k * ((p->n + pf64::TILE - 1) / pf64::TILE);
+  cudaError_t e = cudaFuncSetAttribute(pf64::product_wgrad_f64_kernel<SLOPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, pf64::smem_bytes<SLOPE>());
+  if (e == cudaSuccess)
+    e = launch_dependent(pf64::product_wgrad_f64_kernel<SLOPE>, (unsigned)((p->rows / size + p->experts) * tiles), pf64::NT, pf64::smem_bytes<SLOPE>(), s, groups,
+                         (const double*)x, (const double*)g, (const double*)slope, p->k, p->n, size, tiles_k, tiles, even(p->k, {x}), even(p->n, {g, slope}), (double*)gw,
+                         (double*)gb, (double*)scratch);
+  return e == cudaSuccess ? reduce<double>(p, groups, size, gw, gb, scratch, s) : cuda_fail(e);
 }
 
 template <typename T>
@@ -228,7 +277,7 @@ bool wide(int extent, std::initializer_list<const void*> pointers) {
 // Units of the tensor-core kernel (at most), which counts them, and a CTA's blocks, in 32 bits.
 long long most_units(const fasteq_product_problem* p, int K, int N) {
   const long long units = (p->rows / ptc::BM + p->experts) * ((N + ptc::BN - 1) / ptc::BN);
-  return units > 0x7fffffffLL || (units / 64 + 1) * ((K + ptc::KB - 1) / ptc::KB) > 0x3fffffffLL ? -1 : units;
+  return units > 0x3fffffffLL || units * ((K + ptc::KB - 1) / ptc::KB) > 0x3fffffffLL ? -1 : units;
 }
 bool on_tensor_cores(const fasteq_product_problem* p) {
   return p->dtype == FASTEQ_F32 && p->k > 0 && p->n > 0 && p->rows > 0 && p->rows <= 0x7fffffffLL && most_units(p, p->k, p->n) > 0 && most_units(p, p->n, p->k) > 0;
@@ -386,7 +435,9 @@ extern "C" int fasteq_product_forward(const fasteq_product_problem* p, const voi
     }
     return run_tc<true>(p, x, (p->k + 3) & ~3, nullptr, w, bias, residual, offsets, y, slope, need.split ? at : nullptr, s);
   }
-  return p->dtype == FASTEQ_F32 ? forward<float>(p, x, w, bias, residual, offsets, y, slope, s) : forward<double>(p, x, w, bias, residual, offsets, y, slope, s);
+  if (p->dtype == FASTEQ_F32) return forward<float>(p, x, w, bias, residual, offsets, y, slope, s);
+  if (p->k == 0 || !in_32_bits(p, pf64::TILE)) return forward<double>(p, x, w, bias, residual, offsets, y, slope, s);
+  return product_f64<true, false>(p, x, nullptr, w, bias, residual, offsets, y, slope, s);
 }
 
 extern "C" int fasteq_product_backward(const fasteq_product_problem* p, const void* x, const void* w, const void* grad_y, const void* slope,
@@ -428,8 +479,15 @@ extern "C" int fasteq_product_backward(const fasteq_product_problem* p, const vo
                  : wgrad_tc<false>(p, x, ldx, grad_y, ldg, slope, offsets, grad_w, grad_bias, partial_at, s);
     return rc;
   }
-  const bool f32 = p->dtype == FASTEQ_F32;
   const int rows = chunk_rows(p, on_tensor_cores(p));      // as the scratch was counted with
+  if (p->dtype == FASTEQ_F64 && p->k > 0 && in_32_bits(p, pf64::TILE)) {
+    if (grad_x) rc = slope ? product_f64<false, true>(p, grad_y, slope, w, nullptr, nullptr, offsets, grad_x, nullptr, s)
+                           : product_f64<false, false>(p, grad_y, nullptr, w, nullptr, nullptr, offsets, grad_x, nullptr, s);
+    if (rc == FASTEQ_OK && sums) rc = slope ? wgrad_f64<true>(p, rows, x, grad_y, slope, offsets, grad_w, grad_bias, partial_at, s)
+                                            : wgrad_f64<false>(p, rows, x, grad_y, nullptr, offsets, grad_w, grad_bias, partial_at, s);
+    return rc;
+  }
+  const bool f32 = p->dtype == FASTEQ_F32;
   if (grad_x && p->k > 0) rc = f32 ? dgrad<float>(p, grad_y, slope, w, offsets, grad_x, s) : dgrad<double>(p, grad_y, slope, w, offsets, grad_x, s);
   if (rc == FASTEQ_OK && sums)
     rc = f32 ? wgrad<float>(p, rows, x, grad_y, slope, offsets, grad_w, grad_bias, partial_at, s) : wgrad<double>(p, rows, x, grad_y, slope, offsets, grad_w, grad_bias, partial_at, s);

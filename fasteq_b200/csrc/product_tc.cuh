@@ -7,8 +7,8 @@
 // accumulator of its own and the small ones another: only the first is as large as the result, and the tensor core's truncating additions
 // cost it one rounding toward zero per 16 products.
 //
-// A persistent CTA per SM walks a share of the units (expert, 64 columns, 128 rows), rows innermost: the split weights stay in shared memory
-// as long as expert and columns do (k up to 32 x slots).  Beyond that a kernel before this one splits the weights, and their blocks go through
+// A persistent CTA per SM takes 64 columns and walks a share of the row tiles (128 rows of an expert): the split weights stay in shared memory
+// as long as the expert does (k up to 32 x slots).  Beyond that a kernel before this one splits the weights, and their blocks go through
 // the slots as a ring, a bulk copy each.
 //   warp 0       brings A's raw k-blocks to shared memory (TMA; rows that are not 16-byte aligned a kernel before this one copies apart)
 //   warp 1       issues the MMAs
@@ -54,33 +54,36 @@ __device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, uint32_t n) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(n) : "memory");
 }
 
-// A CTA's walk over its units.  tiles: exclusive prefix sums of the experts' row tiles, [experts + 1].
+// A CTA's walk over its units: the row tiles [first, first + count) of all experts' for its columns n, and again for those n_step further on.
+// tiles: exclusive prefix sums of the experts' row tiles, [experts + 1].
 struct Walk {
   const int* tiles;
-  int experts, n_tiles;
-  int e, n, m, mt;
-  __device__ __forceinline__ Walk(const int* t, int x, int nt, int unit) : tiles(t), experts(x), n_tiles(nt) {
-    int lo = 0, hi = x - 1;
+  int experts, first, count, n_step;
+  int e, n, m, mt, left;
+  __device__ __forceinline__ Walk(const int* t, int x, int f, int c, int n0, int step) : tiles(t), experts(x), first(f), count(c), n_step(step), n(n0) { start(); }
+  __device__ __forceinline__ void start() {
+    int lo = 0, hi = experts - 1;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (tiles[mid + 1] * n_tiles > unit) hi = mid; else lo = mid + 1;
+      if (tiles[mid + 1] > first) hi = mid; else lo = mid + 1;
     }
     e = lo;
     mt = tiles[e + 1] - tiles[e];
-    const int rest = unit - tiles[e] * n_tiles;
-    n = mt ? rest / mt : 0;
-    m = rest - n * mt;
+    m = first - tiles[e];
+    left = count;
   }
   __device__ __forceinline__ void next() {
-    if (++m < mt) return;
-    m = 0;
-    if (++n < n_tiles) return;
-    n = 0;
-    do ++e; while (e < experts && tiles[e + 1] == tiles[e]);
-    mt = e < experts ? tiles[e + 1] - tiles[e] : 0;
+    if (--left == 0) {
+      n += n_step;
+      start();
+    } else if (++m == mt) {
+      m = 0;
+      do ++e; while (tiles[e + 1] == tiles[e]);          // ends at a later one of the CTA's tiles
+      mt = tiles[e + 1] - tiles[e];
+    }
   }
-  __device__ __forceinline__ bool run_begins(bool first) const { return first || m == 0; }
-  __device__ __forceinline__ bool run_ends(bool last) const { return last || m + 1 == mt; }
+  __device__ __forceinline__ bool run_begins() const { return left == count || m == 0; }
+  __device__ __forceinline__ bool run_ends() const { return left == 1 || m + 1 == mt; }
 };
 
 __device__ __forceinline__ void tmem_ld_16_begin(uint32_t taddr, uint32_t (&r)[16]) {
@@ -310,17 +313,19 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
   const uint32_t tmem = *tmem_slot;
   const int n_tiles = (N + BN - 1) / BN, n_kb = (K + KB - 1) / KB;
   const bool resident = p.split == nullptr;        // n_kb <= slots then
-  const long long units = (long long)tiles[X] * n_tiles;
-  const int u0 = (int)(units * blockIdx.x / gridDim.x), u1 = (int)(units * (blockIdx.x + 1) / gridDim.x);
+  // CTAs with neighbouring columns of the same rows lie side by side and walk together, so that A comes from memory once
+  const int beside = min(n_tiles, (int)gridDim.x), sets = (int)gridDim.x / beside, set_no = (int)blockIdx.x / beside, n_first = (int)blockIdx.x % beside;
+  const int first = (int)((long long)tiles[X] * set_no / sets), count = set_no < sets ? (int)((long long)tiles[X] * (set_no + 1) / sets) - first : 0;
+  const int units = count * ((n_tiles - n_first + beside - 1) / beside);
 
-  if (u0 < u1) {
-    Walk w(tiles, X, n_tiles, u0);
+  if (units > 0) {
+    Walk w(tiles, X, first, count, n_first, beside);
     if (warp == 0) {
       // ------------------------------------------------------------------ raw k-blocks of A
       // row r of a block: 128 bytes, 16-byte chunk j at chunk position j ^ (r & 7).  TMA brings the rows behind the expert's last too: their
       // results are not written
       int it = 0;
-      for (int u = u0; u < u1; ++u, w.next()) {
+      for (int u = 0; u < units; ++u, w.next()) {
         const long long row0 = p.groups.first(w.e) + (long long)w.m * BM;
         for (int kb = 0; kb < n_kb; ++kb, ++it) {
           const int s = it % STAGES;
@@ -336,12 +341,15 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
       }
     } else if (warp == 1) {
       // ------------------------------------------------------------------ MMAs (whole warp, one elected lane)
+      // A few MMAs are queued at most, and a wait takes as long as three of 64 columns: the next block is waited for in the middle of this one
+      // (at its end the tensor cores idled 450 of 830 clocks a block).
       const uint32_t idesc2 = wg::idesc_bf16_m128(2 * BN), idesc1 = wg::idesc_bf16_m128(BN);
       const uint32_t tm = uniform(tmem);
       const uint64_t desc0 = wg::desc_sw64(uniform(smem_u32(smem)));
+      const int total = units * n_kb;
       int it = 0, lt = 0, run = 0, run_phase = 0;         // lt: accumulations; run, run_phase: slot of the run's first block and its parity
-      for (int u = u0; u < u1; ++u) {
-        const bool ends = !resident || uniform((uint32_t)w.run_ends(u + 1 == u1));
+      for (int u = 0; u < units; ++u) {
+        const bool ends = !resident || uniform((uint32_t)w.run_ends()), begins = !resident || uniform((uint32_t)w.run_begins());
         int bs = run;
         uint32_t bp = run_phase;
         for (int k0 = 0; k0 < n_kb; k0 += SEG, ++lt) {
@@ -350,14 +358,18 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
           const uint32_t d = tm + (uint32_t)buf * ACC_COLS;
           for (int kb = k0; kb < k1; ++kb, ++it) {
             const int slot = it % A_SLOTS;
-            mbar_wait(&b_full[bs], bp, status);
-            mbar_wait(&s_full[slot], (it / A_SLOTS) & 1u, status);
+            if (begins) mbar_wait(&b_full[bs], bp, status);
+            if (it == 0) mbar_wait(&s_full[0], 0, status);
             __syncwarp();
             tc_fence_after();
             const uint32_t a = tm + A_COL0 + (uint32_t)(slot * A_COLS);
             const uint64_t b = desc_at(desc0, (uint32_t)(bs * B_BYTES));
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
+              if (ks == 1) {
+                if (it + 1 < total) mbar_wait(&s_full[(it + 1) % A_SLOTS], ((it + 1) / A_SLOTS) & 1u, status);
+                __syncwarp();
+              }
               const uint64_t w1 = desc_at(b, (uint32_t)(ks * 32)), w2 = desc_at(w1, B_PART), w3 = desc_at(w1, 2 * B_PART);
               const uint32_t v1 = a + (uint32_t)(ks * 8), v2 = v1 + KB / 2, v3 = v1 + KB;
               warp_mma_bf16_a_tmem(d, v1, w1, idesc2, kb > k0 || ks ? 1u : 0u);
@@ -381,7 +393,7 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
       int slot = resident ? n_kb % slots : 0;        // the first ones are split by the epilogue's warps
       uint32_t phase = resident && n_kb == slots ? 1u : 0u;
       auto next = [&] { if (++slot == slots) { slot = 0; phase ^= 1u; } };
-      for (int u = u0; u < u1; ++u, w.next()) {
+      for (int u = 0; u < units; ++u, w.next()) {
         if (!resident) {
           if (t == 0) {
             const unsigned char* src = p.split + ((size_t)w.e * n_tiles + w.n) * n_kb * B_BYTES;
@@ -393,7 +405,7 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
           }
           continue;
         }
-        if (u == u0 || !w.run_begins(false)) continue;
+        if (u == 0 || !w.run_begins()) continue;
         const float* W = p.W + (size_t)w.e * N * K;
         float v[32], ahead[32];
         load_weights<FORWARD, 64>(W, w.n * BN, N, K, 0, t, p.w_wide, v);
@@ -412,7 +424,7 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
       // ------------------------------------------------------------------ split A into tensor memory
       const int row = (warp & 3) * 32 + lane, set = (warp - 4) >> 2;
       const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + A_COL0;
-      const int total = (u1 - u0) * n_kb;
+      const int total = units * n_kb;
       for (int it = set; it < total; it += 2) {
         const int s = it % STAGES, slot = it % A_SLOTS;
         mbar_wait(&a_full[s], (it / STAGES) & 1u, status);
@@ -469,12 +481,12 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
       float* bias = biases + (warp - 12) * 32;
       const uint32_t cols = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 32);
       int lt = 0;
-      for (int u = u0; u < u1; ++u, w.next()) {
+      for (int u = 0; u < units; ++u, w.next()) {
         const long long begin = p.groups.first(w.e), left = p.groups.first(w.e + 1) - begin - (long long)w.m * BM;
         const int rows = (int)(left < BM ? left : BM) - quarter * 32, n0 = w.n * BN + half * 32;      // of this warp
         const size_t row0 = (size_t)(begin + (long long)w.m * BM + quarter * 32);
         const bool mine = lane < rows;
-        if (FORWARD && w.run_begins(u == u0)) bias[lane] = p.bias && n0 + lane < N ? p.bias[(size_t)w.e * N + n0 + lane] : 0.f;
+        if (FORWARD && w.run_begins()) bias[lane] = p.bias && n0 + lane < N ? p.bias[(size_t)w.e * N + n0 + lane] : 0.f;
         for (int k0 = 0; k0 < n_kb; k0 += SEG, ++lt) {
           const int buf = lt & 1;
           const float gain = GAIN * (float)((min(K, (k0 + SEG) * KB) - k0 * KB + 15) / 16);

@@ -122,14 +122,20 @@ __global__ void __launch_bounds__(NTW, 1) product_wgrad_tc_kernel(const __grid_c
       for (int i = 0; i < n_blocks; ++i) {
         const int slot = i % A_SLOTS, bs = i % SLOTS_W, seg = i / SEG_W, buf = seg & 1;
         if (i % SEG_W == 0) mbar_wait(&acc_empty[buf], ((seg >> 1) & 1u) ^ 1u, status);
-        mbar_wait(&b_full[bs], (i / SLOTS_W) & 1u, status);
-        mbar_wait(&s_full[slot], (i / A_SLOTS) & 1u, status);
+        if (i == 0) { mbar_wait(&b_full[0], 0, status); mbar_wait(&s_full[0], 0, status); }
         __syncwarp();
         tc_fence_after();
         const uint32_t d = tm + (uint32_t)buf * ACC_COLS, a = tm + A_COL0 + (uint32_t)(slot * A_COLS);
         const uint64_t b = desc_at(desc0, (uint32_t)(bs * B_BYTES));
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
+          if (ks == 1) {                           // the next block is waited for while this one's MMAs run
+            if (i + 1 < n_blocks) {
+              mbar_wait(&b_full[(i + 1) % SLOTS_W], ((i + 1) / SLOTS_W) & 1u, status);
+              mbar_wait(&s_full[(i + 1) % A_SLOTS], ((i + 1) / A_SLOTS) & 1u, status);
+            }
+            __syncwarp();
+          }
           const uint64_t w1 = desc_at(b, (uint32_t)(ks * 32)), w2 = desc_at(w1, B_PART), w3 = desc_at(w1, 2 * B_PART);
           const uint32_t v1 = a + (uint32_t)(ks * 8), v2 = v1 + KB / 2, v3 = v1 + KB;
           warp_mma_bf16_a_tmem(d, v1, w1, idesc2, i % SEG_W || ks ? 1u : 0u);
