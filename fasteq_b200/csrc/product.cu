@@ -2,6 +2,8 @@
 //   z = x W[e]^T + bias[e],  y = act(z) + residual;   gz = grad_y act'(z):  grad_x = gz W[e],  grad_w[e] = gz^T x,  grad_bias[e] = sum gz
 // FMA kernels for every extent, FP32 and FP64: 64 x 64 tiles of 4 x 4 sums a thread.
 #include <algorithm>
+#include <atomic>
+#include <mutex>
 #include <cstdint>
 #include <cuda_runtime.h>
 #include "fasteq_b200.h"
@@ -200,6 +202,43 @@ int dgrad(const fasteq_product_problem* p, const void* g, const void* slope, con
                                          (const T*)nullptr, (const T*)nullptr, p->n, p->k, slope_pitch(p), 0, (T*)gx, (T*)nullptr);
   return e == cudaSuccess ? FASTEQ_OK : cuda_fail(e);
 }
+// What a launch needs to know of the current device, asked once: a microsecond or two a call otherwise.
+struct Device {
+  std::atomic<bool> known{false};
+  int sms = 0;
+  int* status = nullptr;                  // the tensor-core kernels' status word
+};
+constexpr int MAX_DEVICES = 64;
+cudaError_t current_device(int* index, Device** device) {
+  static Device devices[MAX_DEVICES];
+  cudaError_t e = cudaGetDevice(index);
+  if (e != cudaSuccess) return e;
+  if (*index >= MAX_DEVICES) return cudaErrorInvalidDevice;
+  Device& d = devices[*index];
+  if (!d.known.load(std::memory_order_acquire)) {      // two threads that get here write the same
+    int sms = 0;
+    int* status = nullptr;
+    e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, *index);
+    if (e == cudaSuccess) e = tc::status_word(&status);
+    if (e != cudaSuccess) return e;
+    static std::mutex lock;
+    std::lock_guard<std::mutex> g(lock);
+    d.sms = sms;
+    d.status = status;
+    d.known.store(true, std::memory_order_release);
+  }
+  *device = &d;
+  return cudaSuccess;
+}
+// lets a kernel have all of an SM's shared memory on a device, once
+template <auto KERNEL> cudaError_t allow_shared_memory(int device) {
+  static std::atomic<uint64_t> done{0};
+  if (done.load(std::memory_order_relaxed) >> device & 1) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+  if (e == cudaSuccess) done.fetch_or(uint64_t(1) << device, std::memory_order_relaxed);
+  return e;
+}
+
 // CTAs of a launch over tiles of rows and columns
 bool in_32_bits(const fasteq_product_problem* p, int tile) {
   const long long columns = (std::max(p->k, p->n) + tile - 1) / tile, rows = p->rows / tile + p->experts + 1;
@@ -214,7 +253,9 @@ template <bool FORWARD, bool SLOPE>
 int product_f64(const fasteq_product_problem* p, const void* A, const void* slope, const void* w, const void* bias, const void* residual, const int32_t* offsets, void* C,
                 void* slope_out, cudaStream_t s) {
   const int K = FORWARD ? p->k : p->n, N = FORWARD ? p->n : p->k, tiles_n = (N + pf64::TILE - 1) / pf64::TILE;
-  cudaError_t e = cudaFuncSetAttribute(pf64::product_f64_kernel<FORWARD, SLOPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, pf64::smem_bytes<SLOPE>());
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = allow_shared_memory<pf64::product_f64_kernel<FORWARD, SLOPE>>(dev);
   if (e == cudaSuccess)
     e = launch_dependent(pf64::product_f64_kernel<FORWARD, SLOPE>, (unsigned)(tile_numbers<pf64::TILE>(p->rows, p->experts + 1) * tiles_n), pf64::NT,
                          pf64::smem_bytes<SLOPE>(), s, groups_of(p, offsets), (const double*)A, (const double*)slope, (const double*)w, (const double*)bias,
@@ -249,7 +290,9 @@ int wgrad_f64(const fasteq_product_problem* p, int size, const void* x, const vo
               cudaStream_t s) {
   const Groups groups = groups_of(p, offsets);
   const int tiles_k = (p->k + pf64::TILE - 1) / pf64::TILE, tiles = tiles_k * ((p->n + pf64::TILE - 1) / pf64::TILE);
-  cudaError_t e = cudaFuncSetAttribute(pf64::product_wgrad_f64_kernel<SLOPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, pf64::smem_bytes<SLOPE>());
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = allow_shared_memory<pf64::product_wgrad_f64_kernel<SLOPE>>(dev);
   if (e == cudaSuccess)
     e = launch_dependent(pf64::product_wgrad_f64_kernel<SLOPE>, (unsigned)((p->rows / size + p->experts) * tiles), pf64::NT, pf64::smem_bytes<SLOPE>(), s, groups,
                          (const double*)x, (const double*)g, (const double*)slope, p->k, p->n, size, tiles_k, tiles, even(p->k, {x}), even(p->n, {g, slope}), (double*)gw,
@@ -331,10 +374,10 @@ Scratch scratch_of(const fasteq_product_problem* p, bool backward) {
 }
 
 template <bool FORWARD, bool SLOPE, int ACT>
-int launch_tc(const fasteq_product_problem* p, ptc::Args& a, int sms, const CUtensorMap (&tm)[4], cudaStream_t s) {
+int launch_tc(const fasteq_product_problem* p, ptc::Args& a, int dev, int sms, const CUtensorMap (&tm)[4], cudaStream_t s) {
   a.slots = ptc::Cfg<SLOPE>::slots(p->experts);
   const int smem = ptc::Cfg<SLOPE>::smem(a.slots, p->experts);
-  cudaError_t e = cudaFuncSetAttribute(ptc::product_tc_kernel<FORWARD, SLOPE, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = allow_shared_memory<ptc::product_tc_kernel<FORWARD, SLOPE, ACT>>(dev);
   if (e == cudaSuccess)
     e = launch_dependent(ptc::product_tc_kernel<FORWARD, SLOPE, ACT>, (unsigned)std::min<long long>(sms, most_units(p, a.K, a.N)), ptc::NT, smem, s, a, tm[0], tm[1],
                          tm[2], tm[3]);
@@ -351,10 +394,12 @@ int run_tc(const fasteq_product_problem* p, const void* A, int lda, const void* 
   a.C = (float*)C; a.slope_out = (float*)slope_out;
   a.K = FORWARD ? p->k : p->n; a.N = FORWARD ? p->n : p->k; a.lda = lda; a.ldd = slope_pitch(p);
   a.w_wide = wide(p->k, {W}); a.c_wide = wide(a.N, {C, residual});
-  int sms = 0, dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (e == cudaSuccess) e = tc::status_word(&a.status);
+  int dev = 0;
+  Device* device = nullptr;
+  cudaError_t e = current_device(&dev, &device);
+  if (e != cudaSuccess) return cuda_fail(e);
+  a.status = device->status;
+  const int sms = device->sms;
   if (e == cudaSuccess && split) {
     const int n_tiles = (a.N + ptc::BN - 1) / ptc::BN, n_kb = (a.K + ptc::KB - 1) / ptc::KB;
     e = launch_dependent(ptc::split_weights_kernel<FORWARD>, (unsigned)((int64_t)p->experts * n_tiles * n_kb), 256, 0, s, a.W, (unsigned char*)split, a.N, a.K, n_tiles,
@@ -372,13 +417,13 @@ int run_tc(const fasteq_product_problem* p, const void* A, int lda, const void* 
   if (a.c_wide) map(2, a.C, a.N, a.N, 32);
   map(3, a.slope_out, a.N, a.ldd, 32);
   if (rc != FASTEQ_OK) return rc;
-  if (!FORWARD) return slope ? launch_tc<false, true, kIdentity>(p, a, sms, tm, s) : launch_tc<false, false, kIdentity>(p, a, sms, tm, s);
+  if (!FORWARD) return slope ? launch_tc<false, true, kIdentity>(p, a, dev, sms, tm, s) : launch_tc<false, false, kIdentity>(p, a, dev, sms, tm, s);
   switch (p->act) {
-    case kSilu: return launch_tc<true, false, kSilu>(p, a, sms, tm, s);
-    case kTanh: return launch_tc<true, false, kTanh>(p, a, sms, tm, s);
-    case kSigmoid: return launch_tc<true, false, kSigmoid>(p, a, sms, tm, s);
-    case kAbs: return launch_tc<true, false, kAbs>(p, a, sms, tm, s);
-    default: return launch_tc<true, false, kIdentity>(p, a, sms, tm, s);
+    case kSilu: return launch_tc<true, false, kSilu>(p, a, dev, sms, tm, s);
+    case kTanh: return launch_tc<true, false, kTanh>(p, a, dev, sms, tm, s);
+    case kSigmoid: return launch_tc<true, false, kSigmoid>(p, a, dev, sms, tm, s);
+    case kAbs: return launch_tc<true, false, kAbs>(p, a, dev, sms, tm, s);
+    default: return launch_tc<true, false, kIdentity>(p, a, dev, sms, tm, s);
   }
 }
 
@@ -400,8 +445,11 @@ int wgrad_tc(const fasteq_product_problem* p, const void* x, int ldx, const void
   };
   map(0, a.g, p->n, ldg, pwg::TM); map(1, a.slope, p->n, a.ldd, pwg::TM); map(2, a.x, p->k, ldx, pwg::TN);
   if (rc != FASTEQ_OK) return rc;
-  cudaError_t e = tc::status_word(&a.status);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(pwg::product_wgrad_tc_kernel<SLOPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, pwg::CfgW<SLOPE>::SMEM);
+  int dev = 0;
+  Device* device = nullptr;
+  cudaError_t e = current_device(&dev, &device);
+  if (e == cudaSuccess) a.status = device->status;
+  if (e == cudaSuccess) e = allow_shared_memory<pwg::product_wgrad_tc_kernel<SLOPE>>(dev);
   if (e == cudaSuccess)
     e = launch_dependent(pwg::product_wgrad_tc_kernel<SLOPE>, (unsigned)((p->rows / a.size + p->experts) * a.tiles), pwg::NTW, pwg::CfgW<SLOPE>::SMEM, s, a, tm[0], tm[1],
                          tm[2]);
