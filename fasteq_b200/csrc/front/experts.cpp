@@ -58,6 +58,7 @@ variable_list run_backward(const Tensor& x, at::IntArrayRef shape, const Tensor&
   fasteq_product_problem p{};
   p.dtype = gc.scalar_type() == at::kDouble ? FASTEQ_F64 : FASTEQ_F32;
   p.experts = (int32_t)shape[0]; p.n = (int32_t)shape[1]; p.k = (int32_t)shape[2]; p.inner = (int32_t)inner; p.rows = gc.size(0);
+  p.act = slope.defined() ? (int32_t)kSilu : (int32_t)kIdentity;      // whether there is a slope is what counts here
   Tensor gx = need_x ? at::empty({gc.size(0), shape[2]}, gc.options()) : Tensor();
   Tensor gw = need_w || need_b ? at::empty(shape, gc.options()) : Tensor();
   Tensor gb = need_b ? at::empty({shape[0], shape[1]}, gc.options()) : Tensor();

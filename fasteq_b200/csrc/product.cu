@@ -249,17 +249,17 @@ bool even(int extent, std::initializer_list<const void*> pointers) {
   for (const void* q : pointers) all |= reinterpret_cast<uintptr_t>(q);
   return extent % 2 == 0 && (all & 15u) == 0;
 }
-template <bool FORWARD, bool SLOPE>
-int product_f64(const fasteq_product_problem* p, const void* A, const void* slope, const void* w, const void* bias, const void* residual, const int32_t* offsets, void* C,
-                void* slope_out, cudaStream_t s) {
+template <bool FORWARD>
+int product_f64(const fasteq_product_problem* p, const void* A, const void* w, const void* bias, const void* residual, const int32_t* offsets, void* C, void* slope_out,
+                cudaStream_t s) {
   const int K = FORWARD ? p->k : p->n, N = FORWARD ? p->n : p->k, tiles_n = (N + pf64::TILE - 1) / pf64::TILE;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = allow_shared_memory<pf64::product_f64_kernel<FORWARD, SLOPE>>(dev);
+  if (e == cudaSuccess) e = allow_shared_memory<pf64::product_f64_kernel<FORWARD>>(dev);
   if (e == cudaSuccess)
-    e = launch_dependent(pf64::product_f64_kernel<FORWARD, SLOPE>, (unsigned)(tile_numbers<pf64::TILE>(p->rows, p->experts + 1) * tiles_n), pf64::NT,
-                         pf64::smem_bytes<SLOPE>(), s, groups_of(p, offsets), (const double*)A, (const double*)slope, (const double*)w, (const double*)bias,
-                         (const double*)residual, K, N, p->act, tiles_n, even(K, {A, slope}), even(p->k, {w}), (double*)C, (double*)slope_out);
+    e = launch_dependent(pf64::product_f64_kernel<FORWARD>, (unsigned)(tile_numbers<pf64::TILE>(p->rows, p->experts + 1) * tiles_n), pf64::NT, pf64::SMEM, s,
+                         groups_of(p, offsets), (const double*)A, (const double*)w, (const double*)bias, (const double*)residual, K, N, p->act, tiles_n, even(K, {A}),
+                         even(p->k, {w}), (double*)C, (double*)slope_out);
   return e == cudaSuccess ? FASTEQ_OK : cuda_fail(e);
 }
 
@@ -285,18 +285,15 @@ template <typename T> int reduce(const fasteq_product_problem* p, const Groups& 
   return e == cudaSuccess ? FASTEQ_OK : cuda_fail(e);
 }
 
-template <bool SLOPE>
-int wgrad_f64(const fasteq_product_problem* p, int size, const void* x, const void* g, const void* slope, const int32_t* offsets, void* gw, void* gb, void* scratch,
-              cudaStream_t s) {
+int wgrad_f64(const fasteq_product_problem* p, int size, const void* x, const void* g, const int32_t* offsets, void* gw, void* gb, void* scratch, cudaStream_t s) {
   const Groups groups = groups_of(p, offsets);
   const int tiles_k = (p->k + pf64::TILE - 1) / pf64::TILE, tiles = tiles_k * ((p->n + pf64::TILE - 1) / pf64::TILE);
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = allow_shared_memory<pf64::product_wgrad_f64_kernel<SLOPE>>(dev);
+  if (e == cudaSuccess) e = allow_shared_memory<pf64::product_wgrad_f64_kernel>(dev);
   if (e == cudaSuccess)
-    e = launch_dependent(pf64::product_wgrad_f64_kernel<SLOPE>, (unsigned)((p->rows / size + p->experts) * tiles), pf64::NT, pf64::smem_bytes<SLOPE>(), s, groups,
-                         (const double*)x, (const double*)g, (const double*)slope, p->k, p->n, size, tiles_k, tiles, even(p->k, {x}), even(p->n, {g, slope}), (double*)gw,
-                         (double*)gb, (double*)scratch);
+    e = launch_dependent(pf64::product_wgrad_f64_kernel, (unsigned)((p->rows / size + p->experts) * tiles), pf64::NT, pf64::SMEM, s, groups, (const double*)x,
+                         (const double*)g, p->k, p->n, size, tiles_k, tiles, even(p->k, {x}), even(p->n, {g}), (double*)gw, (double*)gb, (double*)scratch);
   return e == cudaSuccess ? reduce<double>(p, groups, size, gw, gb, scratch, s) : cuda_fail(e);
 }
 
@@ -326,27 +323,29 @@ bool on_tensor_cores(const fasteq_product_problem* p) {
   return p->dtype == FASTEQ_F32 && p->k > 0 && p->n > 0 && p->rows > 0 && p->rows <= 0x7fffffffLL && most_units(p, p->k, p->n) > 0 && most_units(p, p->n, p->k) > 0;
 }
 
-// dst [rows, (columns + 3) & ~3] = src [rows, columns] (times slope), for rows that TMA cannot take as they lie
-__global__ void __launch_bounds__(256) align_rows_kernel(const float* src, const float* slope, int columns, int ldd, long long rows, float* dst) {
-  const int c = threadIdx.x * 4, pitch = (columns + 3) & ~3;
+// dst [rows, pitch] = src [rows, columns] (times slope, rows of ldd), zeros behind: rows that TMA cannot take as they lie, and FP64's gz
+template <typename T, int V> __global__ void __launch_bounds__(256) align_rows_kernel(const T* src, const T* slope, int columns, int ldd, int pitch, long long rows, T* dst) {
+  struct alignas(sizeof(T) * V) Pack { T v[V]; };
   wait_for_previous_kernel();
   for (long long r = (long long)blockIdx.x * blockDim.y + threadIdx.y; r < rows; r += (long long)gridDim.x * blockDim.y)
-    for (int k = c; k < pitch; k += blockDim.x * 4) {
-      float v[4];
+    for (int k = threadIdx.x * V; k < pitch; k += blockDim.x * V) {
+      Pack x{};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[i] = k + i < columns ? src[r * columns + k + i] : 0.f;
-        if (slope && k + i < columns) v[i] *= slope[r * ldd + k + i];
+      for (int i = 0; i < V; ++i) {
+        if (k + i < columns) x.v[i] = src[r * columns + k + i];
+        if (slope && k + i < columns) x.v[i] *= slope[r * ldd + k + i];
       }
-      *reinterpret_cast<float4*>(dst + r * pitch + k) = make_float4(v[0], v[1], v[2], v[3]);
+      *reinterpret_cast<Pack*>(dst + r * pitch + k) = x;
     }
 }
-cudaError_t align_rows(const void* src, const void* slope, int columns, int ldd, long long rows, void* dst, cudaStream_t s) {
+template <typename T> cudaError_t align_rows(const void* src, const void* slope, int columns, int ldd, int pitch, long long rows, void* dst, cudaStream_t s) {
+  constexpr int V = 16 / sizeof(T);
+  const bool packs = pitch % V == 0;
   int tx = 1;
-  while (tx * 4 < columns && tx < 32) tx *= 2;
+  while (tx * (packs ? V : 1) < columns && tx < 32) tx *= 2;
   const dim3 block((unsigned)tx, (unsigned)(256 / tx));
-  return launch_dependent(align_rows_kernel, (unsigned)std::min<long long>((rows + block.y - 1) / block.y, 148 * 32), block, 0, s, (const float*)src,
-                          (const float*)slope, columns, ldd, rows, (float*)dst);
+  return launch_dependent(packs ? align_rows_kernel<T, V> : align_rows_kernel<T, 1>, (unsigned)std::min<long long>((rows + block.y - 1) / block.y, 148 * 32), block, 0, s,
+                          (const T*)src, (const T*)slope, columns, ldd, pitch, rows, (T*)dst);
 }
 
 // A call's scratch: the aligned copies, the weights split beforehand (none where a CTA keeps them), the weight gradient's partial sums.
@@ -366,6 +365,7 @@ Scratch scratch_of(const fasteq_product_problem* p, bool backward) {
     if (backward && p->n % 4) r.g = round16(p->rows * ((p->n + 3) & ~3) * size);
     if (n_kb > slots) r.split = (int64_t)p->experts * ((N + ptc::BN - 1) / ptc::BN) * n_kb * ptc::B_BYTES;
   }
+  if (backward && p->dtype == FASTEQ_F64 && p->k > 0 && p->act != kIdentity) r.g = round16(p->rows * p->n * size);
   if (backward && p->rows > 0) {
     const int rows = chunk_rows(p, tensor);
     if (p->rows > rows) r.partial = partial_slots(p->rows, rows) * ((int64_t)p->n * p->k + p->n) * size;
@@ -476,7 +476,7 @@ extern "C" int fasteq_product_forward(const fasteq_product_problem* p, const voi
   if (on_tensor_cores(p) && (need.x || wide(0, {x})) && wide(0, {slope, scratch})) {
     char* at = (char*)scratch;
     if (need.x) {
-      const cudaError_t e = align_rows(x, nullptr, p->k, 0, p->rows, at, s);
+      const cudaError_t e = align_rows<float>(x, nullptr, p->k, 0, (p->k + 3) & ~3, p->rows, at, s);
       if (e != cudaSuccess) return cuda_fail(e);
       x = at;
       at += need.x;
@@ -485,7 +485,7 @@ extern "C" int fasteq_product_forward(const fasteq_product_problem* p, const voi
   }
   if (p->dtype == FASTEQ_F32) return forward<float>(p, x, w, bias, residual, offsets, y, slope, s);
   if (p->k == 0 || !in_32_bits(p, pf64::TILE)) return forward<double>(p, x, w, bias, residual, offsets, y, slope, s);
-  return product_f64<true, false>(p, x, nullptr, w, bias, residual, offsets, y, slope, s);
+  return product_f64<true>(p, x, w, bias, residual, offsets, y, slope, s);
 }
 
 extern "C" int fasteq_product_backward(const fasteq_product_problem* p, const void* x, const void* w, const void* grad_y, const void* slope,
@@ -493,11 +493,12 @@ extern "C" int fasteq_product_backward(const fasteq_product_problem* p, const vo
                                        fasteq_stream_t stream) {
   if (const int rc = check(p, offsets)) return rc;
   if (!grad_x && !grad_w && !grad_bias) return FASTEQ_OK;
+  if (p->act == kIdentity) slope = nullptr;
   if (grad_bias && !grad_w && p->k > 0) return FASTEQ_INVALID;
   const bool sums = grad_w || grad_bias, there = p->rows > 0 && p->n > 0;
   const Scratch need = scratch_of(p, true);
   if (need.total() > 0 && (!scratch || scratch_bytes < need.total())) return FASTEQ_INVALID;
-  if (there && (!grad_y || (grad_x && p->k > 0 && !w) || (sums && p->k > 0 && !x))) return FASTEQ_INVALID;
+  if (there && (!grad_y || (p->act != kIdentity && !slope) || (grad_x && p->k > 0 && !w) || (sums && p->k > 0 && !x))) return FASTEQ_INVALID;
   cudaStream_t s = (cudaStream_t)stream;
   const size_t size = p->dtype == FASTEQ_F32 ? 4 : 8;
   cudaError_t e = cudaSuccess;
@@ -512,12 +513,12 @@ extern "C" int fasteq_product_backward(const fasteq_product_problem* p, const vo
   if (on_tensor_cores(p) && (need.g || wide(0, {grad_y})) && (need.x || !sums || wide(0, {x})) && wide(0, {slope, scratch})) {
     const int ldg = (p->n + 3) & ~3, ldx = (p->k + 3) & ~3;
     if (need.g) {                         // with the slope multiplied in, then
-      e = align_rows(grad_y, slope, p->n, ldg, p->rows, g_at, s);
+      e = align_rows<float>(grad_y, slope, p->n, ldg, ldg, p->rows, g_at, s);
       grad_y = g_at;
       slope = nullptr;
     }
     if (sums && need.x && e == cudaSuccess) {
-      e = align_rows(x, nullptr, p->k, 0, p->rows, x_at, s);
+      e = align_rows<float>(x, nullptr, p->k, 0, ldx, p->rows, x_at, s);
       x = x_at;
     }
     if (e != cudaSuccess) return cuda_fail(e);
@@ -529,10 +530,13 @@ extern "C" int fasteq_product_backward(const fasteq_product_problem* p, const vo
   }
   const int rows = chunk_rows(p, on_tensor_cores(p));      // as the scratch was counted with
   if (p->dtype == FASTEQ_F64 && p->k > 0 && in_32_bits(p, pf64::TILE)) {
-    if (grad_x) rc = slope ? product_f64<false, true>(p, grad_y, slope, w, nullptr, nullptr, offsets, grad_x, nullptr, s)
-                           : product_f64<false, false>(p, grad_y, nullptr, w, nullptr, nullptr, offsets, grad_x, nullptr, s);
-    if (rc == FASTEQ_OK && sums) rc = slope ? wgrad_f64<true>(p, rows, x, grad_y, slope, offsets, grad_w, grad_bias, partial_at, s)
-                                            : wgrad_f64<false>(p, rows, x, grad_y, nullptr, offsets, grad_w, grad_bias, partial_at, s);
+    if (slope) {
+      e = align_rows<double>(grad_y, slope, p->n, p->n, p->n, p->rows, g_at, s);
+      if (e != cudaSuccess) return cuda_fail(e);
+      grad_y = g_at;
+    }
+    if (grad_x) rc = product_f64<false>(p, grad_y, w, nullptr, nullptr, offsets, grad_x, nullptr, s);
+    if (rc == FASTEQ_OK && sums) rc = wgrad_f64(p, rows, x, grad_y, offsets, grad_w, grad_bias, partial_at, s);
     return rc;
   }
   const bool f32 = p->dtype == FASTEQ_F32;

@@ -17,7 +17,8 @@ using product::Groups;
 
 constexpr int TILE = 64, BK = 16, NT = 128, STAGES = 3, OUTER_PITCH = BK + 4, K_PITCH = TILE + 4;
 constexpr int OPERAND = TILE * OUTER_PITCH;          // doubles of an operand's stage, either way round
-template <bool SLOPE> constexpr int smem_bytes() { return STAGES * (SLOPE ? 3 : 2) * OPERAND * 8; }
+constexpr int SMEM = STAGES * 2 * OPERAND * 8;
+static_assert(SMEM >= TILE * (TILE + 2) * 8, "the turned tile of the forward");
 
 __device__ __forceinline__ void copy_async(double* dst, const double* src, bool pair, int there) {      // there: 0, 1 or 2 values
   if (pair) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(there * 8) : "memory");
@@ -57,23 +58,21 @@ template <bool OUTER> __device__ __forceinline__ void load_step(double* dst, con
 
 struct Operand {
   const double* src;
-  const double* slope;                 // multiplied in, same shape; or null
-  long long ld, ld_slope;
+  long long ld;
   int outer;                           // values there are in the tile
   bool pair;
 };
 
 // sum[i][j]: the 8 x 8 blocks of this warp's 32 x 32 outputs; column: sums over k of operand A's outer index `threadIdx.x` (COLUMNS)
-template <bool A_OUTER, bool B_OUTER, bool SLOPE, bool COLUMNS>
+template <bool A_OUTER, bool B_OUTER, bool COLUMNS>
 __device__ __forceinline__ void multiply(double* smem, const Operand& a, const Operand& b, int depth, double (&sum)[4][4][2], double& column) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, m0 = (warp >> 1) * 32, n0 = (warp & 1) * 32, steps = (depth + BK - 1) / BK;
-  constexpr int STAGE = (SLOPE ? 3 : 2) * OPERAND;
+  constexpr int STAGE = 2 * OPERAND;
   auto load = [&](int step) {
     double* st = smem + step % STAGES * STAGE;
     if (step < steps) {
       load_step<A_OUTER>(st, a.src, a.ld, a.outer, step * BK, depth, a.pair);
       load_step<B_OUTER>(st + OPERAND, b.src, b.ld, b.outer, step * BK, depth, b.pair);
-      if (SLOPE) load_step<A_OUTER>(st + 2 * OPERAND, a.slope, a.ld_slope, a.outer, step * BK, depth, a.pair);
     }
     commit_async();
   };
@@ -82,11 +81,6 @@ __device__ __forceinline__ void multiply(double* smem, const Operand& a, const O
   for (int step = 0; step < steps; ++step) {
     double* st = smem + step % STAGES * STAGE;
     wait_async<STAGES - 2>();
-    if (SLOPE)                           // each thread its own copies, before the others read them
-      each_copy<A_OUTER>(a.pair, [&](int at, int, int) {
-        st[at] *= st[2 * OPERAND + at];
-        if (a.pair) st[at + 1] *= st[2 * OPERAND + at + 1];
-      });
     __syncthreads();
     load(step + STAGES - 1);             // into the stage that the step before has read
 #pragma unroll
@@ -121,11 +115,11 @@ template <typename F> __device__ __forceinline__ void each_output(const double (
     for (int j = 0; j < 4; ++j) f(m + 8 * i, n + 8 * j, sum[i][j]);
 }
 
-// One tile of C = epilogue((A slope) op(W)); see product_kernel
-template <bool FORWARD, bool SLOPE>
-__global__ void __launch_bounds__(NT, 3) product_f64_kernel(Groups groups, const double* A, const double* slope, const double* W, const double* bias,
-                                                            const double* residual, int K, int N, int act, int tiles_n, bool pair_a, bool pair_w, double* C,
-                                                            double* slope_out) {
+// One tile of C = epilogue(A op(W)); see product_kernel.  The forward turns its tile in shared memory and walks it in a loop: one copy of the
+// activations' code, whole lines stored.
+template <bool FORWARD>
+__global__ void __launch_bounds__(NT, 3) product_f64_kernel(Groups groups, const double* A, const double* W, const double* bias, const double* residual, int K, int N, int act,
+                                                            int tiles_n, bool pair_a, bool pair_w, double* C, double* slope_out) {
   extern __shared__ __align__(16) double smem_f64[];
   wait_for_previous_kernel();
   long long m0;
@@ -133,44 +127,52 @@ __global__ void __launch_bounds__(NT, 3) product_f64_kernel(Groups groups, const
   const int e = product::tile_of<TILE>(groups, groups.experts + 1, blockIdx.x / tiles_n, &m0, &m_rows), n0 = (int)(blockIdx.x % tiles_n) * TILE;
   if (m_rows == 0) return;
   double sum[4][4][2] = {}, none = 0.0;
-  if (e < groups.experts) {
+  const bool routed = e < groups.experts;
+  if (routed) {
     const double* w = W + (size_t)e * N * K;
-    const Operand a{A + m0 * K, SLOPE ? slope + m0 * K : nullptr, K, K, m_rows, pair_a};
-    const Operand b{FORWARD ? w + (size_t)n0 * K : w + n0, nullptr, FORWARD ? K : N, 0, min(TILE, N - n0), pair_w};
-    multiply<true, FORWARD, SLOPE, false>(smem_f64, a, b, K, sum, none);
+    const Operand a{A + m0 * K, K, m_rows, pair_a}, b{FORWARD ? w + (size_t)n0 * K : w + n0, FORWARD ? K : N, min(TILE, N - n0), pair_w};
+    multiply<true, FORWARD, false>(smem_f64, a, b, K, sum, none);
   }
-  each_output(sum, [&](int r, int c, const double (&v)[2]) {
+  if (!FORWARD) {
+    each_output(sum, [&](int r, int c, const double (&v)[2]) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int n = n0 + c + h;
-      if (r >= m_rows || n >= N) continue;
-      const size_t at = (size_t)(m0 + r) * N + n;
-      double y = v[h], d = 1.0;
-      if (FORWARD && e < groups.experts) {
-        if (bias) y += bias[(size_t)e * N + n];
-        y = product::activate(act, y, d);
-        if (residual) y += residual[at];
-      }
-      C[at] = y;
-      if (FORWARD && slope_out) slope_out[at] = d;
+      for (int h = 0; h < 2; ++h)
+        if (r < m_rows && n0 + c + h < N) C[(size_t)(m0 + r) * N + n0 + c + h] = v[h];
+    });
+    return;
+  }
+  constexpr int PITCH = TILE + 2;
+  __syncthreads();                       // the last step has been read
+  each_output(sum, [&](int r, int c, const double (&v)[2]) { *reinterpret_cast<double2*>(smem_f64 + r * PITCH + c) = make_double2(v[0], v[1]); });
+  __syncthreads();
+  const int c = threadIdx.x % TILE, n = n0 + c;
+  if (n >= N) return;
+  const double b = bias && routed ? bias[(size_t)e * N + n] : 0.0;
+#pragma unroll 2
+  for (int r = threadIdx.x / TILE; r < m_rows; r += NT / TILE) {
+    const size_t at = (size_t)(m0 + r) * N + n;
+    double d = 0.0, y = 0.0;
+    if (routed) {
+      y = product::activate(act, smem_f64[r * PITCH + c] + b, d);
+      if (residual) y += residual[at];
     }
-  });
+    C[at] = y;
+    if (slope_out) slope_out[at] = d;
+  }
 }
 
 // A chunk of an expert's rows and a tile of its matrix; see product_wgrad_kernel
-template <bool SLOPE>
-__global__ void __launch_bounds__(NT, 3) product_wgrad_f64_kernel(Groups groups, const double* X, const double* G, const double* slope, int K, int N, int size, int tiles_k,
-                                                                  int tiles, bool pair_x, bool pair_g, double* gw, double* gb, double* partial) {
+__global__ void __launch_bounds__(NT, 3) product_wgrad_f64_kernel(Groups groups, const double* X, const double* G, int K, int N, int size, int tiles_k, int tiles, bool pair_x,
+                                                                  bool pair_g, double* gw, double* gb, double* partial) {
   extern __shared__ __align__(16) double smem_f64[];
   wait_for_previous_kernel();
   const Chunk c = product::chunk_of(groups, groups.experts, size, blockIdx.x / tiles);
   if (c.rows == 0) return;
   const int tile = (int)(blockIdx.x % tiles), n0 = tile / tiles_k * TILE, k0 = tile % tiles_k * TILE;
   double sum[4][4][2] = {}, column = 0.0;
-  const Operand a{G + c.m0 * N + n0, SLOPE ? slope + c.m0 * N + n0 : nullptr, N, N, min(TILE, N - n0), pair_g};
-  const Operand b{X + c.m0 * K + k0, nullptr, K, 0, min(TILE, K - k0), pair_x};
-  if (k0 == 0) multiply<false, false, SLOPE, true>(smem_f64, a, b, c.rows, sum, column);
-  else multiply<false, false, SLOPE, false>(smem_f64, a, b, c.rows, sum, column);
+  const Operand a{G + c.m0 * N + n0, N, min(TILE, N - n0), pair_g}, b{X + c.m0 * K + k0, K, min(TILE, K - k0), pair_x};
+  if (k0 == 0) multiply<false, false, true>(smem_f64, a, b, c.rows, sum, column);
+  else multiply<false, false, false>(smem_f64, a, b, c.rows, sum, column);
   const size_t nk = (size_t)N * K;
   const bool only = c.count == 1;
   double* dst = only ? gw + (size_t)c.e * nk : partial + (size_t)product::partial_slot(c, size) * (nk + N);

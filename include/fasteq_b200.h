@@ -463,7 +463,8 @@ int fasteq_product_scratch(const fasteq_product_problem* p /* host */, int32_t b
 int fasteq_product_forward(const fasteq_product_problem* p /* host */, const void* x, const void* w, const void* bias /* or NULL */,
                            const void* residual /* or NULL */, const int32_t* offsets /* or NULL */, void* y, void* slope /* or NULL */,
                            void* scratch, int64_t scratch_bytes, fasteq_stream_t stream);
-/* Any of the gradients may be NULL; grad_bias goes with grad_w.  w is read for grad_x, x for the others. */
+/* Any of the gradients may be NULL; grad_bias goes with grad_w.  w is read for grad_x, x for the others.  With an act other than the identity slope
+ * is needed, with the identity it is not read. */
 int fasteq_product_backward(const fasteq_product_problem* p /* host */, const void* x, const void* w, const void* grad_y,
                             const void* slope /* or NULL */, const int32_t* offsets /* or NULL */, void* grad_x, void* grad_w, void* grad_bias,
                             void* scratch, int64_t scratch_bytes, fasteq_stream_t stream);
