@@ -110,63 +110,89 @@ Tensor product_w(const Tensor& g, const Tensor& x, const Tensor& offsets, int64_
   return Bilinear::apply(g, x, optional_of(offsets), inner, (int64_t)2, shape.vec());
 }
 
-// The layer.  x [rows, K], w [experts, N, K], bias [experts, N], residual [rows, N]
+// The layer, in the caller's shapes: x [..., K], w [N, K] or [experts, N, K], bias [N] or [experts, N], residual like the result [..., N].  They are
+// brought into the kernels' inside the node: views before it would be nodes of their own in the backward, a few microseconds each.
 struct Layer : torch::autograd::Function<Layer> {
+  static Tensor matrix(const Tensor& w) { return w.dim() == 2 ? w.unsqueeze(0) : w; }
+  static Tensor vectors(const Tensor& b) { return b.defined() && b.dim() == 1 ? b.unsqueeze(0) : b; }
+  static Tensor rows(const Tensor& t, int64_t width) {
+    return !t.defined() || t.dim() == 2 ? t : t.reshape({c10::multiply_integers(t.sizes().begin(), t.sizes().end() - 1), width});
+  }
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const std::optional<Tensor>& bias, const std::optional<Tensor>& residual,
                         const std::optional<Tensor>& offsets, int64_t inner, int64_t act, bool differentiated) {
     const Tensor b = bias.value_or(Tensor()), o = offsets.value_or(Tensor());
     Tensor slope;
-    Tensor y = run_forward(x, w, b, residual.value_or(Tensor()), o, inner, act, differentiated && act != kIdentity ? &slope : nullptr);
+    Tensor y = run_forward(rows(x, w.size(-1)), matrix(w), vectors(b), rows(residual.value_or(Tensor()), w.size(-2)), o, inner, act,
+                           differentiated && act != kIdentity ? &slope : nullptr);
     ctx->save_for_backward({x, w, b, o, slope});
     ctx->saved_data["i"] = inner; ctx->saved_data["a"] = act; ctx->saved_data["r"] = residual.has_value();
-    return y;
+    if (x.dim() == 2) return y;
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = w.size(-2);
+    return y.view(shape);
   }
   static variable_list backward(AutogradContext* ctx, variable_list go) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &w = saved[1], &b = saved[2], &o = saved[3], &slope = saved[4], &g = go[0];
+    const Tensor &x = saved[0], &w = saved[1], &b = saved[2], &o = saved[3], &slope = saved[4];
     const int64_t inner = ctx->saved_data["i"].toInt(), act = ctx->saved_data["a"].toInt();
     // the context numbers the tensors it was given, not the places they could have had
     const bool has_b = b.defined(), has_r = ctx->saved_data["r"].toBool();
     const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = has_b && ctx->needs_input_grad(2);
     Tensor gx, gw, gb;
-    const Tensor gr = has_r && ctx->needs_input_grad(has_b ? 3 : 2) ? g : Tensor();
+    const Tensor gr = has_r && ctx->needs_input_grad(has_b ? 3 : 2) ? go[0] : Tensor();
+    const Tensor g = rows(go[0], w.size(-2)), x2 = rows(x, w.size(-1)), w3 = matrix(w);
     if (at::GradMode::is_enabled()) {
       // to be differentiated again.  The bias and its gradient are products with a column of ones, which stay inside the experts' rows
-      const Tensor ones = b.defined() ? at::ones({x.size(0), 1}, x.options()) : Tensor();
+      const Tensor b2 = vectors(b), ones = has_b ? at::ones({x2.size(0), 1}, x.options()) : Tensor();
       Tensor gz = g;
       if (act != kIdentity) {
-        Tensor z = product(x, w, o, inner);
-        if (b.defined()) z = z + product(ones, b.unsqueeze(2), o, inner);
+        Tensor z = product(x2, w3, o, inner);
+        if (has_b) z = z + product(ones, b2.unsqueeze(2), o, inner);
         if (act == kSilu) gz = silu_gradient(g.contiguous(), z.contiguous());
         else if (act == kTanh) gz = g * (1 - at::tanh(z).square());
         else if (act == kSigmoid) { const Tensor s = at::sigmoid(z); gz = g * (s * (1 - s)); }
         else gz = g * at::sgn(z).detach();
       }
-      if (need_x) gx = product_x(gz, w, o, inner);
-      if (need_w) gw = product_w(gz, x, o, inner, w.sizes());
-      if (need_b) gb = product_w(gz, ones, o, inner, {b.size(0), b.size(1), 1}).squeeze(2);
+      if (need_x) gx = product_x(gz, w3, o, inner);
+      if (need_w) gw = product_w(gz, x2, o, inner, w3.sizes());
+      if (need_b) gb = product_w(gz, ones, o, inner, {b2.size(0), b2.size(1), 1}).squeeze(2);
     } else {
-      auto d = run_backward(x, w.sizes(), w, g, slope, o, inner, need_x, need_w, need_b);
+      auto d = run_backward(x2, w3.sizes(), w3, g, slope, o, inner, need_x, need_w, need_b);
       gx = d[0]; gw = d[1]; gb = d[2];
     }
-    return {gx, gw, gb, gr, Tensor(), Tensor(), Tensor(), Tensor()};
+    auto shaped = [](const Tensor& t, const Tensor& like) { return t.defined() && t.dim() != like.dim() ? t.reshape(like.sizes()) : t; };
+    return {shaped(gx, x), shaped(gw, w), shaped(gb, b), gr, Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 
-// Checked by the callers in Python.  Rows of the last dimension; the result has x's leading extents.
+// CUDA tensors of one device and one type, float32 or float64
+void check_operand(const char* name, const char* what, const Tensor& t, const Tensor& first) {
+  if (!t.is_cuda()) TORCH_CHECK(false, name, ": ", what, " must be a CUDA tensor: fasteq_b200 has no CPU path");
+  TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat || t.scalar_type() == at::kDouble, name, ": only float32 and float64 are supported; ", what, " is ", t.scalar_type());
+  TORCH_CHECK_VALUE(t.scalar_type() == first.scalar_type() && t.device() == first.device(), name, ": all operands must have one dtype and one device; ", what, " is ",
+                    t.scalar_type(), " on ", t.device(), ", not ", first.scalar_type(), " on ", first.device());
+}
+void check_operand(const char* name, const char* what, const std::optional<Tensor>& t, const Tensor& first) {
+  if (t) check_operand(name, what, *t, first);
+}
+
 Tensor layer(const Tensor& x, const Tensor& w, const std::optional<Tensor>& bias, const std::optional<Tensor>& residual, const std::optional<Tensor>& offsets,
              int64_t inner, int64_t act) {
-  std::vector<int64_t> shape = x.sizes().vec();
-  shape.back() = w.size(-2);
-  const int64_t K = w.size(-1), N = w.size(-2), rows = c10::multiply_integers(x.sizes().begin(), x.sizes().end() - 1);
-  const Tensor w3 = w.dim() == 2 ? w.unsqueeze(0) : w;
-  std::optional<Tensor> b2 = bias, r2 = residual;
-  if (b2 && b2->dim() == 1) b2 = b2->unsqueeze(0);
-  if (r2) r2 = r2->reshape({rows, N});
   auto grad = [](const std::optional<Tensor>& t) { return t && t->requires_grad(); };
-  const bool differentiated = at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || grad(bias));
-  const Tensor x2 = x.reshape({rows, K});
-  return Layer::apply(x2, w3, b2, r2, offsets, inner, act, differentiated).reshape(shape);
+  return Layer::apply(x, w, bias, residual, offsets, inner, act, at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || grad(bias)));
+}
+
+Tensor dense_act(const Tensor& x, const Tensor& w, const std::optional<Tensor>& bias, int64_t act, const std::optional<Tensor>& residual) {
+  const char* name = "dense_act";
+  check_operand(name, "x", x, x); check_operand(name, "weight", w, x); check_operand(name, "bias", bias, x); check_operand(name, "residual", residual, x);
+  TORCH_CHECK_VALUE(w.dim() == 2 && x.dim() >= 1 && x.size(-1) == w.size(1), name, ": x [..., K] and weight [N, K] expected, got ", x.sizes(), " and ", w.sizes());
+  TORCH_CHECK_VALUE(!bias || (bias->dim() == 1 && bias->size(0) == w.size(0)), name, ": bias must be [", w.size(0), "], got ", bias->sizes());
+  if (residual) {
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = w.size(0);
+    TORCH_CHECK_VALUE(residual->sizes() == shape, name, ": residual must have the result's shape ", shape, ", got ", residual->sizes());
+  }
+  return layer(x, w, bias, residual, std::nullopt, 1, act);
 }
 
 // ------------------------------------------------------------------------------------------------ experts' order
@@ -300,16 +326,61 @@ OrderPtr make_order(const Tensor& expert, int64_t experts) {
   return c10::make_intrusive<Order>(position, offsets);
 }
 
+// rows (or tokens) of a tensor that go with a plan
+void check_rows(const char* name, const char* what, const Tensor& t, int64_t rows, const Order& o) {
+  TORCH_CHECK_VALUE(t.dim() >= 1 && t.size(0) == rows, name, ": ", what, " must have ", rows, " rows, got ", t.sizes());
+  TORCH_CHECK_VALUE(t.device() == o.offsets.device(), name, ": ", what, " is on ", t.device(), ", the plan on ", o.offsets.device());
+}
+
+Tensor expert_gather(const Tensor& x, const OrderPtr& o) {
+  check_operand("expert_gather", "x", x, x);
+  check_rows("expert_gather", "x", x, o->position.size(0), *o);
+  return Gather::apply(x, o);
+}
+
+Tensor expert_combine(const Tensor& rows, const std::optional<Tensor>& weight, const OrderPtr& o) {
+  const char* name = "expert_combine";
+  check_operand(name, "rows", rows, rows); check_operand(name, "weight", weight, rows);
+  check_rows(name, "rows", rows, o->position.numel(), *o);
+  std::optional<Tensor> w = weight;
+  if (w && w->dim() == 1 && o->slots == 1) w = w->unsqueeze(1);
+  TORCH_CHECK_VALUE(!w || w->sizes() == o->position.sizes(), name, ": weight must be ", o->position.sizes(), ", got ", weight->sizes());
+  return combine(rows, w, o);
+}
+
+Tensor expert_dense(const Tensor& rows, const Tensor& w, const OrderPtr& o, const std::optional<Tensor>& bias, int64_t act) {
+  const char* name = "expert_dense";
+  check_operand(name, "rows", rows, rows); check_operand(name, "weight", w, rows); check_operand(name, "bias", bias, rows);
+  check_rows(name, "rows", rows, o->position.numel(), *o);
+  TORCH_CHECK_VALUE(rows.dim() >= 2 && w.dim() == 3 && w.size(0) == o->experts && w.size(2) == rows.size(-1), name, ": rows [rows, ..., K] and weight [", o->experts,
+                    ", N, K] expected, got ", rows.sizes(), " and ", w.sizes());
+  TORCH_CHECK_VALUE(!bias || (bias->dim() == 2 && bias->size(0) == w.size(0) && bias->size(1) == w.size(1)), name, ": bias must be [", w.size(0), ", ", w.size(1), "], got ",
+                    bias->sizes());
+  const int64_t inner = c10::multiply_integers(rows.sizes().begin() + 1, rows.sizes().end() - 1);
+  return layer(rows, w, bias, std::nullopt, o->offsets, std::max<int64_t>(inner, 1), act);
+}
+
+OrderPtr expert_plan(const Tensor& expert, int64_t experts) {
+  const char* name = "expert_plan";
+  if (!expert.is_cuda()) TORCH_CHECK(false, name, ": expert must be a CUDA tensor: fasteq_b200 has no CPU path");
+  TORCH_CHECK_VALUE(expert.scalar_type() == at::kInt || expert.scalar_type() == at::kLong, name, ": expert must be int32 or int64, got ", expert.scalar_type());
+  TORCH_CHECK_VALUE(expert.dim() == 1 || (expert.dim() == 2 && expert.size(1) >= 1), name, ": expert must be [tokens] or [tokens, slots] with a slot at least, got ",
+                    expert.sizes());
+  TORCH_CHECK_VALUE(experts >= 1 && experts <= FASTEQ_MAX_EXPERTS, name, ": 1 to ", FASTEQ_MAX_EXPERTS, " experts are supported, got ", experts);
+  return make_order((expert.dim() == 1 ? expert.unsqueeze(1) : expert).contiguous(), experts);
+}
+
 }  // namespace
 
 void bind_experts(py::module_& m) {
   py::class_<Order, OrderPtr>(m, "ExpertOrder")
       .def_readonly("position", &Order::position)
       .def_readonly("offsets", &Order::offsets);
-  m.def("product_layer", &layer, py::arg("x"), py::arg("w"), py::arg("bias"), py::arg("residual"), py::arg("offsets"), py::arg("inner"), py::arg("act"));
-  m.def("expert_order", &make_order);
-  m.def("expert_gather", [](const Tensor& x, const OrderPtr& o) -> Tensor { return Gather::apply(x, o); });
-  m.def("expert_combine", [](const Tensor& rows, const std::optional<Tensor>& weight, const OrderPtr& o) -> Tensor { return combine(rows, weight, o); });
+  m.def("dense_act", &dense_act);
+  m.def("expert_plan", &expert_plan);
+  m.def("expert_gather", &expert_gather);
+  m.def("expert_combine", &expert_combine);
+  m.def("expert_dense", &expert_dense);
 }
 
 }  // namespace front

@@ -25,33 +25,8 @@ def act_code(name: str, activation) -> int:
     return ACT_CODES[activation]
 
 
-def check_operands(name: str, **operands) -> None:
-    """CUDA tensors of one device and one type, float32 or float64 (``None``: left out)."""
-    first = None
-    for what, t in operands.items():
-        if t is None:
-            continue
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name}: {what} must be a tensor, got {type(t).__name__}")
-        if not t.is_cuda:
-            raise RuntimeError(f"{name}: {what} must be a CUDA tensor: fasteq_b200 has no CPU path")
-        if t.dtype not in (torch.float32, torch.float64):
-            raise ValueError(f"{name}: only float32 and float64 are supported; {what} is {t.dtype}")
-        first = first if first is not None else t
-        if t.dtype != first.dtype or t.device != first.device:
-            raise ValueError(f"{name}: all operands must have one dtype and one device; {what} is {t.dtype} on {t.device}, not {first.dtype} on {first.device}")
-
-
 def dense_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
               residual: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``act(x @ weight.T + bias) + residual``: ``x [..., K]``, ``weight [N, K]`` (a ``torch.nn.Linear`` weight), ``bias [N]``,
     ``residual [..., N]`` like the result."""
-    code = act_code("dense_act", activation)
-    check_operands("dense_act", x=x, weight=weight, bias=bias, residual=residual)
-    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
-        raise ValueError(f"dense_act: x [..., K] and weight [N, K] expected, got {tuple(x.shape)} and {tuple(weight.shape)}")
-    if bias is not None and bias.shape != weight.shape[:1]:
-        raise ValueError(f"dense_act: bias must be [{weight.shape[0]}], got {tuple(bias.shape)}")
-    if residual is not None and residual.shape != (*x.shape[:-1], weight.shape[0]):
-        raise ValueError(f"dense_act: residual must have the result's shape {(*x.shape[:-1], weight.shape[0])}, got {tuple(residual.shape)}")
-    return _front.lib().product_layer(x, weight, bias, residual, None, 1, code)
+    return _front.lib().dense_act(x, weight, bias, act_code("dense_act", activation), residual)

@@ -20,11 +20,9 @@ from typing import Optional
 import torch
 
 from .. import _cabi, _front
-from .dense_act import act_code, check_operands
+from .dense_act import act_code
 
 __all__ = ["ExpertPlan", "expert_plan", "expert_gather", "expert_dense", "expert_combine", "expert_device_status"]
-
-MAX_EXPERTS = 1024
 
 
 class ExpertPlan:
@@ -48,59 +46,28 @@ def expert_device_status() -> int:
 def expert_plan(expert: torch.Tensor, num_experts: int) -> ExpertPlan:
     """``expert [tokens, slots]`` (or ``[tokens]``: one slot), int32 or int64.  Negative numbers mean no expert; numbers from ``num_experts``
     on are treated like them and reported by ``fasteq_b200.status.device_status``."""
-    if not expert.is_cuda:
-        raise RuntimeError("expert_plan: expert must be a CUDA tensor: fasteq_b200 has no CPU path")
-    if expert.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"expert_plan: expert must be int32 or int64, got {expert.dtype}")
-    if expert.dim() not in (1, 2) or (expert.dim() == 2 and expert.shape[1] < 1):
-        raise ValueError(f"expert_plan: expert must be [tokens] or [tokens, slots] with a slot at least, got {tuple(expert.shape)}")
-    if not 1 <= num_experts <= MAX_EXPERTS:
-        raise ValueError(f"expert_plan: 1 to {MAX_EXPERTS} experts are supported, got {num_experts}")
-    e = expert.unsqueeze(1) if expert.dim() == 1 else expert
-    return ExpertPlan(_front.lib().expert_order(e.contiguous(), int(num_experts)))
+    return ExpertPlan(_front.lib().expert_plan(expert, num_experts))
 
 
-def _check_rows(name: str, what: str, t: torch.Tensor, rows: int, plan: ExpertPlan) -> None:
+def _order(name: str, plan: ExpertPlan):
     if not isinstance(plan, ExpertPlan):
         raise TypeError(f"{name}: plan must be an ExpertPlan, got {type(plan).__name__}")
-    if t.dim() < 1 or t.shape[0] != rows:
-        raise ValueError(f"{name}: {what} must have {rows} rows, got {tuple(t.shape)}")
-    if t.device != plan.offsets.device:
-        raise ValueError(f"{name}: {what} is on {t.device}, the plan on {plan.offsets.device}")
+    return plan._native
 
 
 def expert_gather(x: torch.Tensor, plan: ExpertPlan) -> torch.Tensor:
     """``x [tokens, ...]`` to ``[tokens * slots, ...]`` in the experts' order (zeros for entries of no expert)."""
-    check_operands("expert_gather", x=x)
-    _check_rows("expert_gather", "x", x, plan.tokens if isinstance(plan, ExpertPlan) else -1, plan)
-    return _front.lib().expert_gather(x, plan._native)
+    return _front.lib().expert_gather(x, _order("expert_gather", plan))
 
 
 def expert_combine(rows: torch.Tensor, plan: ExpertPlan, weight: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``y[t] = sum_s weight[t, s] * rows[position[t, s]]``: ``rows [tokens * slots, ...]`` in the experts' order, ``weight [tokens, slots]``
     (``[tokens]`` with one slot; ``None``: ones)."""
-    check_operands("expert_combine", rows=rows, weight=weight)
-    _check_rows("expert_combine", "rows", rows, plan.rows if isinstance(plan, ExpertPlan) else -1, plan)
-    if weight is not None:
-        if weight.dim() == 1 and plan.slots == 1:
-            weight = weight.unsqueeze(1)
-        if weight.shape != plan.position.shape:
-            raise ValueError(f"expert_combine: weight must be {tuple(plan.position.shape)}, got {tuple(weight.shape)}")
-    return _front.lib().expert_combine(rows, weight, plan._native)
+    return _front.lib().expert_combine(rows, weight, _order("expert_combine", plan))
 
 
 def expert_dense(rows: torch.Tensor, weight: torch.Tensor, plan: ExpertPlan, bias: Optional[torch.Tensor] = None,
                  activation: Optional[str] = None) -> torch.Tensor:
     """``act(rows[r] @ weight[e(r)].T + bias[e(r)])`` for rows in the experts' order, ``[tokens * slots, ..., K]``; ``weight [num_experts, N, K]``,
     ``bias [num_experts, N]``, activations as in ``dense_act``.  Rows of no expert come out as zeros."""
-    code = act_code("expert_dense", activation)
-    check_operands("expert_dense", rows=rows, weight=weight, bias=bias)
-    _check_rows("expert_dense", "rows", rows, plan.rows if isinstance(plan, ExpertPlan) else -1, plan)
-    if rows.dim() < 2 or weight.dim() != 3 or weight.shape[0] != plan.num_experts or weight.shape[2] != rows.shape[-1]:
-        raise ValueError(f"expert_dense: rows [rows, ..., K] and weight [{plan.num_experts}, N, K] expected, got {tuple(rows.shape)} and {tuple(weight.shape)}")
-    if bias is not None and bias.shape != weight.shape[:2]:
-        raise ValueError(f"expert_dense: bias must be {tuple(weight.shape[:2])}, got {tuple(bias.shape)}")
-    inner = 1
-    for n in rows.shape[1:-1]:
-        inner *= n
-    return _front.lib().product_layer(rows, weight, bias, None, plan.offsets, max(inner, 1), code)
+    return _front.lib().expert_dense(rows, weight, _order("expert_dense", plan), bias, act_code("expert_dense", activation))

@@ -13,9 +13,10 @@ def test_cpu_tensors_and_unknown_activations_are_refused():
         dense_act(x, w)
     with pytest.raises(ValueError, match="activation"):
         dense_act(x, w, activation="swish")
-    for call in (lambda: expert_plan(torch.zeros(4, dtype=torch.int64), 2), lambda: expert_gather(x, None), lambda: expert_combine(x, None),
-                 lambda: expert_dense(x, w.unsqueeze(0), None)):
-        with pytest.raises(RuntimeError, match="no CPU path"):
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        expert_plan(torch.zeros(4, dtype=torch.int64), 2)
+    for call in (lambda: expert_gather(x, None), lambda: expert_combine(x, None), lambda: expert_dense(x, w.unsqueeze(0), None)):
+        with pytest.raises(TypeError, match="ExpertPlan"):
             call()
 
 
