@@ -7,7 +7,9 @@
 //   combine  y[t] = sum_s w[t, s] rows[position[t, s]]                        gradients: grad_rows[position] = w grad_y[t],
 //                                                                             grad_w[t, s] = <rows[position], grad_y[t]>
 // The permutation is known from both sides, so every sum is a walk over a token's slots in their order: no atomics, the same bits every time.
-// Bound: memory, each row tensor once; a token's row is read once for all its slots.
+// Bound: memory, each row tensor once; a token's row is read once for all its slots.  Rows are loaded and stored past the caches' order of use
+// (__ldcs, __stcs): 301,746 rows of 512 FP32 values take 142 us to gather (927 MB, 6.5 TB/s, the rate of a copy), 151 us to combine, 243 us for the
+// gradients of the combination; with ordinary accesses the gather's own gradient took 177 us instead of 151 us, behind a kernel that left the L2 full.
 #include <cstdint>
 #include <cuda_runtime.h>
 #include "fasteq_b200.h"
@@ -22,7 +24,11 @@ namespace {
 __device__ int g_expert_status;
 
 constexpr int PLAN_THREADS = 1024, PLAN_WARPS = PLAN_THREADS / 32;
-constexpr int CHUNK = 4096;                  // entries of a CTA where there are several
+// Entries of a CTA: GROUPS of 32 a warp, held in registers.  One group keeps the chain of a CTA short, but each of the then many CTAs adds up all CTAs'
+// counts.  24,576 entries of 8 experts: 3.8 us to count and 5.6 us to place with one group, 6 us and 9 us with four; 301,746 entries of 32 experts
+// (four groups): 8 us and 12 us.
+constexpr int MOST_GROUPS = 4, FEW = 64 * 1024;
+int groups_for(long long n) { return n > PLAN_THREADS && n <= FEW ? 1 : MOST_GROUPS; }
 
 // 64-bit expert numbers as torch's top-k gives them, or 32-bit ones; experts that are not there count as none and are reported
 template <typename I> __device__ __forceinline__ int key_of(const I* expert, long long i, int X) {
@@ -32,35 +38,34 @@ template <typename I> __device__ __forceinline__ int key_of(const I* expert, lon
   return (int)e;
 }
 
-// Entries of equal key in a warp find each other; the first of them counts for all.  counts: this warp's [X + 1].
-template <typename I> __device__ __forceinline__ void count_entries(const I* expert, long long first, long long end, int X, int* counts) {
+// This warp's entries (first + 32 g + lane), their keys in registers, -1 beyond the end.
+template <typename I, int GROUPS> __device__ __forceinline__ void load_keys(const I* expert, long long first, long long n, int X, int (&keys)[GROUPS]) {
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) {
+    const long long i = first + g * 32 + (threadIdx.x & 31);
+    keys[g] = i < n ? key_of(expert, i, X) : -1;
+  }
+}
+// Entries of equal key in a group find each other; the first of them counts for all.  counts: this warp's [X + 1].
+template <int GROUPS> __device__ __forceinline__ void count_entries(const int (&keys)[GROUPS], int* counts) {
   const int lane = threadIdx.x & 31;
-  for (long long i = first + lane; i - lane < end; i += 32) {
-    const int k = i < end ? key_of(expert, i, X) : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, k);
-    if (k >= 0 && lane == __ffs(same) - 1) counts[k] += __popc(same);
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) {
+    const unsigned same = __match_any_sync(0xffffffffu, keys[g]);
+    if (keys[g] >= 0 && lane == __ffs(same) - 1) counts[keys[g]] += __popc(same);
     __syncwarp();
   }
 }
-
-template <typename I>
-__device__ __forceinline__ void place_entries(const I* expert, long long first, long long end, int X, int* next, int* position) {
+template <int GROUPS> __device__ __forceinline__ void place_entries(const int (&keys)[GROUPS], long long first, int* next, int* position) {
   const int lane = threadIdx.x & 31;
-  for (long long i = first + lane; i - lane < end; i += 32) {
-    const int k = i < end ? key_of(expert, i, X) : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, k);
-    if (k >= 0) position[i] = next[k] + __popc(same & ((1u << lane) - 1u));
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) {
+    const unsigned same = __match_any_sync(0xffffffffu, keys[g]);
+    if (keys[g] >= 0) position[first + g * 32 + lane] = next[keys[g]] + __popc(same & ((1u << lane) - 1u));
     __syncwarp();
-    if (k >= 0 && lane == __ffs(same) - 1) next[k] += __popc(same);
+    if (keys[g] >= 0 && lane == __ffs(same) - 1) next[keys[g]] += __popc(same);
     __syncwarp();
   }
-}
-
-// the share of the CTA's entries [c0, c1) that a warp takes, whole groups of 32
-__device__ __forceinline__ void warp_share(long long c0, long long c1, long long* first, long long* end) {
-  const long long per = ((c1 - c0 + PLAN_THREADS - 1) / PLAN_THREADS) * 32;
-  *first = min(c1, c0 + (threadIdx.x >> 5) * per);
-  *end = min(c1, *first + per);
 }
 
 // exclusive prefix sums of v[0 .. n) in shared memory (all threads); n <= PLAN_THREADS + 1
@@ -91,46 +96,57 @@ __device__ __forceinline__ void scan_keys(int* v, int n, int* warp_sums) {
   __syncthreads();
 }
 
-template <typename I> __global__ void __launch_bounds__(PLAN_THREADS) expert_count_kernel(const I* expert, long long n, int X, int* counts) {
-  extern __shared__ int sm[];                       // [PLAN_WARPS][X + 1]
-  const int K = X + 1;
-  wait_for_previous_kernel();
-  for (int j = threadIdx.x; j < PLAN_WARPS * K; j += PLAN_THREADS) sm[j] = 0;
-  __syncthreads();
-  const long long c0 = (long long)blockIdx.x * CHUNK, c1 = min(n, c0 + CHUNK);
-  long long first, end;
-  warp_share(c0, c1, &first, &end);
-  count_entries(expert, first, end, X, sm + (threadIdx.x >> 5) * K);
-  __syncthreads();
-  for (int k = threadIdx.x; k < K; k += PLAN_THREADS) {
-    int s = 0;
-    for (int w = 0; w < PLAN_WARPS; ++w) s += sm[w * K + k];
-    counts[(long long)blockIdx.x * K + k] = s;
+// counts of the warps [warp][K] -> counts of the warps before; their sums to total (may be null).  A warp to a key.
+__device__ __forceinline__ void scan_warps(int* counts, int K, int* total) {
+  const int lane = threadIdx.x & 31;
+  for (int k = threadIdx.x >> 5; k < K; k += PLAN_WARPS) {
+    const int mine = counts[lane * K + k];
+    int sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += u;
+    }
+    counts[lane * K + k] = sum - mine;
+    if (total && lane == 31) total[k] = sum;
   }
 }
 
-// One CTA (`counts` null) or CHUNK entries to each, their counts known.
-template <typename I>
-__global__ void __launch_bounds__(PLAN_THREADS) expert_place_kernel(const I* expert, long long n, int X, const int* counts, int* position,
-                                                                    int* offsets) {
+template <typename I, int GROUPS> __global__ void __launch_bounds__(PLAN_THREADS) expert_count_kernel(const I* expert, long long n, int X, int* counts) {
+  extern __shared__ int sm[];                       // [PLAN_WARPS][X + 1] | [X + 1]
+  const int K = X + 1;
+  for (int j = threadIdx.x; j < PLAN_WARPS * K; j += PLAN_THREADS) sm[j] = 0;
+  wait_for_previous_kernel();
+  int keys[GROUPS];
+  load_keys<I, GROUPS>(expert, ((long long)blockIdx.x * PLAN_WARPS + (threadIdx.x >> 5)) * 32 * GROUPS, n, X, keys);
+  __syncthreads();
+  count_entries<GROUPS>(keys, sm + (threadIdx.x >> 5) * K);
+  __syncthreads();
+  scan_warps(sm, K, sm + PLAN_WARPS * K);
+  __syncthreads();
+  for (int k = threadIdx.x; k < K; k += PLAN_THREADS) counts[(long long)blockIdx.x * K + k] = sm[PLAN_WARPS * K + k];
+}
+
+// One CTA (`counts` null), or several, their counts known.
+template <typename I, int GROUPS>
+__global__ void __launch_bounds__(PLAN_THREADS) expert_place_kernel(const I* expert, long long n, int X, const int* counts, int* position, int* offsets) {
   extern __shared__ int sm[];                       // [PLAN_WARPS][X + 1] | [X + 1] totals | [X + 1] of earlier CTAs | [32]
   const int K = X + 1;
   int *total = sm + PLAN_WARPS * K, *earlier = total + K, *warp_sums = earlier + K;
-  wait_for_previous_kernel();
   for (int j = threadIdx.x; j < PLAN_WARPS * K; j += PLAN_THREADS) sm[j] = 0;
   for (int k = threadIdx.x; k < K; k += PLAN_THREADS) total[k] = earlier[k] = 0;
+  wait_for_previous_kernel();
+  const long long first = ((long long)blockIdx.x * PLAN_WARPS + (threadIdx.x >> 5)) * 32 * GROUPS;
+  int keys[GROUPS];
+  load_keys<I, GROUPS>(expert, first, n, X, keys);
   __syncthreads();
-  const long long c0 = counts ? (long long)blockIdx.x * CHUNK : 0, c1 = counts ? min(n, c0 + CHUNK) : n;
-  long long first, end;
-  warp_share(c0, c1, &first, &end);
-  count_entries(expert, first, end, X, sm + (threadIdx.x >> 5) * K);
   if (counts) {
     // all CTAs' counts, a key and a share of the CTAs to each thread; whole numbers, so that the order of the additions does not matter
     const int parts = max(1, PLAN_THREADS / K), n_ctas = (int)gridDim.x;
     for (int j = threadIdx.x; j < parts * K; j += PLAN_THREADS) {
       const int k = j % K, p = j / K;
       int s = 0, b = 0;
-#pragma unroll 4
+#pragma unroll 8
       for (int c = p; c < n_ctas; c += parts) {
         const int v = counts[(long long)c * K + k];
         s += v;
@@ -140,17 +156,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) expert_place_kernel(const I* exp
       atomicAdd(&earlier[k], b);
     }
   }
+  count_entries<GROUPS>(keys, sm + (threadIdx.x >> 5) * K);
   __syncthreads();
-  // counts of the warps -> counts of the warps before; without `counts` their sum is the total
-  for (int k = threadIdx.x; k < K; k += PLAN_THREADS) {
-    int s = 0;
-    for (int w = 0; w < PLAN_WARPS; ++w) {
-      const int v = sm[w * K + k];
-      sm[w * K + k] = s;
-      s += v;
-    }
-    if (!counts) total[k] = s;
-  }
+  scan_warps(sm, K, counts ? nullptr : total);
   __syncthreads();
   scan_keys(total, K, warp_sums);
   if (blockIdx.x == 0)
@@ -160,32 +168,55 @@ __global__ void __launch_bounds__(PLAN_THREADS) expert_place_kernel(const I* exp
     sm[j] += total[k] + earlier[k];
   }
   __syncthreads();
-  place_entries(expert, first, end, X, sm + (threadIdx.x >> 5) * K, position);
+  place_entries<GROUPS>(keys, first, sm + (threadIdx.x >> 5) * K, position);
 }
 
-template <typename I>
+int plan_ctas(long long n) { return (int)((n + groups_for(n) * PLAN_THREADS - 1) / (groups_for(n) * PLAN_THREADS)); }
+
+template <typename I, int GROUPS>
 int launch_plan(const void* expert, long long n, int X, int* position, int* offsets, void* scratch, cudaStream_t s) {
-  const int K = X + 1, ctas = (int)((n + CHUNK - 1) / CHUNK);
-  const size_t count_smem = (size_t)PLAN_WARPS * K * 4, place_smem = count_smem + (2 * (size_t)K + 32) * 4;
+  const int K = X + 1, ctas = plan_ctas(n);
+  const size_t count_smem = (size_t)(PLAN_WARPS + 1) * K * 4, place_smem = ((size_t)(PLAN_WARPS + 2) * K + 32) * 4;
   cudaError_t e = cudaSuccess;
   if (place_smem > 48 * 1024) {
-    e = cudaFuncSetAttribute(expert_count_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)count_smem);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(expert_place_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)place_smem);
+    e = cudaFuncSetAttribute(expert_count_kernel<I, GROUPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)count_smem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(expert_place_kernel<I, GROUPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)place_smem);
     if (e != cudaSuccess) return cuda_fail(e);
   }
   const int* counts = nullptr;
   if (ctas > 1) {
-    e = launch_dependent(expert_count_kernel<I>, (unsigned)ctas, PLAN_THREADS, count_smem, s, (const I*)expert, n, X, (int*)scratch);
+    e = launch_dependent(expert_count_kernel<I, GROUPS>, (unsigned)ctas, PLAN_THREADS, count_smem, s, (const I*)expert, n, X, (int*)scratch);
     if (e != cudaSuccess) return cuda_fail(e);
     counts = (const int*)scratch;
   }
-  e = launch_dependent(expert_place_kernel<I>, (unsigned)(ctas > 1 ? ctas : 1), PLAN_THREADS, place_smem, s, (const I*)expert, n, X, counts, position, offsets);
+  e = launch_dependent(expert_place_kernel<I, GROUPS>, (unsigned)(ctas > 1 ? ctas : 1), PLAN_THREADS, place_smem, s, (const I*)expert, n, X, counts, position, offsets);
   return e == cudaSuccess ? FASTEQ_OK : cuda_fail(e);
+}
+template <typename I> int launch_plan(const void* expert, long long n, int X, int* position, int* offsets, void* scratch, cudaStream_t s) {
+  return groups_for(n) == 1 ? launch_plan<I, 1>(expert, n, X, position, offsets, scratch, s) : launch_plan<I, MOST_GROUPS>(expert, n, X, position, offsets, scratch, s);
 }
 
 // ------------------------------------------------------------------------------------------------ rows
 // blockDim = (tx, ty): tx threads (a power of two) walk a row's packs of V values, ty tokens to a CTA
 template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
+template <typename T, int V> __device__ __forceinline__ Pack<T, V> read_once(const T* p, long long i) {
+  Pack<T, V> r;
+  if constexpr (sizeof(r) == 16) {
+    *reinterpret_cast<float4*>(&r) = __ldcs(reinterpret_cast<const float4*>(p) + i);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) r.v[k] = __ldcs(p + i * V + k);
+  }
+  return r;
+}
+template <typename T, int V> __device__ __forceinline__ void write_once(T* p, long long i, const Pack<T, V>& r) {
+  if constexpr (sizeof(r) == 16) {
+    __stcs(reinterpret_cast<float4*>(p) + i, *reinterpret_cast<const float4*>(&r));
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) __stcs(p + i * V + k, r.v[k]);
+  }
+}
 
 template <typename T, int V>
 __global__ void __launch_bounds__(256) expert_gather_kernel(const T* x, const int* position, const int* offsets, int X, long long tokens, int slots,
@@ -195,10 +226,10 @@ __global__ void __launch_bounds__(256) expert_gather_kernel(const T* x, const in
   const int routed = offsets[X];
   for (long long t = (long long)blockIdx.x * blockDim.y + threadIdx.y; t < tokens; t += (long long)gridDim.x * blockDim.y) {
     for (int c = threadIdx.x; c < packs; c += blockDim.x) {
-      const P v = reinterpret_cast<const P*>(x)[t * packs + c];
+      const P v = read_once<T, V>(x, t * packs + c);
       for (int s = 0; s < slots; ++s) {
         const int p = position[t * slots + s];
-        reinterpret_cast<P*>(rows)[(long long)p * packs + c] = p < routed ? v : P{};
+        write_once<T, V>(rows, (long long)p * packs + c, p < routed ? v : P{});
       }
     }
   }
@@ -216,12 +247,12 @@ __global__ void __launch_bounds__(256) expert_combine_kernel(const T* rows, cons
       for (int s = 0; s < slots; ++s) {
         const int p = position[t * slots + s];
         if (p >= routed) continue;
-        const P v = reinterpret_cast<const P*>(rows)[(long long)p * packs + c];
+        const P v = read_once<T, V>(rows, (long long)p * packs + c);
         const T w = WEIGHTED ? weight[t * slots + s] : T(1);
 #pragma unroll
         for (int k = 0; k < V; ++k) sum.v[k] = WEIGHTED ? vfma(w, v.v[k], sum.v[k]) : sum.v[k] + v.v[k];
       }
-      reinterpret_cast<P*>(y)[t * packs + c] = sum;
+      write_once<T, V>(y, t * packs + c, sum);
     }
   }
 }
@@ -252,14 +283,14 @@ __global__ void __launch_bounds__(256) expert_combine_backward_kernel(const T* r
           if (live) {
             const P gv = reinterpret_cast<const P*>(g)[t * packs + c];
             if (gweight) {
-              const P v = reinterpret_cast<const P*>(rows)[(long long)p * packs + c];
+              const P v = read_once<T, V>(rows, (long long)p * packs + c);
 #pragma unroll
               for (int k = 0; k < V; ++k) dot = vfma(v.v[k], gv.v[k], dot);
             }
 #pragma unroll
             for (int k = 0; k < V; ++k) o.v[k] = w * gv.v[k];
           }
-          if (grows) reinterpret_cast<P*>(grows)[(long long)p * packs + c] = o;
+          if (grows) write_once<T, V>(grows, (long long)p * packs + c, o);
         }
       }
       if (gweight) {
@@ -320,7 +351,7 @@ bool sizes_ok(int32_t dtype, int64_t tokens, int32_t slots, int32_t experts, int
 extern "C" int fasteq_expert_plan_scratch(int64_t entries, int32_t experts, int64_t* bytes) {
   if (!bytes || entries < 0 || experts < 1) return FASTEQ_INVALID;
   if (experts > FASTEQ_MAX_EXPERTS || entries > 0x7fff0000LL) return FASTEQ_UNSUPPORTED;
-  const int64_t ctas = (entries + CHUNK - 1) / CHUNK;
+  const int64_t ctas = plan_ctas(entries);
   *bytes = ctas > 1 ? ctas * (experts + 1) * 4 : 0;
   return FASTEQ_OK;
 }
