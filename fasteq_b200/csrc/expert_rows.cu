@@ -24,11 +24,12 @@ namespace {
 __device__ int g_expert_status;
 
 constexpr int PLAN_THREADS = 1024, PLAN_WARPS = PLAN_THREADS / 32;
-// Entries of a CTA: GROUPS of 32 a warp, held in registers.  One group keeps the chain of a CTA short, but each of the then many CTAs adds up all CTAs'
-// counts.  24,576 entries of 8 experts: 3.8 us to count and 5.6 us to place with one group, 6 us and 9 us with four; 301,746 entries of 32 experts
-// (four groups): 8 us and 12 us.
-constexpr int MOST_GROUPS = 4, FEW = 64 * 1024;
-int groups_for(long long n) { return n > PLAN_THREADS && n <= FEW ? 1 : MOST_GROUPS; }
+// Entries of a CTA: GROUPS of 32 a warp, held in registers.  One group keeps a CTA's chain short (1,000 entries of 8 experts 3.9 us, with four groups 5.0 us;
+// 20,000 in 3.1 + 4.8 us to count and to place, 4.6 + 6.9 us; 300,000 of 89 experts 5.9 + 14.4 us, 7.9 + 14.5 us).  Four where they leave one CTA, which
+// needs no counts before it (4,000 entries of 8 experts 6.2 us, with one group 3.1 + 4.8 us), and where there would be so many CTAs that
+// adding up all their counts in each takes over.
+constexpr int MOST_GROUPS = 4, MANY = 512 * 1024;
+int groups_for(long long n) { return n <= PLAN_THREADS || (n > MOST_GROUPS * PLAN_THREADS && n <= MANY) ? 1 : MOST_GROUPS; }
 
 // 64-bit expert numbers as torch's top-k gives them, or 32-bit ones; experts that are not there count as none and are reported
 template <typename I> __device__ __forceinline__ int key_of(const I* expert, long long i, int X) {

@@ -176,8 +176,14 @@ void check_operand(const char* name, const char* what, const std::optional<Tenso
   if (t) check_operand(name, what, *t, first);
 }
 
-Tensor layer(const Tensor& x, const Tensor& w, const std::optional<Tensor>& bias, const std::optional<Tensor>& residual, const std::optional<Tensor>& offsets,
+// extents that the C interface takes as 32-bit numbers
+void check_extent(const char* name, const char* what, int64_t v) {
+  TORCH_CHECK_VALUE(v <= INT32_MAX, name, ": ", what, " must be below 2^31, got ", v);
+}
+
+Tensor layer(const char* name, const Tensor& x, const Tensor& w, const std::optional<Tensor>& bias, const std::optional<Tensor>& residual, const std::optional<Tensor>& offsets,
              int64_t inner, int64_t act) {
+  check_extent(name, "channels", std::max(w.size(-1), w.size(-2))); check_extent(name, "rows of an entry", inner);
   auto grad = [](const std::optional<Tensor>& t) { return t && t->requires_grad(); };
   return Layer::apply(x, w, bias, residual, offsets, inner, act, at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || grad(bias)));
 }
@@ -192,7 +198,7 @@ Tensor dense_act(const Tensor& x, const Tensor& w, const std::optional<Tensor>& 
     shape.back() = w.size(0);
     TORCH_CHECK_VALUE(residual->sizes() == shape, name, ": residual must have the result's shape ", shape, ", got ", residual->sizes());
   }
-  return layer(x, w, bias, residual, std::nullopt, 1, act);
+  return layer(name, x, w, bias, residual, std::nullopt, 1, act);
 }
 
 // ------------------------------------------------------------------------------------------------ experts' order
@@ -329,6 +335,7 @@ OrderPtr make_order(const Tensor& expert, int64_t experts) {
 // rows (or tokens) of a tensor that go with a plan
 void check_rows(const char* name, const char* what, const Tensor& t, int64_t rows, const Order& o) {
   TORCH_CHECK_VALUE(t.dim() >= 1 && t.size(0) == rows, name, ": ", what, " must have ", rows, " rows, got ", t.sizes());
+  check_extent(name, "a row's values", width_of(t));
   TORCH_CHECK_VALUE(t.device() == o.offsets.device(), name, ": ", what, " is on ", t.device(), ", the plan on ", o.offsets.device());
 }
 
@@ -357,7 +364,7 @@ Tensor expert_dense(const Tensor& rows, const Tensor& w, const OrderPtr& o, cons
   TORCH_CHECK_VALUE(!bias || (bias->dim() == 2 && bias->size(0) == w.size(0) && bias->size(1) == w.size(1)), name, ": bias must be [", w.size(0), ", ", w.size(1), "], got ",
                     bias->sizes());
   const int64_t inner = c10::multiply_integers(rows.sizes().begin() + 1, rows.sizes().end() - 1);
-  return layer(rows, w, bias, std::nullopt, o->offsets, std::max<int64_t>(inner, 1), act);
+  return layer(name, rows, w, bias, std::nullopt, o->offsets, std::max<int64_t>(inner, 1), act);
 }
 
 OrderPtr expert_plan(const Tensor& expert, int64_t experts) {

@@ -301,7 +301,8 @@ template <typename T>
 int wgrad(const fasteq_product_problem* p, int size, const void* x, const void* g, const void* slope, const int32_t* offsets, void* gw, void* gb, void* scratch,
           cudaStream_t s) {
   const Groups groups = groups_of(p, offsets);
-  const int tiles = ((p->n + TILE - 1) / TILE) * std::max(1, (p->k + TILE - 1) / TILE);
+  const long long tiles = (long long)((p->n + TILE - 1) / TILE) * std::max(1, (p->k + TILE - 1) / TILE);
+  if (tiles > 65535) return FASTEQ_UNSUPPORTED;
   const cudaError_t e = launch_dependent(product_wgrad_kernel<T>, dim3((unsigned)(p->rows / size + p->experts), (unsigned)tiles), THREADS, 0, s, groups, (const T*)x,
                                          (const T*)g, (const T*)slope, p->k, p->n, slope_pitch(p), size, (T*)gw, (T*)gb, (T*)scratch);
   return e == cudaSuccess ? reduce<T>(p, groups, size, gw, gb, scratch, s) : cuda_fail(e);
@@ -471,9 +472,10 @@ extern "C" int fasteq_product_forward(const fasteq_product_problem* p, const voi
   if (const int rc = check(p, offsets)) return rc;
   if (p->rows == 0 || p->n == 0) return FASTEQ_OK;
   const Scratch need = scratch_of(p, false);
+  if (need.total() > 0 && !wide(0, {scratch})) return FASTEQ_INVALID;
   if (!y || (p->k > 0 && (!x || !w)) || (need.total() > 0 && (!scratch || scratch_bytes < need.total()))) return FASTEQ_INVALID;
   cudaStream_t s = (cudaStream_t)stream;
-  if (on_tensor_cores(p) && (need.x || wide(0, {x})) && wide(0, {slope, scratch})) {
+  if (on_tensor_cores(p) && (need.x || wide(0, {x})) && wide(0, {slope})) {
     char* at = (char*)scratch;
     if (need.x) {
       const cudaError_t e = align_rows<float>(x, nullptr, p->k, 0, (p->k + 3) & ~3, p->rows, at, s);
@@ -497,7 +499,7 @@ extern "C" int fasteq_product_backward(const fasteq_product_problem* p, const vo
   if (grad_bias && !grad_w && p->k > 0) return FASTEQ_INVALID;
   const bool sums = grad_w || grad_bias, there = p->rows > 0 && p->n > 0;
   const Scratch need = scratch_of(p, true);
-  if (need.total() > 0 && (!scratch || scratch_bytes < need.total())) return FASTEQ_INVALID;
+  if (need.total() > 0 && (!scratch || !wide(0, {scratch}) || scratch_bytes < need.total())) return FASTEQ_INVALID;
   if (there && (!grad_y || (p->act != kIdentity && !slope) || (grad_x && p->k > 0 && !w) || (sums && p->k > 0 && !x))) return FASTEQ_INVALID;
   cudaStream_t s = (cudaStream_t)stream;
   const size_t size = p->dtype == FASTEQ_F32 ? 4 : 8;
@@ -510,7 +512,7 @@ extern "C" int fasteq_product_backward(const fasteq_product_problem* p, const vo
   }
   char *x_at = (char*)scratch, *g_at = x_at + need.x, *split_at = g_at + need.g, *partial_at = split_at + need.split;
   int rc = FASTEQ_OK;
-  if (on_tensor_cores(p) && (need.g || wide(0, {grad_y})) && (need.x || !sums || wide(0, {x})) && wide(0, {slope, scratch})) {
+  if (on_tensor_cores(p) && (need.g || wide(0, {grad_y})) && (need.x || !sums || wide(0, {x})) && wide(0, {slope})) {
     const int ldg = (p->n + 3) & ~3, ldx = (p->k + 3) & ~3;
     if (need.g) {                         // with the slope multiplied in, then
       e = align_rows<float>(grad_y, slope, p->n, ldg, ldg, p->rows, g_at, s);

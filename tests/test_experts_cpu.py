@@ -60,6 +60,11 @@ def test_other_entries_refuse_null_pointers_and_sizes():
         assert lib.fasteq_product_scratch(C.byref(q), I32(backward), C.byref(one)) == OK and (one.value > 0) == there, change
     long = Problem(**{**GOOD, "k": 2048})
     assert lib.fasteq_product_forward(C.byref(long), some, some, None, None, None, some, None, some, I64(16), None) == INVALID
+    buffer = C.create_string_buffer(1 << 20)
+    need = C.c_int64(0)
+    assert lib.fasteq_product_scratch(C.byref(long), I32(0), C.byref(need)) == OK and need.value + 16 <= len(buffer)
+    odd = C.c_void_p(C.addressof(buffer) // 16 * 16 + 20)                                       # scratch that is not 16-byte aligned
+    assert lib.fasteq_product_forward(C.byref(long), some, some, None, None, None, some, None, odd, need, None) == INVALID
     many = Problem(**{**GOOD, "experts": 1025})
     assert lib.fasteq_product_scratch(C.byref(many), I32(1), C.byref(one)) == UNSUPPORTED
     assert lib.fasteq_expert_plan_scratch(I64(-1), I32(3), C.byref(one)) == INVALID
