@@ -26,11 +26,6 @@ constexpr float kLog2e = 1.44269502f;
 // did before; infinities come out as 0 and 1.
 __device__ __forceinline__ float sigmoid(float z) { return reciprocal(1.f + power_of_two(z * -kLog2e)); }
 __device__ __forceinline__ double sigmoid(double z) { return 1.0 / (1.0 + exp(-z)); }
-__device__ __forceinline__ float2 sigmoid(float2 z) {
-  const float2 t = vmul(z, make_float2(-kLog2e, -kLog2e));
-  const float2 d = vadd(make_float2(power_of_two(t.x), power_of_two(t.y)), make_float2(1.f, 1.f));
-  return make_float2(reciprocal(d.x), reciprocal(d.y));
-}
 
 // tanh(z): up to 0.8 its Pade approximant of degrees 5 and 4 (8e-9 off at most), beyond (e - 1) / (e + 1) with e = exp(2 |z|), which is 1 from |z| = 9 on
 __device__ __forceinline__ float hyperbolic_tangent(float z) {
@@ -66,21 +61,6 @@ template <int ACT, typename T> __device__ __forceinline__ T activate(T z, T& slo
   }
   slope = T(1);
   return z;
-}
-// two values; the slope where it is asked for
-template <int ACT> __device__ __forceinline__ float2 activate(float2 z, bool with_slope, float2& slope) {
-  if (ACT == kSilu || ACT == kSigmoid) {
-    const float2 s = sigmoid(z), one = make_float2(1.f, 1.f);
-    if (with_slope) {
-      const float2 rest = make_float2(1.f - s.x, 1.f - s.y);
-      slope = ACT == kSilu ? vmul(s, vfma(z, rest, one)) : vmul(s, rest);
-    }
-    return ACT == kSilu ? vmul(z, s) : s;
-  }
-  float2 y;
-  y.x = activate<ACT>(z.x, slope.x);
-  y.y = activate<ACT>(z.y, slope.y);
-  return y;
 }
 template <typename T> __device__ __forceinline__ T activate(int act, T z, T& slope) {
   return act == kSilu ? activate<kSilu>(z, slope) : act == kTanh ? activate<kTanh>(z, slope) : act == kSigmoid ? activate<kSigmoid>(z, slope)

@@ -181,52 +181,30 @@ struct Args {
   int* status;
 };
 
-// a sum of row r (of all) and column n of expert e that is not finite, again with FP32's own products
-template <bool FORWARD, bool SLOPE> __device__ __noinline__ float again(const Args& p, int e, size_t r, int n, float v) {
-  if (fabsf(v) <= 3.402823466e38f) return v;
-  const float *a = p.A + r * p.lda, *d = SLOPE ? p.slope + r * p.ldd : nullptr, *b = p.W + (size_t)e * p.N * p.K + (FORWARD ? (size_t)n * p.K : (size_t)n);
-  v = 0.f;
-#pragma unroll 1
-  for (int k = 0; k < p.K; ++k) v = fmaf(SLOPE ? a[k] * d[k] : a[k], b[FORWARD ? (size_t)k : (size_t)k * p.N], v);
-  return v;
-}
 // 16-byte chunk j of row r in a slab of 32 rows and 32 columns (what a TMA store with 128-byte swizzle takes)
 __device__ __forceinline__ int slab_at(int r, int j) { return r * 128 + ((j ^ (r & 7)) << 4); }
 
-// Values of 16 columns of this thread's row whose sums, in the slab, are not all finite.  Apart from the kernel and with nothing handed back:
-// values whose addresses a call takes would live in memory for good.
+// 32 columns of this thread's row again with FP32's own products, where a sum is not finite.  Apart from the kernel and with nothing handed back: values
+// whose addresses a call takes would live in memory for good.
 template <bool FORWARD, bool SLOPE, int ACT>
-__device__ __noinline__ void wild_row(const Args& p, int e, size_t row, int n, int h, unsigned char* slab, unsigned char* slopes) {
+__device__ __noinline__ void wild_row(const Args& p, int e, size_t row, int n, unsigned char* slab, unsigned char* slopes) {
   const int lane = threadIdx.x & 31;
+  const float *a = p.A + row * p.lda, *g = SLOPE ? p.slope + row * p.ldd : nullptr, *b = p.W + (size_t)e * p.N * p.K + (FORWARD ? (size_t)n * p.K : (size_t)n);
 #pragma unroll 1
-  for (int j = 0; j < 16 && n + j < p.N; ++j) {
-    const int at = slab_at(lane, h * 4 + (j >> 2)) + (j & 3) * 4;
-    float d = 1.f, v = again<FORWARD, SLOPE>(p, e, row, n + j, *reinterpret_cast<const float*>(slab + at));
+  for (int j = 0; j < 32 && n + j < p.N; ++j) {
+    const int at = slab_at(lane, j >> 2) + (j & 3) * 4;
+    float d = 1.f, v = 0.f;
+#pragma unroll 1
+    for (int k = 0; k < p.K; ++k) v = fmaf(SLOPE ? a[k] * g[k] : a[k], b[FORWARD ? (size_t)j * p.K + k : (size_t)k * p.N + j], v);
     if (FORWARD) {
       v = product::activate<ACT>(p.bias ? v + p.bias[(size_t)e * p.N + n + j] : v, d);
-      if (p.residual) v += p.residual[row * p.N + n + j];
       if (ACT != product::kIdentity && p.slope_out) *reinterpret_cast<float*>(slopes + at) = d;
     }
     *reinterpret_cast<float*>(slab + at) = v;
   }
 }
 
-// 16 values from `src`, of which `count` are there
-__device__ __forceinline__ void load_16(const float* src, int count, bool wide, float2 (&v)[8]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (wide) { if (4 * i < count) x = *reinterpret_cast<const float4*>(src + 4 * i); }
-    else {
-      if (4 * i < count) x.x = src[4 * i];
-      if (4 * i + 1 < count) x.y = src[4 * i + 1];
-      if (4 * i + 2 < count) x.z = src[4 * i + 2];
-      if (4 * i + 3 < count) x.w = src[4 * i + 3];
-    }
-    v[2 * i] = make_float2(x.x, x.y);
-    v[2 * i + 1] = make_float2(x.z, x.w);
-  }
-}
+// 16 values to `dst`, of which `count` are there
 __device__ __forceinline__ void store_16(float* dst, int count, bool wide, const float2 (&v)[8]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -239,19 +217,42 @@ __device__ __forceinline__ void store_16(float* dst, int count, bool wide, const
     }
   }
 }
-// A slab's rows, without TMA: where the tile ends inside the tensor (another expert's rows follow), or its rows are not 16-byte aligned.
-__device__ __forceinline__ void store_slab(float* C, size_t row0, int rows, int n0, int N, int pitch, bool wide, const unsigned char* slab) {
+
+// A slab's rows without TMA: plus a residual, where the tile ends inside the tensor (another expert's rows follow), or where rows are not 16-byte aligned.
+__device__ __noinline__ void store_slab(float* C, const float* residual, size_t row0, int rows, int n0, int N, int pitch, bool wide, const unsigned char* slab) {
   const int lane = threadIdx.x & 31;
   if (wide) {
     const int n = n0 + (lane & 7) * 4;
-#pragma unroll 2
-    for (int r = lane >> 3; r < 32; r += 4)
-      if (r < rows && n < N) *reinterpret_cast<float4*>(C + (row0 + r) * pitch + n) = *reinterpret_cast<const float4*>(slab + slab_at(r, lane & 7));
+    if (n >= N) return;
+    for (int r0 = lane >> 3; r0 < rows; r0 += 16) {
+      float4 more[4] = {};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (residual && r0 + 4 * i < rows) more[i] = *reinterpret_cast<const float4*>(residual + (row0 + r0 + 4 * i) * pitch + n);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (r0 + 4 * i >= rows) break;
+        float4 v = *reinterpret_cast<const float4*>(slab + slab_at(r0 + 4 * i, lane & 7));
+        v.x += more[i].x; v.y += more[i].y; v.z += more[i].z; v.w += more[i].w;
+        *reinterpret_cast<float4*>(C + (row0 + r0 + 4 * i) * pitch + n) = v;
+      }
+    }
   } else {
     const int n = n0 + lane;
-#pragma unroll 4
-    for (int r = 0; r < 32; ++r)
-      if (r < rows && n < N) C[(row0 + r) * pitch + n] = *reinterpret_cast<const float*>(slab + slab_at(r, lane >> 2) + (lane & 3) * 4);
+    if (n >= N) return;
+    float* to = C + row0 * pitch + n;
+    const float* from = residual ? residual + row0 * pitch + n : nullptr;
+#pragma unroll 1
+    for (int r0 = 0; r0 < rows; r0 += 8, to += 8 * (size_t)pitch) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = from && r0 + i < rows ? from[(size_t)(r0 + i) * pitch] : 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += *reinterpret_cast<const float*>(slab + slab_at(r0 + i, lane >> 2) + (lane & 3) * 4);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (r0 + i < rows) to[(size_t)i * pitch] = v[i];
+    }
   }
 }
 
@@ -478,22 +479,25 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
       const int quarter = warp & 3, half = (warp - 12) >> 2;
       unsigned char* slab = slabs + (size_t)(warp - 12) * (SLOPE ? 4096 : 8192);
       unsigned char* slopes = slab + 4096;
+      const bool keep = FORWARD && ACT != product::kIdentity && p.slope_out;
       float* bias = biases + (warp - 12) * 32;
       const uint32_t cols = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 32);
       int lt = 0;
       for (int u = 0; u < units; ++u, w.next()) {
         const long long begin = p.groups.first(w.e), left = p.groups.first(w.e + 1) - begin - (long long)w.m * BM;
-        const int rows = (int)(left < BM ? left : BM) - quarter * 32, n0 = w.n * BN + half * 32;      // of this warp
+        const int rows = min((int)(left < BM ? left : BM) - quarter * 32, 32), n0 = w.n * BN + half * 32;      // of this warp, 0 or fewer: none
         const size_t row0 = (size_t)(begin + (long long)w.m * BM + quarter * 32);
         const bool mine = lane < rows;
         if (FORWARD && w.run_begins()) bias[lane] = p.bias && n0 + lane < N ? p.bias[(size_t)w.e * N + n0 + lane] : 0.f;
         for (int k0 = 0; k0 < n_kb; k0 += SEG, ++lt) {
           const int buf = lt & 1;
           const float gain = GAIN * (float)((min(K, (k0 + SEG) * KB) - k0 * KB + 15) / 16);
-          if (lane == 0) bulk_wait_read<0>();      // the slabs' last stores have read them
+          if (lane == 0 && k0 == 0) bulk_wait_read<0>();      // the slabs' last stores have read them
           mbar_wait(&acc_full[buf], (lt >> 1) & 1u, status);
-          // One copy of this code for both halves, and the warp together all through it: it is bound by the instructions of two warps to a
-          // scheduler, which wait for their code where it is long.
+          // One copy of this code for both halves, with what is rare apart, and the warp together all through it: it is bound by the instructions
+          // of two warps to a scheduler, which wait for their code where it is long.
+          const bool whole = k0 + SEG >= n_kb;
+          float check = 0.f;
 #pragma unroll 1
           for (int h = 0; h < 2; ++h) {
             __syncwarp();
@@ -504,85 +508,78 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
             tmem_ld_16_begin(at + BN, y);
             tmem_ld_wait(x);
             tmem_ld_wait(y);
-            float2 v[8], sum = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float2 large = make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
-              v[i] = vadd(large, vfma(large, make_float2(gain, gain), make_float2(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1]))));
+            if (h == 1) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&acc_empty[buf]);
             }
-            float scale = wg::UNSCALE;
-            if (n_kb > SEG) {                        // the sum so far, which this thread left where its result goes
-              float* C = p.C + (row0 + lane) * N + n0 + h * 16;
-              if (k0 > 0) {
-                float2 before[8];
-                load_16(C, mine ? N - n0 - h * 16 : 0, p.c_wide, before);
+            float v[16];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = vfma(v[i], make_float2(scale, scale), before[i]);
-                scale = 1.f;
-              }
-              if (k0 + SEG < n_kb) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = vmul(v[i], make_float2(scale, scale));
-                store_16(C, mine ? N - n0 - h * 16 : 0, p.c_wide, v);
-                continue;
-              }
+            for (int i = 0; i < 16; ++i) {
+              const float large = __uint_as_float(x[i]);
+              v[i] = large + fmaf(large, gain, __uint_as_float(y[i]));
             }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sum = vadd(sum, v[i]);
-            if (__any_sync(0xffffffffu, mine && !(fabsf(sum.x + sum.y) <= 3.402823466e38f))) {      // a sum may not be finite
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                *reinterpret_cast<float4*>(slab + slab_at(lane, h * 4 + j)) = make_float4(v[2 * j].x * scale, v[2 * j].y * scale, v[2 * j + 1].x * scale, v[2 * j + 1].y * scale);
-              if (mine) wild_row<FORWARD, SLOPE, ACT>(p, w.e, row0 + lane, n0 + h * 16, h, slab, slopes);
-              continue;
-            }
-            if (FORWARD) {
+            if (k0 > 0) {                            // and the sums so far
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
-                const float4 b = *reinterpret_cast<const float4*>(bias + h * 16 + 4 * j);
-                v[2 * j] = vfma(v[2 * j], make_float2(scale, scale), make_float2(b.x, b.y));
-                v[2 * j + 1] = vfma(v[2 * j + 1], make_float2(scale, scale), make_float2(b.z, b.w));
+                const float4 before = *reinterpret_cast<const float4*>(slab + slab_at(lane, h * 4 + j));
+                v[4 * j] += before.x; v[4 * j + 1] += before.y; v[4 * j + 2] += before.z; v[4 * j + 3] += before.w;
               }
-              if (ACT != product::kIdentity) {
-                float2 d[8];
-                const bool keep = p.slope_out != nullptr;
+            }
+            if (whole) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = product::activate<ACT>(v[i], keep, d[i]);
-                if (keep) {
+              for (int i = 0; i < 16; i += 4) check += (v[i] + v[i + 1]) + (v[i + 2] + v[i + 3]);
+              if (FORWARD) {
 #pragma unroll
-                  for (int j = 0; j < 4; ++j)
-                    *reinterpret_cast<float4*>(slopes + slab_at(lane, h * 4 + j)) = make_float4(d[2 * j].x, d[2 * j].y, d[2 * j + 1].x, d[2 * j + 1].y);
+                for (int j = 0; j < 4; ++j) {
+                  const float4 b = *reinterpret_cast<const float4*>(bias + h * 16 + 4 * j);
+                  v[4 * j] = fmaf(v[4 * j], wg::UNSCALE, b.x); v[4 * j + 1] = fmaf(v[4 * j + 1], wg::UNSCALE, b.y);
+                  v[4 * j + 2] = fmaf(v[4 * j + 2], wg::UNSCALE, b.z); v[4 * j + 3] = fmaf(v[4 * j + 3], wg::UNSCALE, b.w);
                 }
-              }
-              if (p.residual) {
-                float2 res[8];
-                load_16(p.residual + (row0 + lane) * N + n0 + h * 16, mine ? N - n0 - h * 16 : 0, p.c_wide, res);
+                if (ACT != product::kIdentity) {
+                  if (keep) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = vadd(v[i], res[i]);
-              }
-            } else {
+                    for (int j = 0; j < 4; ++j) {
+                      float d[4];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) v[i] = vmul(v[i], make_float2(scale, scale));
+                      for (int i = 0; i < 4; ++i) v[4 * j + i] = product::activate<ACT>(v[4 * j + i], d[i]);
+                      *reinterpret_cast<float4*>(slopes + slab_at(lane, h * 4 + j)) = make_float4(d[0], d[1], d[2], d[3]);
+                    }
+                  } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                      float d;
+                      v[i] = product::activate<ACT>(v[i], d);
+                    }
+                  }
+                }
+              } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[i] *= wg::UNSCALE;
+              }
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              *reinterpret_cast<float4*>(slab + slab_at(lane, h * 4 + j)) = make_float4(v[2 * j].x, v[2 * j].y, v[2 * j + 1].x, v[2 * j + 1].y);
+              *reinterpret_cast<float4*>(slab + slab_at(lane, h * 4 + j)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
           }
-          tc_fence_before();
+          if (!whole) continue;
+          if (mine && !(fabsf(check) <= 3.402823466e38f)) wild_row<FORWARD, SLOPE, ACT>(p, w.e, row0 + lane, n0, slab, slopes);
           fence_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&acc_empty[buf]);
-          if (k0 + SEG < n_kb) continue;
-          const bool keep = FORWARD && ACT != product::kIdentity && p.slope_out;
-          if (p.c_wide && (rows >= 32 || row0 + rows == (size_t)p.groups.rows)) {
-            if (lane == 0 && rows > 0 && n0 < N) {
-              tma_store_3d(&tmC, n0, (int)row0, slab);
-              if (keep) tma_store_3d(&tmD, n0, (int)row0, slopes);
-              bulk_commit();
+          if (n0 < N && rows > 0) {
+            if (p.c_wide && !p.residual && (rows == 32 || row0 + rows == (size_t)p.groups.rows)) {
+              if (lane == 0) tma_store_3d(&tmC, n0, (int)row0, slab);
+            } else {
+              store_slab(p.C, p.residual, row0, rows, n0, N, N, p.c_wide, slab);
             }
-          } else {
-            store_slab(p.C, row0, rows, n0, N, N, p.c_wide, slab);
-            if (keep) store_slab(p.slope_out, row0, rows, n0, N, p.ldd, true, slopes);
+            if (keep) {
+              if (rows == 32 || row0 + rows == (size_t)p.groups.rows) {
+                if (lane == 0) tma_store_3d(&tmD, n0, (int)row0, slopes);
+              } else {
+                store_slab(p.slope_out, nullptr, row0, rows, n0, N, p.ldd, true, slopes);
+              }
+            }
+            if (lane == 0) bulk_commit();
           }
           __syncwarp();
         }

@@ -5,10 +5,10 @@
 // rows as contraction index: both operands are split column by column as they come, thread = channel, pairs of rows packed, so nothing is turned.
 // A CTA takes a chunk of an expert's rows and a tile of 128 x 64 of its matrix:
 //   warp 0       brings blocks of 32 rows of g (and slope) and x (TMA)
-//   warp 1       issues the MMAs
+//   warps 1, 2   issue the MMAs, of the even blocks and of the odd ones: each has accumulators of its own, and its waits pass under the other's MMAs
 //   warps 4-11   split g into tensor memory, four warps the even and four the odd blocks, and add its columns for gb
 //   warps 12-15  split x into shared memory
-//   warps 16-23  every 256 rows add the accumulators to their registers; in the end write the tile's sums
+//   warps 16-23  every 256 rows of either add the accumulators to their registers; in the end write the tile's sums
 // Chunks are long enough to give each SM one tile (at least 256 rows); an expert of several chunks leaves partial sums, which a second kernel adds
 // in order.  Sums that are not finite are formed again in FP32, the whole tile.
 #pragma once
@@ -115,30 +115,26 @@ __global__ void __launch_bounds__(NTW, 1) product_wgrad_tc_kernel(const __grid_c
         }
         __syncwarp();
       }
-    } else if (warp == 1) {
+    } else if (warp == 1 || warp == 2) {
       // ------------------------------------------------------------------ MMAs
+      const int pipe = warp - 1;
       const uint32_t idesc2 = wg::idesc_bf16_m128(2 * BN), idesc1 = wg::idesc_bf16_m128(BN), tm = uniform(tmem);
       const uint64_t desc0 = wg::desc_sw64(uniform(smem_u32(smem)));
-      for (int i = 0; i < n_blocks; ++i) {
-        const int slot = i % A_SLOTS, bs = i % SLOTS_W, seg = i / SEG_W, buf = seg & 1;
-        if (i % SEG_W == 0) mbar_wait(&acc_empty[buf], ((seg >> 1) & 1u) ^ 1u, status);
-        if (i == 0) { mbar_wait(&b_full[0], 0, status); mbar_wait(&s_full[0], 0, status); }
+      const uint32_t d = tm + (uint32_t)pipe * ACC_COLS;
+      for (int i = pipe, j = 0; i < n_blocks; i += 2, ++j) {
+        const int slot = i % A_SLOTS, bs = i % SLOTS_W;
+        if (j % SEG_W == 0) mbar_wait(&acc_empty[pipe], ((j / SEG_W) & 1u) ^ 1u, status);
+        mbar_wait(&b_full[bs], (i / SLOTS_W) & 1u, status);
+        mbar_wait(&s_full[slot], (i / A_SLOTS) & 1u, status);
         __syncwarp();
         tc_fence_after();
-        const uint32_t d = tm + (uint32_t)buf * ACC_COLS, a = tm + A_COL0 + (uint32_t)(slot * A_COLS);
+        const uint32_t a = tm + A_COL0 + (uint32_t)(slot * A_COLS);
         const uint64_t b = desc_at(desc0, (uint32_t)(bs * B_BYTES));
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
-          if (ks == 1) {                           // the next block is waited for while this one's MMAs run
-            if (i + 1 < n_blocks) {
-              mbar_wait(&b_full[(i + 1) % SLOTS_W], ((i + 1) / SLOTS_W) & 1u, status);
-              mbar_wait(&s_full[(i + 1) % A_SLOTS], ((i + 1) / A_SLOTS) & 1u, status);
-            }
-            __syncwarp();
-          }
           const uint64_t w1 = desc_at(b, (uint32_t)(ks * 32)), w2 = desc_at(w1, B_PART), w3 = desc_at(w1, 2 * B_PART);
           const uint32_t v1 = a + (uint32_t)(ks * 8), v2 = v1 + KB / 2, v3 = v1 + KB;
-          warp_mma_bf16_a_tmem(d, v1, w1, idesc2, i % SEG_W || ks ? 1u : 0u);
+          warp_mma_bf16_a_tmem(d, v1, w1, idesc2, j % SEG_W || ks ? 1u : 0u);
           warp_mma_bf16_a_tmem(d + BN, v1, w3, idesc1, 1u);
           warp_mma_bf16_a_tmem(d + BN, v2, w1, idesc1, 1u);
           warp_mma_bf16_a_tmem(d + BN, v2, w2, idesc1, 1u);
@@ -146,7 +142,7 @@ __global__ void __launch_bounds__(NTW, 1) product_wgrad_tc_kernel(const __grid_c
         }
         warp_mma_commit(&s_empty[slot]);
         warp_mma_commit(&b_empty[bs]);
-        if ((i + 1) % SEG_W == 0 || i + 1 == n_blocks) warp_mma_commit(&acc_full[buf]);
+        if ((j + 1) % SEG_W == 0 || i + 2 >= n_blocks) warp_mma_commit(&acc_full[pipe]);
       }
     } else if (warp >= 4 && warp < 12) {
       // ------------------------------------------------------------------ g: thread = channel = TMEM lane
@@ -215,10 +211,14 @@ __global__ void __launch_bounds__(NTW, 1) product_wgrad_tc_kernel(const __grid_c
       float2 sum[16];
 #pragma unroll
       for (int j = 0; j < 16; ++j) sum[j] = make_float2(0.f, 0.f);
-      const int n_seg = (n_blocks + SEG_W - 1) / SEG_W;
-      for (int seg = 0; seg < n_seg; ++seg) {
-        const int buf = seg & 1;
-        const float gain = GAIN * (float)((min(c.rows, (seg + 1) * SEG_W * ROWS) - seg * SEG_W * ROWS + 15) / 16);
+      // accumulations of the two pipes in turn: 0 and 1 their first, 2 and 3 their second, ...
+      const int n_acc = (n_blocks + 2 * SEG_W - 1) / (2 * SEG_W) * 2;
+      for (int seg = 0; seg < n_acc; ++seg) {
+        const int buf = seg & 1, first = (seg >> 1) * 2 * SEG_W + buf, blocks = min(SEG_W, (n_blocks - first + 1) / 2);
+        if (blocks <= 0) continue;
+        const bool last = first + 2 * blocks - 2 == n_blocks - 1;
+        const int steps = 2 * blocks - (last && c.rows - (n_blocks - 1) * ROWS <= 16 ? 1 : 0);      // of 16 rows
+        const float gain = GAIN * (float)steps;
         mbar_wait(&acc_full[buf], (seg >> 1) & 1u, status);
         __syncwarp();
         tc_fence_after();
