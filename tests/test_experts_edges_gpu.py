@@ -47,6 +47,31 @@ def test_weight_gradients_that_are_not_finite(M, K, N, act):
     assert torch.all((gx.cpu().double() - ref).abs()[rows] <= tol[rows])
 
 
+@pytest.mark.parametrize("act", ["silu", "tanh", None])
+@pytest.mark.parametrize("M,K,N", [(300, 64, 96), (200, 33, 50), (150, 600, 40)])
+def test_values_that_are_not_finite_with_a_residual(M, K, N, act):
+    """Rows whose sums are not finite are formed again, with bias, activation, residual and slope; the others are as without them."""
+    from fasteq_b200.ops.dense_act import dense_act
+    x, w, b, r, g = single._inputs(M, K, N, torch.float32)
+    clean = single.run(x, w, b, r, g, act)
+    wild = [7, M // 2, M - 1]
+    x[7], x[M // 2, 3], x[M - 1, K - 1] = 2.0 ** 115, float("inf"), float("nan")       # 2^115: finite, its sums are too
+    leaf = x.cuda().requires_grad_(True)
+    y = dense_act(leaf, w.cuda(), b.cuda(), act, r.cuda())
+    (gx,) = torch.autograd.grad(y, leaf, g.cuda())
+    z = x @ w.t() + b
+    pattern = single.F[act](z) + r
+    y, gx = y.detach().cpu(), gx.cpu()
+    assert torch.equal(y.isnan(), pattern.isnan()) and torch.equal(y.isinf(), pattern.isinf())
+    want = single.reference(x[7:8], w, b, r[7:8], g[7:8], act, single.U[torch.float32])
+    for n, v in (("y", y), ("x", gx)):
+        ref, tol = want[n]
+        assert torch.all((v[7:8].double() - ref).abs() <= tol), n
+    others = [i for i in range(M) if i not in wild]
+    assert torch.equal(y[others], clean["y"].cpu()[others]) and torch.equal(gx[others], clean["x"].cpu()[others])
+    assert gx[M - 1].isnan().all() or act is None
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
 @pytest.mark.parametrize("K,N", [(64, 64), (20, 33)])
 def test_one_experts_infinities_stay_with_it(K, N, dtype):
