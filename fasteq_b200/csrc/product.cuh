@@ -27,7 +27,7 @@ constexpr float kLog2e = 1.44269502f;
 __device__ __forceinline__ float sigmoid(float z) { return reciprocal(1.f + power_of_two(z * -kLog2e)); }
 // In FP64 exp(t) = 2^n exp(r), t = n ln 2 + r (ln 2 in two parts, the first of 33 bits, so that its product with n is exact), exp(r) by its Taylor polynomial
 // of degree 13 (|r| <= 0.347: 4e-18 left out); the reciprocal by Newton's iteration, each step squaring the error of the first 20 bits.  No branch, so that
-// a thread's values run side by side.  |z| beyond 700 counts as 700: 1e-304, or one.
+// a thread's values run side by side.  Beyond |z| = 700 it is 0 (for 1e-304) or one.
 __device__ __forceinline__ double sigmoid(double z) {
   const double t = z < -700.0 ? 700.0 : z > 700.0 ? -700.0 : -z, n = rint(t * 0x1.71547652b82fep+0);
   const double r = fma(n, -0x1.473de6af278edp-34, fma(n, -0x1.62e42fef00000p-1, t));
@@ -49,7 +49,8 @@ __device__ __forceinline__ double sigmoid(double z) {
   double y;
   asm("rcp.approx.ftz.f64 %0, %1;" : "=d"(y) : "d"(d));
   y = fma(y, fma(-d, y, 1.0), y);
-  return fma(y, fma(-d, y, 1.0), y);
+  y = fma(y, fma(-d, y, 1.0), y);
+  return z < -700.0 ? 0.0 : y;
 }
 
 // tanh(z): up to 0.8 its Pade approximant of degrees 5 and 4 (8e-9 off at most), beyond (e - 1) / (e + 1) with e = exp(2 |z|), which is 1 from |z| = 9 on

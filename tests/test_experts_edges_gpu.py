@@ -47,6 +47,34 @@ def test_weight_gradients_that_are_not_finite(M, K, N, act):
     assert torch.all((gx.cpu().double() - ref).abs()[rows] <= tol[rows])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+@pytest.mark.parametrize("act", ["silu", "tanh", "sigmoid", "abs"])
+def test_activations_over_the_whole_line(act, dtype):
+    """Values and slopes of a layer of one channel and weight one, from the smallest arguments to infinity and NaN.  Within 8 half steps of the value (of one,
+    for slopes, and of the exponential's argument: FP32 rounds z log2(e), which moves exp by |z| half steps), or of the smallest normal number."""
+    from fasteq_b200.ops.dense_act import dense_act
+    inf = float("inf")
+    z = torch.cat([s * torch.logspace(-30, 2, 3001, dtype=torch.float64) for s in (1, -1)])
+    z = torch.cat([z, torch.linspace(-20, 20, 4001, dtype=torch.float64), torch.tensor([0.0, 88.0, -88.0, 709.0, -709.0, 750.0, -750.0, 3e30, -3e30, inf, -inf, float("nan")])])
+    z = z.to(dtype).unsqueeze(1)
+    leaf = z.cuda().requires_grad_(True)
+    y = dense_act(leaf, torch.ones(1, 1, dtype=dtype, device="cuda"), None, act)
+    (d,) = torch.autograd.grad(y.sum(), leaf)
+    want = z.double().requires_grad_(True)
+    ref = single.F[act](want)
+    (slope,) = torch.autograd.grad(ref.sum(), want)
+    y, d, ref, z = y.detach().cpu().double(), d.cpu().double(), ref.detach(), z.double()
+    assert torch.equal(y.isnan(), ref.isnan()) and torch.equal(y.isinf(), ref.isinf())
+    u, least = single.U[dtype], torch.finfo(dtype).tiny * 1e8 if dtype == torch.float64 else torch.finfo(dtype).tiny
+    ok = ref.isfinite() & z.isfinite()
+    reach = z.abs().clamp(max=800)                                       # beyond, the exponential is 0 in both types
+    off, may = (y - ref).abs(), (8 + 2 * reach) * u * ref.abs() + least * (1 + reach)
+    assert torch.all(off[ok] <= may[ok]), float((off - may)[ok].max())
+    # a slope is a sum of terms up to one and |z| exp(-|z|) <= 0.4, each off by what the sigmoid is, in FP32 by |z| half steps of it
+    off, may = (d - slope).abs(), 9 * u * torch.ones_like(d) + 2 * reach * u * (slope.abs() + torch.exp(-reach)) + least * (1 + reach)
+    assert torch.all(off[ok] <= may[ok]), float((off - may)[ok].max())
+
+
 @pytest.mark.parametrize("act", ["silu", "tanh", None])
 @pytest.mark.parametrize("M,K,N", [(300, 64, 96), (200, 33, 50), (150, 600, 40)])
 def test_values_that_are_not_finite_with_a_residual(M, K, N, act):
