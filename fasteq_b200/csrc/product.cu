@@ -1,6 +1,9 @@
 // Dense layers with an epilogue, one matrix for all rows or one per expert (rows in the experts' order):
 //   z = x W[e]^T + bias[e],  y = act(z) + residual;   gz = grad_y act'(z):  grad_x = gz W[e],  grad_w[e] = gz^T x,  grad_bias[e] = sum gz
-// FMA kernels for every extent, FP32 and FP64: 64 x 64 tiles of 4 x 4 sums a thread.
+// FP32 goes to the tensor cores (product_tc.cuh, product_wgrad_tc.cuh), FP64 to the FP64 ones (product_f64.cuh).  Here are the entries, and FMA kernels for what
+// those do not take (addresses that are not 16-byte aligned, no channels to sum over, extents beyond their 32-bit counts): 64 x 64 tiles of 4 x 4 sums a
+// thread, bound by shared-memory reads.  12,288 rows of 128 to 256 channels, forward / grad_x / weights: 43 / 55 / 60 us, on the tensor
+// cores 16 / 16 / 18 us.
 #include <algorithm>
 #include <atomic>
 #include <mutex>
@@ -242,7 +245,7 @@ template <auto KERNEL> cudaError_t allow_shared_memory(int device) {
 // CTAs of a launch over tiles of rows and columns
 bool in_32_bits(const fasteq_product_problem* p, int tile) {
   const long long columns = (std::max(p->k, p->n) + tile - 1) / tile, rows = p->rows / tile + p->experts + 1;
-  return rows * columns <= 0x7fffffffLL && columns * columns * (p->rows / 256 + p->experts) <= 0x7fffffffLL;
+  return rows * columns <= 0x7fffffffLL && columns * columns * (p->rows / 64 + p->experts) <= 0x7fffffffLL;
 }
 bool even(int extent, std::initializer_list<const void*> pointers) {
   uintptr_t all = 0;
@@ -263,13 +266,16 @@ int product_f64(const fasteq_product_problem* p, const void* A, const void* w, c
   return e == cudaSuccess ? FASTEQ_OK : cuda_fail(e);
 }
 
-// Rows of a chunk: as many as give every SM `per_sm` tiles of rows x matrix, in one wave.  Every expert may add a chunk to those; many experts take
-// half of the places at most.  At least 256 rows: below that a chunk's start and its sums' way out take longer than its rows.
+// Rows of a chunk: as many as give every SM `per_sm` tiles of rows x matrix, in one wave (24,576 rows of 128 x 256 in FP32: 148 CTAs 18.4 us, 196 CTAs
+// 28.4, 100 CTAs 23.8).  Every expert may add a chunk to those; many experts take half of the places at most.  At least 64 rows (1,000 rows of 128 x 256 with
+// the sums' way out: FP32 16.1 us, 18.4 with 256 rows at least; FP64 31.7 and 39.8).  Experts of 256 rows or fewer on average stay whole, and need no
+// partial sums (ten experts of 100 rows, 128 x 256, FP64: 27.5 us, 42.1 in pieces of 64; of 400 rows 68.9 and 50.4).
 int chunk_rows(const fasteq_product_problem* p, int tile_n, int tile_k, int per_sm) {
   const long long tiles = (long long)((p->n + tile_n - 1) / tile_n) * std::max(1, (p->k + tile_k - 1) / tile_k), places = std::max<long long>(1, 148 * per_sm / tiles);
   const long long chunks = std::max<long long>(std::max<long long>(places - (p->experts > 1 ? p->experts : 0), places / 2), 1);
   const long long rows = ((p->rows + chunks - 1) / chunks + 31) / 32 * 32;
-  return (int)std::min<long long>(1 << 24, std::max<long long>(256, rows));
+  const long long least = p->experts > 1 && p->rows <= 256LL * p->experts ? 256 : 64;
+  return (int)std::min<long long>(1 << 24, std::max<long long>(least, rows));
 }
 int chunk_rows(const fasteq_product_problem* p, bool tensor_cores) { return tensor_cores ? chunk_rows(p, pwg::TM, pwg::TN, 1) : chunk_rows(p, TILE, TILE, 3); }
 

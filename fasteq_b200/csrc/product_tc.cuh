@@ -15,8 +15,16 @@
 //   warps 2-3    load, split and store the weights' k-blocks, or bring the split ones
 //   warps 4-11   split raw blocks into tensor memory (thread = row = TMEM lane), four warps the even and four the odd ones
 //   warps 12-19  split the first weights, then add the two accumulators, bias, activation and residual, and store tiles of 32 x 32 by TMA
-// Every 256 of k the accumulators are emptied (into C, for the sum to go on from there): see GAIN.
-// All waits are bounded; sums that are not finite (operands that are not, or beyond the split's range) are formed again in FP32.
+// Every 256 of k the accumulators are emptied (into the slabs, for the sum to go on from there): see GAIN.
+// All waits are bounded; sums that are not finite (operands that are not, or beyond the split's range) are formed again in FP32, the 32 columns of
+// such a row that a warp holds.
+//
+// Why so: 2 x 128 columns of accumulators and 4 x 48 of A's parts fill 448 of the 512 columns of tensor memory, eight blocks of the weights (k = 256), four
+// raw ones of A and the slabs 227 KB of shared memory.  The six products' rate is the bf16 one / 6 (271 TFLOP/s of 1627), a K = 16 step takes 25 + 0.44
+// columns clocks an MMA, 294 for the five.  Measured: 100,000 rows of 256 to 256 channels 99 us (132 TFLOP/s of FP32-accurate products; the MMA warp's
+// handshakes leave the tensor cores idle for half of a block's 1,050 clocks), 24,576 of 128 to 256 21 us, 644,000 of 64 to 64 with SiLU 75 us (330 MB,
+// 4.4 TB/s: the epilogue's instructions), 192 of 128 to 128 8 us (one tile's chain).  Two tiles side by side with an issuing warp each instead: 90, 21.6,
+// 77 and 8.4 us, taken back; 16 warps of the epilogue spill at 72 registers.
 #pragma once
 #include "product.cuh"
 #include "tcgen05_util.cuh"

@@ -11,6 +11,8 @@
 //   warps 16-23  every 256 rows of either add the accumulators to their registers; in the end write the tile's sums
 // Chunks are long enough to give each SM one tile (at least 256 rows); an expert of several chunks leaves partial sums, which a second kernel adds
 // in order.  Sums that are not finite are formed again in FP32, the whole tile.
+// Bound: the warps' instructions between the waits (the tensor cores are busy for 31 %, issue slots for 53 % of the time).  Measured, g without a slope:
+// 12,288 rows of 128 x 256 12.9 us, 24,576 18.8 us, 100,000 of 128 x 128 32.0 us (103 TFLOP/s of FP32-accurate products; one issuing warp: 34.3).
 #pragma once
 #include "product_tc.cuh"
 
