@@ -100,8 +100,10 @@ __device__ __forceinline__ void multiply(double* smem, const Operand& a, const O
                        : "+d"(sum[i][j][0]), "+d"(sum[i][j][1]) : "d"(x[i]), "d"(y[j]));
     }
     if (COLUMNS && threadIdx.x < TILE) {
+      double part = 0.0;                 // two levels: a long sum's error is its additions'
 #pragma unroll
-      for (int k = 0; k < BK; ++k) column += st[A_OUTER ? threadIdx.x * OUTER_PITCH + k : k * K_PITCH + threadIdx.x];
+      for (int k = 0; k < BK; ++k) part += st[A_OUTER ? threadIdx.x * OUTER_PITCH + k : k * K_PITCH + threadIdx.x];
+      column += part;
     }
   }
   wait_async<0>();
