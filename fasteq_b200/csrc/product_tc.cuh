@@ -179,6 +179,9 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, int column,
                : "memory");
 }
 
+// a map on its way to the cache before its first copy needs it
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
+
 struct Args {
   Groups groups;
   const float *A, *slope, *W, *bias, *residual;
@@ -308,30 +311,38 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
     for (int s = 0; s < A_SLOTS; ++s) { mbar_init(&s_full[s], 4); mbar_init(&s_empty[s], 1); }
     for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 8); }
     mbar_fence_init();
+    tiles[0] = 0;                                  // of one matrix; experts' follow
+    tiles[1] = (int)((p.groups.rows + BM - 1) / BM);
   }
   if (warp == 1) tmem_alloc(tmem_slot, 512);
+  if (threadIdx.x == 64) {
+    prefetch_map(&tmA);
+    if (SLOPE) prefetch_map(&tmSlope);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   wait_for_previous_kernel();
-  for (int e = threadIdx.x; e < X; e += NT) tiles[e] = (int)((p.groups.first(e + 1) - p.groups.first(e) + BM - 1) / BM);
-  __syncthreads();
-  if (warp == 0) {
-    int total = 0;
-    for (int e0 = 0; e0 < X; e0 += 32) {
-      const int v = e0 + lane < X ? tiles[e0 + lane] : 0;
-      int sum = v;
+  if (p.groups.offsets) {
+    for (int e = threadIdx.x; e < X; e += NT) tiles[e] = (int)((p.groups.first(e + 1) - p.groups.first(e) + BM - 1) / BM);
+    __syncthreads();
+    if (warp == 0) {
+      int total = 0;
+      for (int e0 = 0; e0 < X; e0 += 32) {
+        const int v = e0 + lane < X ? tiles[e0 + lane] : 0;
+        int sum = v;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += u;
+        for (int o = 1; o < 32; o <<= 1) {
+          const int u = __shfl_up_sync(0xffffffffu, sum, o);
+          if (lane >= o) sum += u;
+        }
+        if (e0 + lane < X) tiles[e0 + lane] = total + sum - v;
+        total += __shfl_sync(0xffffffffu, sum, 31);
       }
-      if (e0 + lane < X) tiles[e0 + lane] = total + sum - v;
-      total += __shfl_sync(0xffffffffu, sum, 31);
+      if (lane == 0) tiles[X] = total;
     }
-    if (lane == 0) tiles[X] = total;
+    __syncthreads();
   }
-  __syncthreads();
   const uint32_t tmem = *tmem_slot;
   const int n_tiles = (N + BN - 1) / BN, n_kb = (K + KB - 1) / KB;
   const bool resident = p.split == nullptr;        // n_kb <= slots then

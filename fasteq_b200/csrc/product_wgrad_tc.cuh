@@ -91,6 +91,11 @@ __global__ void __launch_bounds__(NTW, 1) product_wgrad_tc_kernel(const __grid_c
     *redo = 0;
   }
   if (warp == 1) tmem_alloc(tmem_slot, 512);
+  if (threadIdx.x == 64) {
+    prefetch_map(&tmG);
+    prefetch_map(&tmX);
+    if (SLOPE) prefetch_map(&tmD);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
