@@ -290,3 +290,16 @@ def test_extents_beyond_32_bits_are_refused():
         expert_gather(one.expand(1, big), plan)
     with pytest.raises(ValueError, match="expert_combine: a row's values"):
         expert_combine(one.expand(1, big), plan)
+
+
+def test_dual_tensors_are_refused():
+    """Forward-mode differentiation is not offered: a tangent is not dropped in silence."""
+    import torch.autograd.forward_ad as forward_ad
+    from fasteq_b200.ops.dense_act import dense_act
+    from fasteq_b200.ops.experts import expert_combine, expert_gather, expert_plan
+    plan = expert_plan(torch.tensor([0, 1, 0], device="cuda"), 2)
+    with forward_ad.dual_level():
+        x = forward_ad.make_dual(torch.ones(3, 4, device="cuda"), torch.ones(3, 4, device="cuda"))
+        for call in (lambda: dense_act(x, torch.ones(2, 4, device="cuda")), lambda: expert_gather(x, plan), lambda: expert_combine(x, plan)):
+            with pytest.raises(RuntimeError):
+                call()
