@@ -262,8 +262,17 @@ __device__ __noinline__ void store_slab(float* C, const float* residual, size_t 
       }
     }
   } else {
-    const int n = n0 + lane;
-    if (n >= N) return;
+    const int n = n0 + lane, columns = N - n0;
+    if (columns < 32) {                    // a few columns of many rows, side by side in the lanes
+#pragma unroll 4
+      for (int i = lane; i < rows * columns; i += 32) {
+        const int r = i / columns, c = i - r * columns;
+        const size_t at = (row0 + r) * pitch + n0 + c;
+        const float v = *reinterpret_cast<const float*>(slab + slab_at(r, c >> 2) + (c & 3) * 4);
+        C[at] = residual ? v + residual[at] : v;
+      }
+      return;
+    }
     float* to = C + row0 * pitch + n;
     const float* from = residual ? residual + row0 * pitch + n : nullptr;
 #pragma unroll 1
