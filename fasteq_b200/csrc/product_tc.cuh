@@ -15,7 +15,10 @@
 //   warps 2-3    load, split and store the weights' k-blocks, or bring the split ones
 //   warps 4-11   split raw blocks into tensor memory (thread = row = TMEM lane), four warps the even and four the odd ones
 //   warps 12-19  split the first weights, then add the two accumulators, bias, activation and residual, and store tiles of 32 x 32 by TMA
-// Every 256 of k the accumulators are emptied (into the slabs, for the sum to go on from there): see GAIN.
+// Every 256 of k the accumulators are emptied (into the slabs, for the sum to go on from there), which bounds what the truncations add up to.  Nothing is given
+// back for them: that would move sums that lose nothing (one-hot rows, whole numbers), which come out exact so.  Errors against 64 bits (2-norm, 1e-8;
+// torch's FP32 products, this) at k = 64, 256, 1,664: operands of both signs 14.4, 7.0; 28.6, 23.1; 73.2, 23.1; of one sign, where truncations do not cancel,
+// 12.2, 9.0; 24.7, 38.7; 56.1, 36.5.
 // All waits are bounded; sums that are not finite (operands that are not, or beyond the split's range) are formed again in FP32, the 32 columns of
 // such a row that a warp holds.
 //
@@ -41,11 +44,6 @@ constexpr int SEG = 256 / KB;              // k-blocks of an accumulation
 constexpr int A_BYTES = BM * KB * 4, B_PART = BN * KB * 2, B_BYTES = 3 * B_PART;
 constexpr uint32_t ACC_COLS = 2 * BN, A_COL0 = 2 * ACC_COLS, A_COLS = 3 * KB / 2;
 constexpr int A_SLOTS = 4;                 // of tensor memory: 2 x 128 columns of accumulators, 4 x 48 of A's parts
-// What a K = 16 step's truncation costs on average, of the sum: measured 0.18 to 0.21 x 2^-24 with operands of both signs, 0.27 to 0.40 with those of
-// one.  Given back with the small parts.  Errors (2-norm, 1e-8; torch's FP32 products, this without the gain, this) at k = 64, 128, 256: both signs
-// 14.5, 7.1, 5.1; 20.3, 12.1, 7.9; 28.8, 22.9, 14.4; one sign 12.2, 9.1, 5.0; 17.5, 17.9, 8.6; 24.7, 38.8, 15.3.
-constexpr float GAIN = 0.27f / 16777216.f;
-
 template <bool SLOPE> struct Cfg {
   // Even: a stage then always belongs to the same set of split warps, which sees each of its phases (a set that saw every other one could take
   // the parity of a phase long past for its own).
@@ -532,7 +530,6 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
         if (FORWARD && w.run_begins()) bias[lane] = p.bias && n0 + lane < N ? p.bias[(size_t)w.e * N + n0 + lane] : 0.f;
         for (int k0 = 0; k0 < n_kb; k0 += SEG, ++lt) {
           const int buf = lt & 1;
-          const float gain = GAIN * (float)((min(K, (k0 + SEG) * KB) - k0 * KB + 15) / 16);
           if (lane == 0 && k0 == 0) bulk_wait_read<0>();      // the slabs' last stores have read them
           if (early) {
             __syncwarp();
@@ -561,10 +558,7 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
             }
             float v[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float large = __uint_as_float(x[i]);
-              v[i] = large + fmaf(large, gain, __uint_as_float(y[i]));
-            }
+            for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(x[i]) + __uint_as_float(y[i]);
             if (k0 > 0) {                            // and the sums so far
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
