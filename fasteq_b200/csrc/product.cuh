@@ -53,14 +53,13 @@ __device__ __forceinline__ double sigmoid(double z) {
   return z < -700.0 ? 0.0 : y;
 }
 
-// tanh(z): up to 0.8 its Pade approximant of degrees 5 and 4 (8e-9 off at most), beyond (e - 1) / (e + 1) with e = exp(2 |z|), which is 1 from |z| = 9 on
+// tanh(z): up to |z| = 0.8 its Pade approximant of degrees 5 and 4 (8e-9 off at most), beyond 1 - 2 / (exp(2 |z|) + 1), which is nowhere above one (so that
+// the slope is nowhere negative) and one itself from |z| = 10 on
 __device__ __forceinline__ float hyperbolic_tangent(float z) {
-  float a;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(fabsf(z)), "f"(20.f));
-  const float e = power_of_two(a * (2.f * kLog2e)), q = z * z;
+  const float a = fabsf(z), e = power_of_two(a * (2.f * kLog2e)), q = z * z;
   const bool small = a <= 0.8f;
-  const float num = small ? z * fmaf(q, 105.f + q, 945.f) : copysignf(e - 1.f, z), den = small ? fmaf(q, fmaf(q, 15.f, 420.f), 945.f) : e + 1.f;
-  return num * reciprocal(den);
+  const float r = reciprocal(small ? fmaf(q, fmaf(q, 15.f, 420.f), 945.f) : e + 1.f);
+  return small ? z * fmaf(q, 105.f + q, 945.f) * r : copysignf(fmaf(-2.f, r, 1.f), z);
 }
 __device__ __forceinline__ double hyperbolic_tangent(double z) { return tanh(z); }
 
