@@ -25,8 +25,8 @@
 // Why so: 2 x 128 columns of accumulators and 4 x 48 of A's parts fill 448 of the 512 columns of tensor memory, eight blocks of the weights (k = 256), four
 // raw ones of A and the slabs 227 KB of shared memory.  The six products' rate is the bf16 one / 6 (271 TFLOP/s of 1627), a K = 16 step takes 25 + 0.44
 // columns clocks an MMA, 294 for the five.  Measured: 100,000 rows of 256 to 256 channels 99 us (132 TFLOP/s of FP32-accurate products; the ten MMAs
-// are 588 of a block's 1,050 clocks, a wait of their warp 240 while some are queued), 24,576 of 128 to 256 21 us, 644,000 of 64 to 64 with SiLU 75 us (330 MB,
-// 4.4 TB/s: the epilogue's instructions), 192 of 128 to 128 8 us (one tile's chain).  Two tiles side by side with an issuing warp each instead: 90, 21.6,
+// are 588 of a block's 1,050 clocks, a wait of their warp 240 while some are queued), 24,576 of 128 to 256 21 us, 644,000 of 64 to 64 with SiLU 78 us (330 MB,
+// 4.2 TB/s: the epilogue's instructions), 192 of 128 to 128 8 us (one tile's chain).  Two tiles side by side with an issuing warp each instead: 90, 21.6,
 // 77 and 8.4 us, taken back; 16 warps of the epilogue spill at 72 registers.
 #pragma once
 #include "product.cuh"
@@ -224,6 +224,26 @@ __device__ __noinline__ void wild_row(const Args& p, int e, size_t row, int n, u
     }
     *reinterpret_cast<float*>(slab + at) = v;
   }
+}
+
+// Activations of 16 columns of this thread's row with a |z| beyond kNear: z lies where the slopes go.  Apart from the kernel, as it hardly ever happens.
+template <int ACT> __device__ __noinline__ void far_row(unsigned char* slab, unsigned char* slopes, int chunk, bool residual) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  for (int i = 0; i < 16; ++i) {
+    const int at = slab_at(lane, chunk + (i >> 2)) + (i & 3) * 4;
+    float d;
+    const float y = product::activate<ACT>(*reinterpret_cast<const float*>(slopes + at), d);
+    *reinterpret_cast<float*>(slopes + at) = d;
+    *reinterpret_cast<float*>(slab + at) = residual ? y + *reinterpret_cast<const float*>(slab + at) : y;
+  }
+}
+
+// the largest magnitude of three, NaN if one is
+__device__ __forceinline__ float largest(float a, float b, float c) {
+  float m;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+  return m;
 }
 
 // 16 values to `dst`, of which `count` are there
@@ -567,8 +587,6 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
               }
             }
             if (whole) {
-#pragma unroll
-              for (int i = 0; i < 16; i += 4) check += (v[i] + v[i + 1]) + (v[i + 2] + v[i + 3]);
               if (FORWARD) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -576,33 +594,48 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
                   v[4 * j] = fmaf(v[4 * j], wg::UNSCALE, b.x); v[4 * j + 1] = fmaf(v[4 * j + 1], wg::UNSCALE, b.y);
                   v[4 * j + 2] = fmaf(v[4 * j + 2], wg::UNSCALE, b.z); v[4 * j + 3] = fmaf(v[4 * j + 3], wg::UNSCALE, b.w);
                 }
-                if (ACT != product::kIdentity) {
-                  if (keep) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                      float d[4];
-#pragma unroll
-                      for (int i = 0; i < 4; ++i) v[4 * j + i] = product::activate<ACT>(v[4 * j + i], d[i]);
-                      *reinterpret_cast<float4*>(slopes + slab_at(lane, h * 4 + j)) = make_float4(d[0], d[1], d[2], d[3]);
-                    }
-                  } else {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                      float d;
-                      v[i] = product::activate<ACT>(v[i], d);
-                    }
-                  }
-                }
-                if (early) {
-#pragma unroll
-                  for (int j = 0; j < 4; ++j) {
-                    const float4 more = *reinterpret_cast<const float4*>(slab + slab_at(lane, h * 4 + j));
-                    v[4 * j] += more.x; v[4 * j + 1] += more.y; v[4 * j + 2] += more.z; v[4 * j + 3] += more.w;
-                  }
-                }
               } else {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) v[i] *= wg::UNSCALE;
+              }
+              float reach = 0.f;
+#pragma unroll
+              for (int i = 0; i < 16; i += 2) reach = largest(reach, v[i], v[i + 1]);
+              check = largest(check, reach, 0.f);
+              if ((ACT == product::kSilu || ACT == product::kSigmoid) && !(reach <= product::kNear)) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  *reinterpret_cast<float4*>(slopes + slab_at(lane, h * 4 + j)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                far_row<ACT>(slab, slopes, h * 4, early);
+                continue;
+              }
+              if (FORWARD && ACT != product::kIdentity) {
+                if (keep) {
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) {
+                    float2 d[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                      const float2 r = product::activate_near<ACT>(make_float2(v[4 * j + 2 * i], v[4 * j + 2 * i + 1]), d[i]);
+                      v[4 * j + 2 * i] = r.x; v[4 * j + 2 * i + 1] = r.y;
+                    }
+                    *reinterpret_cast<float4*>(slopes + slab_at(lane, h * 4 + j)) = make_float4(d[0].x, d[0].y, d[1].x, d[1].y);
+                  }
+                } else {
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) {
+                    float2 d;
+                    const float2 r = product::activate_near<ACT>(make_float2(v[2 * i], v[2 * i + 1]), d);
+                    v[2 * i] = r.x; v[2 * i + 1] = r.y;
+                  }
+                }
+              }
+              if (early) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  const float4 more = *reinterpret_cast<const float4*>(slab + slab_at(lane, h * 4 + j));
+                  v[4 * j] += more.x; v[4 * j + 1] += more.y; v[4 * j + 2] += more.z; v[4 * j + 3] += more.w;
+                }
               }
             }
 #pragma unroll
@@ -610,7 +643,7 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
               *reinterpret_cast<float4*>(slab + slab_at(lane, h * 4 + j)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
           }
           if (!whole) continue;
-          if (mine && !(fabsf(check) <= 3.402823466e38f)) wild_row<FORWARD, SLOPE, ACT>(p, w.e, row0 + lane, n0, slab, slopes);
+          if (mine && !(check <= 3.402823466e38f)) wild_row<FORWARD, SLOPE, ACT>(p, w.e, row0 + lane, n0, slab, slopes);
           fence_async_smem();
           __syncwarp();
           if (n0 < N && rows > 0) {
