@@ -476,6 +476,7 @@ extern "C" int fasteq_product_forward(const fasteq_product_problem* p, const voi
                                       const int32_t* offsets, void* y, void* slope, void* scratch, int64_t scratch_bytes, fasteq_stream_t stream) {
   if (const int rc = check(p, offsets)) return rc;
   if (p->rows == 0 || p->n == 0) return FASTEQ_OK;
+  if (p->act == kIdentity) slope = nullptr;
   const Scratch need = scratch_of(p, false);
   if (need.total() > 0 && !wide(0, {scratch})) return FASTEQ_INVALID;
   if (!y || (p->k > 0 && (!x || !w)) || (need.total() > 0 && (!scratch || scratch_bytes < need.total()))) return FASTEQ_INVALID;
