@@ -11,6 +11,14 @@ namespace {
 
 enum Act : int64_t { kIdentity = 0, kSilu = 1, kTanh = 2, kSigmoid = 3, kAbs = 4 };
 
+// Forward-mode differentiation is not offered.  Nodes refuse tangents by themselves; this is for where none is made, whatever the grad mode: no_grad does not
+// switch it off.
+void refuse_tangents(const char* name, std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    if (t && t->defined()) TORCH_CHECK(!t->_fw_grad(0).defined(), name, ": forward-mode differentiation is not supported");
+}
+const Tensor* pointer_of(const std::optional<Tensor>& t) { return t ? &*t : nullptr; }
+
 // x [rows, K], w [experts, N, K]; offsets undefined: one matrix
 fasteq_product_problem problem(const Tensor& x, const Tensor& w, int64_t inner, int64_t act) {
   fasteq_product_problem p{};
@@ -141,6 +149,7 @@ struct Layer : torch::autograd::Function<Layer> {
     // the context numbers the tensors it was given, not the places they could have had
     const bool has_b = b.defined(), has_r = ctx->saved_data["r"].toBool();
     const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = has_b && ctx->needs_input_grad(2);
+    refuse_tangents("dense layer", {&go[0]});
     Tensor gx, gw, gb;
     const Tensor gr = has_r && ctx->needs_input_grad(has_b ? 3 : 2) ? go[0] : Tensor();
     const Tensor g = rows(go[0], w.size(-2)), x2 = rows(x, w.size(-1)), w3 = matrix(w);
@@ -179,11 +188,11 @@ void check_operand(const char* name, const char* what, const std::optional<Tenso
   if (t) check_operand(name, what, *t, first);
 }
 
-// Whether a node is wanted of any of these (a dual tensor's node refuses it).  Without one a call is about 2 us of host time shorter.
+// Whether a node is wanted of any of these.  Without one a call is about 2 us of host time shorter.
 bool on_tape(std::initializer_list<const Tensor*> tensors) {
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : tensors)
-    if (t && t->defined() && (t->requires_grad() || t->_fw_grad(0).defined())) return true;
+    if (t && t->defined() && t->requires_grad()) return true;
   return false;
 }
 
@@ -195,9 +204,10 @@ void check_extent(const char* name, const char* what, int64_t v) {
 Tensor layer(const char* name, const Tensor& x, const Tensor& w, const std::optional<Tensor>& bias, const std::optional<Tensor>& residual, const std::optional<Tensor>& offsets,
              int64_t inner, int64_t act) {
   check_extent(name, "channels", std::max(w.size(-1), w.size(-2))); check_extent(name, "rows of an entry", inner);
-  if (!on_tape({&x, &w, bias ? &*bias : nullptr, residual ? &*residual : nullptr}))
+  refuse_tangents(name, {&x, &w, pointer_of(bias), pointer_of(residual)});
+  if (!on_tape({&x, &w, pointer_of(bias), pointer_of(residual)}))
     return Layer::run(x, w, bias.value_or(Tensor()), residual.value_or(Tensor()), offsets.value_or(Tensor()), inner, act, nullptr);
-  return Layer::apply(x, w, bias, residual, offsets, inner, act, on_tape({&x, &w, bias ? &*bias : nullptr}));
+  return Layer::apply(x, w, bias, residual, offsets, inner, act, on_tape({&x, &w, pointer_of(bias)}));
 }
 
 Tensor dense_act(const Tensor& x, const Tensor& w, const std::optional<Tensor>& bias, int64_t act, const std::optional<Tensor>& residual) {
@@ -311,6 +321,7 @@ struct Combine : torch::autograd::Function<Combine> {
     const bool need_weight = ctx->needs_input_grad(1);
     if (at::GradMode::is_enabled())
       return {need_rows ? Tensor(Spread::apply(weight, go[0], o)) : Tensor(), need_weight ? Tensor(Dots::apply(rows, go[0], o)) : Tensor(), Tensor()};
+    refuse_tangents("expert_combine", {&go[0]});
     auto d = run_combine_backward(rows, weight, go[0], *o, need_rows, need_weight);
     return {d[0], d[1], Tensor()};
   }
@@ -354,6 +365,7 @@ void check_rows(const char* name, const char* what, const Tensor& t, int64_t row
 Tensor expert_gather(const Tensor& x, const OrderPtr& o) {
   check_operand("expert_gather", "x", x, x);
   check_rows("expert_gather", "x", x, o->position.size(0), *o);
+  refuse_tangents("expert_gather", {&x});
   return on_tape({&x}) ? Tensor(Gather::apply(x, o)) : run_gather(x, *o);
 }
 
@@ -364,7 +376,8 @@ Tensor expert_combine(const Tensor& rows, const std::optional<Tensor>& weight, c
   std::optional<Tensor> w = weight;
   if (w && w->dim() == 1 && o->slots == 1) w = w->unsqueeze(1);
   TORCH_CHECK_VALUE(!w || w->sizes() == o->position.sizes(), name, ": weight must be ", o->position.sizes(), ", got ", weight->sizes());
-  return on_tape({&rows, w ? &*w : nullptr}) ? combine(rows, w, o) : run_combine(rows, w.value_or(Tensor()), *o);
+  refuse_tangents(name, {&rows, pointer_of(w)});
+  return on_tape({&rows, pointer_of(w)}) ? combine(rows, w, o) : run_combine(rows, w.value_or(Tensor()), *o);
 }
 
 Tensor expert_dense(const Tensor& rows, const Tensor& w, const OrderPtr& o, const std::optional<Tensor>& bias, int64_t act) {

@@ -38,3 +38,41 @@ def test_slopes_of_the_identity_are_not_touched(M, K, N, offset, dtype):
     assert lib.fasteq_product_forward(C.byref(p), _ptr(xd), _ptr(wd), _ptr(bd), None, None, _ptr(y), _ptr(slope), _ptr(scratch), need, _stream()) == 0
     single.check({"y": y}, single.reference(x, w, b, None, torch.zeros(M, N), None, single.U[dtype]))
     assert torch.all(slope == 77.0)
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_tangents_are_refused_whatever_the_grad_mode(grad):
+    """Forward-mode differentiation is not offered; no_grad does not switch it off, so a tangent is refused there too, of whichever operand."""
+    import torch.autograd.forward_ad as forward_ad
+    from fasteq_b200.ops.dense_act import dense_act
+    from fasteq_b200.ops.experts import expert_combine, expert_dense, expert_gather, expert_plan
+    z = lambda *s: torch.ones(*s, device="cuda")
+    plan = expert_plan(torch.tensor([[0, 1], [1, 0], [0, 0]], device="cuda"), 2)
+    calls = [(lambda x, w, b, r: dense_act(x, w, b, "silu", r), (z(3, 4), z(5, 4), z(5), z(3, 5))), (lambda x: expert_gather(x, plan), (z(3, 4),)),
+             (lambda rows, weight: expert_combine(rows, plan, weight), (z(6, 4), z(3, 2))),
+             (lambda rows, w, b: expert_dense(rows, w, plan, b, "tanh"), (z(6, 4), z(2, 5, 4), z(2, 5)))]
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        for f, args in calls:
+            for i in range(len(args)):
+                dual = [forward_ad.make_dual(t, torch.ones_like(t)) if i == j else t for j, t in enumerate(args)]
+                with pytest.raises(RuntimeError):
+                    f(*dual)
+            f(*args)
+
+
+def test_tangents_of_cotangents_are_refused():
+    """The gradients are linear in the cotangent: its tangent would have to come out as theirs."""
+    import torch.autograd.forward_ad as forward_ad
+    from fasteq_b200.ops.dense_act import dense_act
+    from fasteq_b200.ops.experts import expert_combine, expert_dense, expert_gather, expert_plan
+    leaf = lambda *s: torch.ones(*s, device="cuda", requires_grad=True)
+    plan = expert_plan(torch.tensor([[0, 1], [1, 0], [0, 0]], device="cuda"), 2)
+    x, rows, w, weight = leaf(3, 4), leaf(6, 4), leaf(2, 5, 4), leaf(3, 2)
+    outputs = [(dense_act(x, w[0], None, "silu"), x), (expert_gather(x, plan), x), (expert_combine(rows, plan, weight), weight), (expert_combine(rows, plan), rows),
+               (expert_dense(rows, w, plan), rows)]
+    with forward_ad.dual_level():
+        for y, to in outputs:
+            g = torch.ones_like(y)
+            with pytest.raises(RuntimeError):
+                torch.autograd.grad(y, to, forward_ad.make_dual(g, g.clone()), retain_graph=True)
+            torch.autograd.grad(y, to, g)
