@@ -172,25 +172,27 @@ __global__ void __launch_bounds__(PLAN_THREADS) expert_place_kernel(const I* exp
   place_entries<GROUPS>(keys, first, sm + (threadIdx.x >> 5) * K, position);
 }
 
+constexpr size_t count_smem(int K) { return (size_t)(PLAN_WARPS + 1) * K * 4; }
+constexpr size_t place_smem(int K) { return ((size_t)(PLAN_WARPS + 2) * K + 32) * 4; }
 int plan_ctas(long long n) { return (int)((n + groups_for(n) * PLAN_THREADS - 1) / (groups_for(n) * PLAN_THREADS)); }
 
 template <typename I, int GROUPS>
 int launch_plan(const void* expert, long long n, int X, int* position, int* offsets, void* scratch, cudaStream_t s) {
   const int K = X + 1, ctas = plan_ctas(n);
-  const size_t count_smem = (size_t)(PLAN_WARPS + 1) * K * 4, place_smem = ((size_t)(PLAN_WARPS + 2) * K + 32) * 4;
   cudaError_t e = cudaSuccess;
-  if (place_smem > 48 * 1024) {
-    e = cudaFuncSetAttribute(expert_count_kernel<I, GROUPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)count_smem);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(expert_place_kernel<I, GROUPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)place_smem);
+  if (place_smem(K) > 48 * 1024) {       // the same limit in every call: another thread may be between this and its launch
+    constexpr int MOST = FASTEQ_MAX_EXPERTS + 1;
+    e = cudaFuncSetAttribute(expert_count_kernel<I, GROUPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)count_smem(MOST));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(expert_place_kernel<I, GROUPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)place_smem(MOST));
     if (e != cudaSuccess) return cuda_fail(e);
   }
   const int* counts = nullptr;
   if (ctas > 1) {
-    e = launch_dependent(expert_count_kernel<I, GROUPS>, (unsigned)ctas, PLAN_THREADS, count_smem, s, (const I*)expert, n, X, (int*)scratch);
+    e = launch_dependent(expert_count_kernel<I, GROUPS>, (unsigned)ctas, PLAN_THREADS, count_smem(K), s, (const I*)expert, n, X, (int*)scratch);
     if (e != cudaSuccess) return cuda_fail(e);
     counts = (const int*)scratch;
   }
-  e = launch_dependent(expert_place_kernel<I, GROUPS>, (unsigned)(ctas > 1 ? ctas : 1), PLAN_THREADS, place_smem, s, (const I*)expert, n, X, counts, position, offsets);
+  e = launch_dependent(expert_place_kernel<I, GROUPS>, (unsigned)(ctas > 1 ? ctas : 1), PLAN_THREADS, place_smem(K), s, (const I*)expert, n, X, counts, position, offsets);
   return e == cudaSuccess ? FASTEQ_OK : cuda_fail(e);
 }
 template <typename I> int launch_plan(const void* expert, long long n, int X, int* position, int* offsets, void* scratch, cudaStream_t s) {

@@ -76,3 +76,36 @@ def test_tangents_of_cotangents_are_refused():
             with pytest.raises(RuntimeError):
                 torch.autograd.grad(y, to, forward_ad.make_dual(g, g.clone()), retain_graph=True)
             torch.autograd.grad(y, to, g)
+
+
+def test_plans_of_several_threads():
+    """Threads that plan for different numbers of experts through the C interface, which takes no lock of Python's: no call takes shared memory from another's launch."""
+    lib = cabi._core()
+    threads, bad = [], []
+    start = threading.Barrier(4)
+
+    def work(i):
+        experts, n = (1024, 400, 800, 600)[i], 200 + i
+        g = torch.Generator().manual_seed(i)
+        e = torch.randint(0, experts, (n,), generator=g, dtype=torch.int32)
+        position, offsets = experts_tests._order(e.view(-1, 1), experts)
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            ed, pd = e.cuda(), torch.empty(n, dtype=torch.int32, device="cuda")
+            od = torch.empty(experts + 1, dtype=torch.int32, device="cuda")
+        args = (_ptr(ed), C.c_int32(4), C.c_int64(n), C.c_int32(experts), _ptr(pd), _ptr(od), None, C.c_void_p(stream.cuda_stream))
+        start.wait()
+        for _ in range(3000):
+            rc = lib.fasteq_expert_plan(*args)
+            if rc != 0:
+                bad.append((experts, rc))
+        stream.synchronize()
+        if not (torch.equal(pd.cpu().long(), position.flatten()) and torch.equal(od.cpu().long(), offsets)):
+            bad.append((experts, "order"))
+    torch.cuda.synchronize()
+    for i in range(4):
+        threads.append(threading.Thread(target=work, args=(i,)))
+        threads[-1].start()
+    for t in threads:
+        t.join()
+    assert not bad, (len(bad), bad[:5])
