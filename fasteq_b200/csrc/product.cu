@@ -218,7 +218,7 @@ cudaError_t current_device(int* index, Device** device) {
   if (e != cudaSuccess) return e;
   if (*index >= MAX_DEVICES) return cudaErrorInvalidDevice;
   Device& d = devices[*index];
-  if (!d.known.load(std::memory_order_acquire)) {      // two threads that get here write the same
+  if (!d.known.load(std::memory_order_acquire)) {
     int sms = 0;
     int* status = nullptr;
     e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, *index);
@@ -226,9 +226,11 @@ cudaError_t current_device(int* index, Device** device) {
     if (e != cudaSuccess) return e;
     static std::mutex lock;
     std::lock_guard<std::mutex> g(lock);
-    d.sms = sms;
-    d.status = status;
-    d.known.store(true, std::memory_order_release);
+    if (!d.known.load(std::memory_order_relaxed)) {      // the first thread writes; others may be reading already
+      d.sms = sms;
+      d.status = status;
+      d.known.store(true, std::memory_order_release);
+    }
   }
   *device = &d;
   return cudaSuccess;

@@ -109,3 +109,30 @@ def test_plans_of_several_threads():
     for t in threads:
         t.join()
     assert not bad, (len(bad), bad[:5])
+
+
+def test_first_calls_of_several_threads():
+    """A fresh process whose first dense layers come from eight threads at once: what a call needs to know of the device is asked for once, and every result is right."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import threading, torch
+from fasteq_b200.ops.dense_act import dense_act
+x, w = torch.arange(64 * 48, device="cuda").remainder(7).float().view(64, 48), torch.arange(40 * 48, device="cuda").remainder(5).float().view(40, 48)
+torch.cuda.synchronize()
+out, start = [None] * 8, threading.Barrier(8)
+def work(i):
+    start.wait()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        out[i] = dense_act(x, w)
+        torch.cuda.current_stream().synchronize()
+threads = [threading.Thread(target=work, args=(i,)) for i in range(8)]
+[t.start() for t in threads]
+[t.join() for t in threads]
+want = x.cpu().double() @ w.cpu().double().t()
+assert all(o is not None and torch.equal(o.cpu().double(), want) for o in out)
+print("right")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=150, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0 and "right" in r.stdout, r.stderr[-2000:]
