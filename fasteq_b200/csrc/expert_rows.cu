@@ -221,18 +221,27 @@ template <typename T, int V> __device__ __forceinline__ void write_once(T* p, lo
   }
 }
 
+// An entry's row.  Positions are the caller's memory: one that is not among the rows is reported and becomes -1, which no kernel reads or writes at.
+__device__ __forceinline__ int row_of(const int* position, long long entry, long long entries) {
+  const int p = position[entry];
+  if (p >= 0 && p < entries) return p;
+  atomicExch(&g_expert_status, (int)kDevBadIndex);
+  return -1;
+}
+
 template <typename T, int V>
 __global__ void __launch_bounds__(256) expert_gather_kernel(const T* x, const int* position, const int* offsets, int X, long long tokens, int slots,
                                                             int packs, T* rows) {
   using P = Pack<T, V>;
   wait_for_previous_kernel();
   const int routed = offsets[X];
+  const long long entries = tokens * slots;
   for (long long t = (long long)blockIdx.x * blockDim.y + threadIdx.y; t < tokens; t += (long long)gridDim.x * blockDim.y) {
     for (int c = threadIdx.x; c < packs; c += blockDim.x) {
       const P v = read_once<T, V>(x, t * packs + c);
       for (int s = 0; s < slots; ++s) {
-        const int p = position[t * slots + s];
-        write_once<T, V>(rows, (long long)p * packs + c, p < routed ? v : P{});
+        const int p = row_of(position, t * slots + s, entries);
+        if (p >= 0) write_once<T, V>(rows, (long long)p * packs + c, p < routed ? v : P{});
       }
     }
   }
@@ -244,12 +253,13 @@ __global__ void __launch_bounds__(256) expert_combine_kernel(const T* rows, cons
   using P = Pack<T, V>;
   wait_for_previous_kernel();
   const int routed = offsets[X];
+  const long long entries = tokens * slots;
   for (long long t = (long long)blockIdx.x * blockDim.y + threadIdx.y; t < tokens; t += (long long)gridDim.x * blockDim.y) {
     for (int c = threadIdx.x; c < packs; c += blockDim.x) {
       P sum{};
       for (int s = 0; s < slots; ++s) {
-        const int p = position[t * slots + s];
-        if (p >= routed) continue;
+        const int p = row_of(position, t * slots + s, entries);
+        if (p < 0 || p >= routed) continue;
         const P v = read_once<T, V>(rows, (long long)p * packs + c);
         const T w = WEIGHTED ? weight[t * slots + s] : T(1);
 #pragma unroll
@@ -268,6 +278,7 @@ __global__ void __launch_bounds__(256) expert_combine_backward_kernel(const T* r
   using P = Pack<T, V>;
   wait_for_previous_kernel();
   const int routed = offsets[X];
+  const long long entries = tokens * slots;
   const long long step = (long long)gridDim.x * blockDim.y;
   // whole warps run the loop together, for the sums over their lanes
   const long long rounds = (tokens + step - 1) / step;
@@ -275,8 +286,8 @@ __global__ void __launch_bounds__(256) expert_combine_backward_kernel(const T* r
     const long long t = r * step + (long long)blockIdx.x * blockDim.y + threadIdx.y;
     const bool there = t < tokens;
     for (int s = 0; s < slots; ++s) {
-      const int p = there ? position[t * slots + s] : 0;
-      const bool live = there && p < routed;
+      const int p = there ? row_of(position, t * slots + s, entries) : -1;
+      const bool live = p >= 0 && p < routed;
       const T w = live && grows ? weight[t * slots + s] : T(0);
       T dot = T(0);
       if (there) {
@@ -293,7 +304,7 @@ __global__ void __launch_bounds__(256) expert_combine_backward_kernel(const T* r
 #pragma unroll
             for (int k = 0; k < V; ++k) o.v[k] = w * gv.v[k];
           }
-          if (grows) write_once<T, V>(grows, (long long)p * packs + c, o);
+          if (grows && p >= 0) write_once<T, V>(grows, (long long)p * packs + c, o);
         }
       }
       if (gweight) {

@@ -227,7 +227,13 @@ Tensor dense_act(const Tensor& x, const Tensor& w, const std::optional<Tensor>& 
 struct Order : torch::CustomClassHolder {
   Tensor position, offsets;              // [tokens, slots] and [experts + 1], int32
   int64_t experts, slots;
-  Order(Tensor p, Tensor o) : position(std::move(p)), offsets(std::move(o)), experts(offsets.size(0) - 1), slots(position.size(1)) {}
+  uint32_t versions[2];
+  Order(Tensor p, Tensor o)
+      : position(std::move(p)), offsets(std::move(o)), experts(offsets.size(0) - 1), slots(position.size(1)), versions{position._version(), offsets._version()} {}
+  // The kernels index with these, and a backward has to find them as its forward did; callers see them (as tensors of their own, which share the version).
+  void check(const char* name) const {
+    TORCH_CHECK(position._version() == versions[0] && offsets._version() == versions[1], name, ": the plan's position or offsets were changed in place since expert_plan made them");
+  }
 };
 using OrderPtr = c10::intrusive_ptr<Order>;
 
@@ -240,6 +246,7 @@ std::vector<int64_t> with_rows(const Tensor& t, int64_t rows) {
 }
 
 Tensor run_gather(const Tensor& x, const Order& o) {
+  o.check("expert_gather");
   c10::cuda::CUDAGuard guard(x.device());
   const Tensor xc = x.contiguous();
   Tensor rows = at::empty(with_rows(x, x.size(0) * o.slots), xc.options());
@@ -249,6 +256,7 @@ Tensor run_gather(const Tensor& x, const Order& o) {
   return rows;
 }
 Tensor run_combine(const Tensor& rows, const Tensor& weight, const Order& o) {
+  o.check("expert_combine");
   c10::cuda::CUDAGuard guard(rows.device());
   const Tensor rc = rows.contiguous(), wc = defined_contiguous(weight);
   const int64_t tokens = o.position.size(0);
@@ -259,6 +267,7 @@ Tensor run_combine(const Tensor& rows, const Tensor& weight, const Order& o) {
   return y;
 }
 variable_list run_combine_backward(const Tensor& rows, const Tensor& weight, const Tensor& g, const Order& o, bool need_rows, bool need_weight) {
+  o.check("expert_combine");
   c10::cuda::CUDAGuard guard(rows.device());
   const Tensor rc = rows.contiguous(), wc = defined_contiguous(weight), gc = g.contiguous();
   Tensor gr = need_rows ? at::empty_like(rc) : Tensor(), gw = need_weight ? at::empty(o.position.sizes(), rc.options()) : Tensor();
@@ -293,6 +302,7 @@ struct Dots : torch::autograd::Function<Dots> {
 // rows w[t, s] g[t], 0 for no expert
 struct Spread : torch::autograd::Function<Spread> {
   static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& g, const OrderPtr& o) {
+    o->check("expert_combine");
     ctx->save_for_backward({weight, g});
     ctx->saved_data["o"] = capsule(o);
     c10::cuda::CUDAGuard guard(g.device());
@@ -344,6 +354,7 @@ variable_list Spread::backward(AutogradContext* ctx, variable_list go) {
 // expert [tokens, slots], int32 or int64, contiguous
 OrderPtr make_order(const Tensor& expert, int64_t experts) {
   c10::cuda::CUDAGuard guard(expert.device());
+  c10::InferenceMode ordinary(false);    // tensors made in inference mode have no version
   const auto ints = expert.options().dtype(at::kInt);
   Tensor position = at::empty(expert.sizes(), ints), offsets = at::empty({experts + 1}, ints);
   int64_t need = 0;
@@ -382,6 +393,7 @@ Tensor expert_combine(const Tensor& rows, const std::optional<Tensor>& weight, c
 
 Tensor expert_dense(const Tensor& rows, const Tensor& w, const OrderPtr& o, const std::optional<Tensor>& bias, int64_t act) {
   const char* name = "expert_dense";
+  o->check(name);
   check_operand(name, "rows", rows, rows); check_operand(name, "weight", w, rows); check_operand(name, "bias", bias, rows);
   check_rows(name, "rows", rows, o->position.numel(), *o);
   TORCH_CHECK_VALUE(rows.dim() >= 2 && w.dim() == 3 && w.size(0) == o->experts && w.size(2) == rows.size(-1), name, ": rows [rows, ..., K] and weight [", o->experts,
@@ -406,8 +418,9 @@ OrderPtr expert_plan(const Tensor& expert, int64_t experts) {
 
 void bind_experts(py::module_& m) {
   py::class_<Order, OrderPtr>(m, "ExpertOrder")
-      .def_readonly("position", &Order::position)
-      .def_readonly("offsets", &Order::offsets);
+      .def_property_readonly("position", [](const Order& o) { return o.position.detach(); })
+      .def_property_readonly("offsets", [](const Order& o) { return o.offsets.detach(); })
+      .def_property_readonly("shape", [](const Order& o) { return std::make_tuple(o.position.size(0), o.slots, o.experts); });
   m.def("dense_act", &dense_act);
   m.def("expert_plan", &expert_plan);
   m.def("expert_gather", &expert_gather);

@@ -138,7 +138,8 @@ template <typename T> __device__ __forceinline__ T activate(int act, T z, T& slo
        : act == kAbs ? activate<kAbs>(z, slope) : activate<kIdentity>(z, slope);
 }
 
-// Rows of group e: [first(e), first(e + 1)); group `experts` holds those of no expert.
+// Rows of group e: [first(e), first(e + 1)); group `experts` holds those of no expert.  Offsets are the caller's memory: whatever they hold, the tiles and
+// chunks made of them stay within the rows.
 struct Groups {
   const int* offsets;                   // null: one group of all rows
   int experts, inner;
@@ -146,7 +147,8 @@ struct Groups {
   __device__ __forceinline__ long long first(int e) const {
     if (e > experts) return rows;
     if (!offsets) return e == 0 ? 0 : rows;
-    return (long long)offsets[e] * inner;
+    const long long row = (long long)offsets[e] * inner;
+    return row < 0 ? 0 : row > rows ? rows : row;
   }
 };
 
@@ -164,7 +166,7 @@ template <int SIZE> __device__ __forceinline__ int tile_of(const Groups& g, int 
   const long long begin = g.first(lo), end = g.first(lo + 1);
   *m0 = begin + (b - (begin / SIZE + lo)) * SIZE;
   const long long left = end - *m0;
-  *n_rows = left <= 0 ? 0 : left < SIZE ? (int)left : SIZE;
+  *n_rows = left <= 0 || *m0 < begin ? 0 : left < SIZE ? (int)left : SIZE;
   return lo;
 }
 
@@ -176,15 +178,15 @@ struct Chunk {
 __device__ __forceinline__ Chunk chunk_of(const Groups& g, int n_groups, int size, long long b) {
   const int lane = threadIdx.x & 31, step = (n_groups + 31) / 32;
   auto begins = [&](int e) { return e < n_groups && g.first(e) / size + e <= b; };
-  int e = (__popc(__ballot_sync(0xffffffffu, begins(lane * step))) - 1) * step;
-  if (step > 1) e += __popc(__ballot_sync(0xffffffffu, lane < step && begins(e + lane))) - 1;
+  int e = max(__popc(__ballot_sync(0xffffffffu, begins(lane * step))) - 1, 0) * step;
+  if (step > 1) e += max(__popc(__ballot_sync(0xffffffffu, lane < step && begins(e + lane))) - 1, 0);
   Chunk c;
   c.e = e;
   c.begin = g.first(e);
   const long long end = g.first(e + 1), left = end - c.begin - (b - (c.begin / size + e)) * size;
   c.count = (end - c.begin + size - 1) / size;
   c.m0 = end - left;
-  c.rows = left <= 0 ? 0 : left < size ? (int)left : size;
+  c.rows = left <= 0 || c.m0 < c.begin ? 0 : left < size ? (int)left : size;
   return c;
 }
 // Where a chunk's partial sums go, of chunks(rows, size): groups of several chunks have more than their share of 2 rows / size, so that

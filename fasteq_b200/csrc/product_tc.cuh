@@ -351,9 +351,10 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
   tc_fence_after();
   wait_for_previous_kernel();
   if (p.groups.offsets) {
-    for (int e = threadIdx.x; e < X; e += NT) tiles[e] = (int)((p.groups.first(e + 1) - p.groups.first(e) + BM - 1) / BM);
+    for (int e = threadIdx.x; e < X; e += NT) tiles[e] = (int)max((p.groups.first(e + 1) - p.groups.first(e) + BM - 1) / BM, 0LL);
     __syncthreads();
     if (warp == 0) {
+      const int most = (int)(p.groups.rows / BM) + X;       // of offsets that ascend
       int total = 0;
       for (int e0 = 0; e0 < X; e0 += 32) {
         const int v = e0 + lane < X ? tiles[e0 + lane] : 0;
@@ -363,8 +364,8 @@ __global__ void __launch_bounds__(NT, 1) product_tc_kernel(const __grid_constant
           const int u = __shfl_up_sync(0xffffffffu, sum, o);
           if (lane >= o) sum += u;
         }
-        if (e0 + lane < X) tiles[e0 + lane] = total + sum - v;
-        total += __shfl_sync(0xffffffffu, sum, 31);
+        if (e0 + lane < X) tiles[e0 + lane] = min(total + sum - v, most);
+        total = min(total + __shfl_sync(0xffffffffu, sum, 31), most);
       }
       if (lane == 0) tiles[X] = total;
     }

@@ -15,6 +15,7 @@ Float32 and float64, differentiable to every order.  CUDA tensors only.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import Optional
 
 import torch
@@ -27,17 +28,26 @@ __all__ = ["ExpertPlan", "expert_plan", "expert_gather", "expert_dense", "expert
 
 class ExpertPlan:
     """Order of the entries ``(token, slot)`` by expert.  ``position [tokens, slots]``: the entry's row; ``offsets [num_experts + 1]``: expert
-    ``e`` has rows ``offsets[e]`` to ``offsets[e + 1]``, those from ``offsets[-1]`` on have none (both int32, on the device)."""
+    ``e`` has rows ``offsets[e]`` to ``offsets[e + 1]``, those from ``offsets[-1]`` on have none (both int32, on the device; to be read: calls and
+    gradients refuse a plan whose tensors were changed in place)."""
 
     def __init__(self, native):
         self._native = native
-        self.position, self.offsets = native.position, native.offsets
-        self.tokens, self.slots = self.position.shape
-        self.rows, self.num_experts = self.tokens * self.slots, self.offsets.shape[0] - 1
+        self.tokens, self.slots, self.num_experts = native.shape
+        self.rows = self.tokens * self.slots
+
+    @functools.cached_property
+    def position(self) -> torch.Tensor:
+        return self._native.position
+
+    @functools.cached_property
+    def offsets(self) -> torch.Tensor:
+        return self._native.offsets
 
 
 def expert_device_status() -> int:
-    """Reads and clears the status word of the plans (synchronises): 0, or 2 = an expert number was not below ``num_experts``."""
+    """Reads and clears the status word of the plans (synchronises): 0, or 2 = an expert number was not below ``num_experts``, or a
+    position not among the rows."""
     lib, v = _cabi.core(), C.c_int32(0)
     _cabi.check(lib.fasteq_expert_device_status(C.byref(v)), lib, "fasteq_expert_device_status")
     return int(v.value)

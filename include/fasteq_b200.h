@@ -487,7 +487,8 @@ int fasteq_expert_combine(int32_t dtype, const void* rows, const void* weight /*
 int fasteq_expert_combine_backward(int32_t dtype, const void* rows, const void* weight, const void* grad_y, const int32_t* position,
                                    const int32_t* offsets, int32_t experts, int64_t tokens, int32_t slots, int32_t width,
                                    void* grad_rows /* or NULL */, void* grad_weight /* or NULL */, fasteq_stream_t stream);
-/* Reads and clears the status word of the expert order (synchronises): 0, or 2 = an expert number was out of range. */
+/* Reads and clears the status word of the expert order (synchronises): 0, or 2 = an expert number, or a position in the three calls above, was out of range.
+ * Rows at such positions are neither read nor written; offsets that are not a plan's give results without meaning, within the rows. */
 int fasteq_expert_device_status(int32_t* code /* host */);
 
 #ifdef __cplusplus

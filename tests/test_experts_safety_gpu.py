@@ -136,3 +136,129 @@ print("right")
 """
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=150, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
     assert r.returncode == 0 and "right" in r.stdout, r.stderr[-2000:]
+
+
+def test_a_plan_changed_in_place_is_refused():
+    """By every call, and by the gradients of calls made before the change; in inference mode too, and resized or exchanged storage as well."""
+    from fasteq_b200.ops.experts import expert_combine, expert_dense, expert_gather, expert_plan
+    e = torch.tensor([[0, 1], [1, 0], [2, -1]], device="cuda")
+    z = lambda *s: torch.randn(*s, device="cuda", requires_grad=True)
+    x, rows, w, weight = z(3, 4), z(6, 4), z(3, 5, 4), z(3, 2)
+    calls = [lambda p: expert_gather(x, p), lambda p: expert_combine(rows, p, weight), lambda p: expert_combine(rows, p), lambda p: expert_dense(rows, w, p, None, "silu")]
+    for change in (lambda p: p.position.add_(1), lambda p: p.offsets.zero_(), lambda p: p.position[0].fill_(2 ** 30)):
+        for inference in (False, True):
+            with torch.inference_mode(inference):
+                plan = expert_plan(e, 3)
+                before = [f(plan) for f in calls]
+                change(plan)
+                for f in calls:
+                    with pytest.raises(RuntimeError, match="changed in place"):
+                        f(plan)
+            for y, f in zip(before, calls) if not inference else ():
+                leaves = [t for t in (x, rows, w, weight) if any(n is t for n in _leaves(y))]
+                if f is calls[3] and torch.equal(plan.offsets.cpu(), torch.tensor([0, 2, 4, 5], dtype=torch.int32)):
+                    continue                                            # its gradients need the offsets alone
+                with pytest.raises(RuntimeError, match="changed in place|modified by an inplace operation"):
+                    torch.autograd.grad(y, leaves, torch.ones_like(y))
+    for change in (lambda p: p.position.set_(), lambda p: p.offsets.set_()):
+        plan = expert_plan(e, 3)
+        change(plan)
+        for f in calls:
+            with pytest.raises(RuntimeError, match="changed in place"):
+                f(plan)
+
+
+def _leaves(y):
+    out, todo = [], [y.grad_fn]
+    while todo:
+        for f, _ in todo.pop().next_functions:
+            if f is not None:
+                todo.append(f)
+                if hasattr(f, "variable"):
+                    out.append(f.variable)
+    return out
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+@pytest.mark.parametrize("width", [5, 64])
+def test_positions_out_of_range_are_reported_and_left_alone(width, dtype):
+    """Through the C interface, where positions are the caller's memory: nothing is read or written at them, the other entries are as ever."""
+    from fasteq_b200.ops.experts import expert_device_status
+    lib = cabi._core()
+    tokens, slots, experts = 50, 2, 4
+    e = experts_tests._experts(tokens, slots, experts, 0.1)
+    position, offsets = experts_tests._order(e, experts)
+    r = lambda *s: torch.randn(*s, generator=torch.Generator().manual_seed(width), dtype=torch.float64).to(dtype)
+    bad = {(3, 0): -1, (10, 1): tokens * slots, (20, 0): 2 ** 31 - 1, (21, 1): -2 ** 31, (49, 1): tokens * slots + 7}
+    wrong = position.clone()
+    for at, p in bad.items():
+        wrong[at] = p
+    x, rows, weight, g = r(tokens, width), r(tokens * slots, width), r(tokens, slots), r(tokens, width)
+    xd, rd, wd, gd, pd, od = (t.cuda() for t in (x, rows, weight, g, wrong.int(), offsets.int()))
+    nan = lambda *s: torch.full(s, float("nan"), dtype=dtype, device="cuda")
+    there, y, gr, gw = nan(tokens * slots, width), nan(tokens, width), nan(tokens * slots, width), nan(tokens, slots)
+    dt, sizes = C.c_int32(0 if dtype == torch.float32 else 1), (C.c_int32(experts), C.c_int64(tokens), C.c_int32(slots), C.c_int32(width))
+    assert expert_device_status() == 0
+    for call in (lambda: lib.fasteq_expert_gather(dt, _ptr(xd), _ptr(pd), _ptr(od), *sizes, _ptr(there), _stream()),
+                 lambda: lib.fasteq_expert_combine(dt, _ptr(rd), _ptr(wd), _ptr(pd), _ptr(od), *sizes, _ptr(y), _stream()),
+                 lambda: lib.fasteq_expert_combine_backward(dt, _ptr(rd), _ptr(wd), _ptr(gd), _ptr(pd), _ptr(od), *sizes, _ptr(gr), _ptr(gw), _stream())):
+        assert call() == 0
+        torch.cuda.synchronize()
+        assert expert_device_status() == 2 and expert_device_status() == 0
+    left_out = torch.zeros(tokens, slots, dtype=torch.bool)
+    for at in bad:
+        left_out[at] = True
+    live = ((e >= 0) & ~left_out).double()
+    untouched = position[left_out]
+    for t in (there, gr):
+        assert t[untouched.cuda()].isnan().all() and t.isnan().any(1).sum() == len(bad)
+    u, terms = single.U[dtype], (weight.double() * live)[:, :, None] * rows.double()[position]
+    assert torch.all((y.cpu().double() - terms.sum(1)).abs() <= 3 * u * terms.abs().sum(1))
+    prod = rows.double()[position] * g.double()[:, None] * live[:, :, None]
+    assert torch.all((gw.cpu().double() - prod.sum(2)).abs() <= (width + 8) * u * prod.abs().sum(2))
+    keep = (e >= 0) & ~left_out
+    assert torch.equal(there.cpu()[position[keep]], x[:, None].expand(-1, slots, -1)[keep])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+@pytest.mark.parametrize("shift", [0, 1])
+@pytest.mark.parametrize("offsets", [[0, 300, 2 ** 30, 2 ** 31 - 1], [-5, 300, 700, 700], [0, 700, 300, 700], [700, 300, 100, 0], [500, -2 ** 31, 900, 20]])
+def test_offsets_of_no_plan_stay_within_the_rows(offsets, shift, dtype):
+    """Through the C interface, where offsets are the caller's memory: nothing is written beside the results, and offsets beyond the rows end with them."""
+    lib = cabi._core()
+    X, M, K, N, pad = 3, 700, 40, 72, 64
+    r = lambda *s: torch.randn(*s, generator=torch.Generator().manual_seed(M), dtype=torch.float64).to(dtype)
+    x, w, b, g = r(M, K), r(X, N, K) / K ** 0.5, r(X, N), r(M, N)
+    p = cabi.Problem(dtype=0 if dtype == torch.float32 else 1, k=K, n=N, experts=X, inner=1, act=2, rows=M)
+    bases = []
+
+    def put(t):                          # between guards, `shift` values off alignment
+        base = torch.full((t.numel() + 2 * pad + 8,), 77.0, dtype=dtype, device="cuda")
+        v = base[pad + shift:pad + shift + t.numel()].view(t.shape)
+        v.copy_(t)
+        bases.append((base, v))
+        return v
+    xd, wd, bd, gd = (put(t) for t in (x, w, b, g))
+    y, gx, gw, gb = (put(torch.zeros_like(t)) for t in (g, x, w, b))
+    slope = torch.zeros(M + pad, N, dtype=dtype, device="cuda")
+    od = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+    scratch = []
+    for backward in (0, 1):
+        need = C.c_int64(0)
+        assert lib.fasteq_product_scratch(C.byref(p), C.c_int32(backward), C.byref(need)) == 0
+        scratch.append((torch.full((need.value + 256,), 77, dtype=torch.uint8, device="cuda"), need))
+    assert lib.fasteq_product_forward(C.byref(p), _ptr(xd), _ptr(wd), _ptr(bd), None, _ptr(od), _ptr(y), _ptr(slope), _ptr(scratch[0][0]), scratch[0][1], _stream()) == 0
+    assert lib.fasteq_product_backward(C.byref(p), _ptr(xd), _ptr(wd), _ptr(gd), _ptr(slope), _ptr(od), _ptr(gx), _ptr(gw), _ptr(gb), _ptr(scratch[1][0]), scratch[1][1],
+                                       _stream()) == 0
+    torch.cuda.synchronize()
+    for base, v in bases:
+        assert torch.all(base[:pad + shift] == 77.0) and torch.all(base[pad + shift + v.numel():] == 77.0)
+    for buffer, need in scratch:
+        assert torch.all(buffer[need.value:] == 77)
+    assert not slope[M:].any()
+    ends = [min(max(o, 0), M) for o in offsets]
+    if ends == sorted(ends) and ends[0] == 0:
+        want = experts_tests._dense_reference(x, w, b, ends, "tanh", g, single.U[dtype])
+        for n, v in (("y", y), ("x", gx), ("w", gw), ("b", gb)):
+            ref, tol = want[n]
+            assert torch.all((v.cpu().double() - ref).abs() <= tol), n
