@@ -194,7 +194,8 @@ extern "C" int fasteq_edge_geometry_backward(int32_t dtype, const void* pos, con
 extern "C" int fasteq_edge_geometry_device_status(int32_t* code) {
   if (!code) return FASTEQ_INVALID;
   int v = 0, zero = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(&v, g_geom_status, sizeof(int));
+  cudaError_t e = cudaDeviceSynchronize();      // the copy would not wait for streams that do not wait for the default one
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&v, g_geom_status, sizeof(int));
   if (e != cudaSuccess) return cuda_fail(e);
   e = cudaMemcpyToSymbol(g_geom_status, &zero, sizeof(int));
   if (e != cudaSuccess) return cuda_fail(e);

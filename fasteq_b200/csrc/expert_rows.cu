@@ -425,7 +425,8 @@ extern "C" int fasteq_expert_device_status(int32_t* code) {
   if (!code) return FASTEQ_INVALID;
   int v = 0;
   const int zero = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(&v, g_expert_status, sizeof(int));
+  cudaError_t e = cudaDeviceSynchronize();      // the copy would not wait for streams that do not wait for the default one
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&v, g_expert_status, sizeof(int));
   if (e == cudaSuccess && v != 0) e = cudaMemcpyToSymbol(g_expert_status, &zero, sizeof(int));
   if (e != cudaSuccess) return cuda_fail(e);
   *code = v;

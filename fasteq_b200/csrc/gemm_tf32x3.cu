@@ -1143,7 +1143,8 @@ cudaError_t status_word(int** word) { return cudaGetSymbolAddress((void**)word, 
 
 int device_status(int* code) {
   int v = 0, zero = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(&v, g_tc_status, sizeof(int));
+  cudaError_t e = cudaDeviceSynchronize();      // the copy would not wait for streams that do not wait for the default one
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&v, g_tc_status, sizeof(int));
   if (e != cudaSuccess) return cuda_fail(e);
   e = cudaMemcpyToSymbol(g_tc_status, &zero, sizeof(int));
   if (e != cudaSuccess) return cuda_fail(e);

@@ -399,7 +399,8 @@ __device__ int g_chain_status;
 
 int device_status(int* code) {
   int v = 0, zero = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(&v, g_chain_status, sizeof(int));
+  cudaError_t e = cudaDeviceSynchronize();      // the copy would not wait for streams that do not wait for the default one
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&v, g_chain_status, sizeof(int));
   if (e != cudaSuccess) return cuda_fail(e);
   e = cudaMemcpyToSymbol(g_chain_status, &zero, sizeof(int));
   if (e != cudaSuccess) return cuda_fail(e);

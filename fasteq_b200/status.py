@@ -3,7 +3,8 @@
 Every kernel with a bounded wait or an index check records why it gave up or what it skipped in a status word
 instead of trapping (wait timed out, index outside its operand); results of that launch are then not to be used.
 The words live per generated module (tensor product, symmetric contraction) and per family in the core library
-(tcgen05 GEMMs and the radial chain, edge geometry, experts).  Reading synchronises the device."""
+(tcgen05 GEMMs, dense layers and the radial chain, edge geometry, experts), one of each on every device.  Reading
+synchronises the current device, all its streams, and reads its words."""
 from __future__ import annotations
 
 from typing import Dict
@@ -16,6 +17,7 @@ def device_status() -> Dict[str, int]:
     out: Dict[str, int] = {}
     if not torch.cuda.is_available():
         return out
+    torch.cuda.synchronize()             # the modules' words are read by copies that would not wait for a side stream
     from .ops import uniform1d_jit as u1d
     from .ops import stc_uniform1d_jit as stc
     from .ops.dense import tensorcore_device_status

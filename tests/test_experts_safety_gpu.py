@@ -262,3 +262,18 @@ def test_offsets_of_no_plan_stay_within_the_rows(offsets, shift, dtype):
         for n, v in (("y", y), ("x", gx), ("w", gw), ("b", gb)):
             ref, tol = want[n]
             assert torch.all((v.cpu().double() - ref).abs() <= tol), n
+
+
+def test_status_words_wait_for_every_stream():
+    """A plan on a side stream, behind work that takes a while: its report is read, not overlooked, by either way of reading it."""
+    from fasteq_b200.ops.experts import expert_device_status, expert_plan
+    from fasteq_b200.status import device_status
+    side, e = torch.cuda.Stream(), torch.tensor([0, 7, 1], device="cuda")
+    torch.cuda.synchronize()
+    for read, want, nothing in ((expert_device_status, 2, 0), (device_status, {"experts": 2}, {})):
+        assert read() == nothing
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(200_000_000)
+            expert_plan(e, 3)
+        assert read() == want
+        assert read() == nothing
