@@ -197,13 +197,13 @@ bool on_tape(std::initializer_list<const Tensor*> tensors) {
 }
 
 // extents that the C interface takes as 32-bit numbers
-void check_extent(const char* name, const char* what, int64_t v) {
-  TORCH_CHECK_VALUE(v <= INT32_MAX, name, ": ", what, " must be below 2^31, got ", v);
+void check_extent(const char* name, const char* what, int64_t v, int64_t most = INT32_MAX) {
+  TORCH_CHECK_VALUE(v <= most, name, ": ", what, " must be ", most, " at most, got ", v);
 }
 
 Tensor layer(const char* name, const Tensor& x, const Tensor& w, const std::optional<Tensor>& bias, const std::optional<Tensor>& residual, const std::optional<Tensor>& offsets,
              int64_t inner, int64_t act) {
-  check_extent(name, "channels", std::max(w.size(-1), w.size(-2))); check_extent(name, "rows of an entry", inner);
+  check_extent(name, "channels", std::max(w.size(-1), w.size(-2)), FASTEQ_MAX_CHANNELS); check_extent(name, "rows of an entry", inner);
   refuse_tangents(name, {&x, &w, pointer_of(bias), pointer_of(residual)});
   if (!on_tape({&x, &w, pointer_of(bias), pointer_of(residual)}))
     return Layer::run(x, w, bias.value_or(Tensor()), residual.value_or(Tensor()), offsets.value_or(Tensor()), inner, act, nullptr);

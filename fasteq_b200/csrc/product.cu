@@ -25,6 +25,7 @@ using namespace fasteq::product;
 namespace {
 
 constexpr int TILE = 64, BK = 16, PITCH = TILE + 4, THREADS = 256;
+static_assert(FASTEQ_MAX_CHANNELS == TILE * 65535, "tiles of columns in a grid's second extent");
 
 // One tile of C = epilogue(A op(W)).  A [rows, K], times `slope` where it is given.  FORWARD: W [N, K], bias, act and residual;
 // else W [K, N] (grad_x: K the layer's outputs, N its inputs).
@@ -181,7 +182,7 @@ int check(const fasteq_product_problem* p, const int32_t* offsets) {
   if (!p || (p->dtype != FASTEQ_F32 && p->dtype != FASTEQ_F64) || p->k < 0 || p->n < 0 || p->rows < 0 || p->experts < 1 || p->inner < 1 ||
       p->act < 0 || p->act > 4 || (!offsets && p->experts != 1))
     return FASTEQ_INVALID;
-  if (p->experts > FASTEQ_MAX_EXPERTS || p->rows / p->inner > 0x7fff0000LL || p->rows / TILE > 0x7fff0000LL || p->n > TILE * 65535LL || p->k > TILE * 65535LL)
+  if (p->experts > FASTEQ_MAX_EXPERTS || p->rows / p->inner > 0x7fff0000LL || p->rows / TILE > 0x7fff0000LL || p->n > FASTEQ_MAX_CHANNELS || p->k > FASTEQ_MAX_CHANNELS)
     return FASTEQ_UNSUPPORTED;
   return FASTEQ_OK;
 }
@@ -246,8 +247,8 @@ template <auto KERNEL> cudaError_t allow_shared_memory(int device) {
 
 // CTAs of a launch over tiles of rows and columns
 bool in_32_bits(const fasteq_product_problem* p, int tile) {
-  const long long columns = (std::max(p->k, p->n) + tile - 1) / tile, rows = p->rows / tile + p->experts + 1;
-  return rows * columns <= 0x7fffffffLL && columns * columns * (p->rows / 64 + p->experts) <= 0x7fffffffLL;
+  const long long tiles_k = (p->k + tile - 1) / tile, tiles_n = (p->n + tile - 1) / tile, rows = p->rows / tile + p->experts + 1;
+  return rows * std::max(tiles_k, tiles_n) <= 0x7fffffffLL && tiles_k * tiles_n <= 0x7fffffffLL && tiles_k * tiles_n * (p->rows / 64 + p->experts) <= 0x7fffffffLL;
 }
 bool even(int extent, std::initializer_list<const void*> pointers) {
   uintptr_t all = 0;

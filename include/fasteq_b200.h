@@ -450,6 +450,7 @@ int fasteq_readout_backward(int32_t dtype, const void* g, const void* w, void* g
  * take FP32 multiply-adds).  The reference leaves such layers to the model package.
  * ------------------------------------------------------------------------- */
 #define FASTEQ_MAX_EXPERTS 1024
+#define FASTEQ_MAX_CHANNELS 4194240       /* k and n each; more are FASTEQ_UNSUPPORTED */
 typedef struct fasteq_product_problem {
   int32_t dtype;                /* fasteq_dtype */
   int32_t k, n;                 /* channels in and out */

@@ -277,3 +277,27 @@ def test_status_words_wait_for_every_stream():
             expert_plan(e, 3)
         assert read() == want
         assert read() == nothing
+
+
+def test_the_widest_layers_and_one_channel_more():
+    """4,194,240 channels are the most: with all gradients; one more is refused by name before anything runs."""
+    from fasteq_b200.ops.dense_act import dense_act
+    from fasteq_b200.ops.experts import expert_dense, expert_plan
+    most = 64 * 65535
+    one = torch.zeros(1, 1, device="cuda")
+    plan = expert_plan(torch.zeros(1, dtype=torch.int64, device="cuda"), 1)
+    for call in (lambda: dense_act(one, one.expand(most + 1, 1)), lambda: dense_act(one.expand(1, most + 1), one.expand(1, most + 1)),
+                 lambda: expert_dense(one, one.expand(1, most + 1, 1), plan)):
+        with pytest.raises(ValueError, match="channels"):
+            call()
+    for dtype, K in ((torch.float64, 65), (torch.float32, 9)):
+        x, w = torch.randint(-3, 4, (3, K), device="cuda").to(dtype), torch.randint(-3, 4, (most, K), device="cuda").to(dtype)
+        g = torch.randint(-3, 4, (3, most), device="cuda").to(dtype)
+        x.requires_grad_(True), w.requires_grad_(True)
+        y = dense_act(x, w)
+        gx, gw = torch.autograd.grad(y, (x, w), g)
+        xd, wd, gd = x.detach().double(), w.detach().double(), g.double()
+        assert torch.equal(y.detach().double(), xd @ wd.t()) and torch.equal(gw.double(), gd.t() @ xd)
+        assert torch.equal(gx.double(), gd @ wd) or dtype == torch.float32       # FP32 sums beyond 2^24 round
+        assert float((gx.double() - gd @ wd).abs().max()) <= (most + 8) * 2.0 ** -24 * float((gd.abs() @ wd.abs()).max())
+        del x, w, g, y, gx, gw, xd, wd, gd
