@@ -255,18 +255,28 @@ bool even(int extent, std::initializer_list<const void*> pointers) {
   for (const void* q : pointers) all |= reinterpret_cast<uintptr_t>(q);
   return extent % 2 == 0 && (all & 15u) == 0;
 }
+template <bool FORWARD, int TN>
+int launch_f64(const fasteq_product_problem* p, const void* A, const void* w, const void* bias, const void* residual, const int32_t* offsets, void* C, void* slope_out,
+               cudaStream_t s) {
+  const int K = FORWARD ? p->k : p->n, N = FORWARD ? p->n : p->k, tiles_n = (N + TN - 1) / TN;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = allow_shared_memory<pf64::product_f64_kernel<FORWARD, TN>>(dev);
+  if (e == cudaSuccess)
+    e = launch_dependent(pf64::product_f64_kernel<FORWARD, TN>, (unsigned)(tile_numbers<pf64::ROWS>(p->rows, p->experts + 1) * tiles_n), pf64::NT,
+                         pf64::Shape<pf64::ROWS, TN, true, FORWARD>::SMEM, s, groups_of(p, offsets), (const double*)A, (const double*)w, (const double*)bias,
+                         (const double*)residual, K, N, p->act, tiles_n, even(K, {A}), even(p->k, {w}), (double*)C, (double*)slope_out);
+  return e == cudaSuccess ? FASTEQ_OK : cuda_fail(e);
+}
 template <bool FORWARD>
 int product_f64(const fasteq_product_problem* p, const void* A, const void* w, const void* bias, const void* residual, const int32_t* offsets, void* C, void* slope_out,
                 cudaStream_t s) {
-  const int K = FORWARD ? p->k : p->n, N = FORWARD ? p->n : p->k, tiles_n = (N + pf64::TILE - 1) / pf64::TILE;
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = allow_shared_memory<pf64::product_f64_kernel<FORWARD>>(dev);
-  if (e == cudaSuccess)
-    e = launch_dependent(pf64::product_f64_kernel<FORWARD>, (unsigned)(tile_numbers<pf64::TILE>(p->rows, p->experts + 1) * tiles_n), pf64::NT, pf64::SMEM, s,
-                         groups_of(p, offsets), (const double*)A, (const double*)w, (const double*)bias, (const double*)residual, K, N, p->act, tiles_n, even(K, {A}),
-                         even(p->k, {w}), (double*)C, (double*)slope_out);
-  return e == cudaSuccess ? FASTEQ_OK : cuda_fail(e);
+  switch (pf64::tile_for(FORWARD ? p->n : p->k)) {
+    case 8: return launch_f64<FORWARD, 8>(p, A, w, bias, residual, offsets, C, slope_out, s);
+    case 16: return launch_f64<FORWARD, 16>(p, A, w, bias, residual, offsets, C, slope_out, s);
+    case 32: return launch_f64<FORWARD, 32>(p, A, w, bias, residual, offsets, C, slope_out, s);
+    default: return launch_f64<FORWARD, 64>(p, A, w, bias, residual, offsets, C, slope_out, s);
+  }
 }
 
 // Rows of a chunk: as many as give every SM `per_sm` tiles of rows x matrix, in one wave (24,576 rows of 128 x 256 in FP32: 148 CTAs 18.4 us, 196 CTAs
@@ -294,16 +304,21 @@ template <typename T> int reduce(const fasteq_product_problem* p, const Groups& 
   return e == cudaSuccess ? FASTEQ_OK : cuda_fail(e);
 }
 
-int wgrad_f64(const fasteq_product_problem* p, int size, const void* x, const void* g, const int32_t* offsets, void* gw, void* gb, void* scratch, cudaStream_t s) {
+template <int TM, int TN>
+int launch_wgrad_f64(const fasteq_product_problem* p, int size, const void* x, const void* g, const int32_t* offsets, void* gw, void* gb, void* scratch, cudaStream_t s) {
   const Groups groups = groups_of(p, offsets);
-  const int tiles_k = (p->k + pf64::TILE - 1) / pf64::TILE, tiles = tiles_k * ((p->n + pf64::TILE - 1) / pf64::TILE);
+  const int tiles_k = (p->k + TN - 1) / TN, tiles = tiles_k * ((p->n + TM - 1) / TM);
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = allow_shared_memory<pf64::product_wgrad_f64_kernel>(dev);
+  if (e == cudaSuccess) e = allow_shared_memory<pf64::product_wgrad_f64_kernel<TM, TN>>(dev);
   if (e == cudaSuccess)
-    e = launch_dependent(pf64::product_wgrad_f64_kernel, (unsigned)((p->rows / size + p->experts) * tiles), pf64::NT, pf64::SMEM, s, groups, (const double*)x,
-                         (const double*)g, p->k, p->n, size, tiles_k, tiles, even(p->k, {x}), even(p->n, {g}), (double*)gw, (double*)gb, (double*)scratch);
+    e = launch_dependent(pf64::product_wgrad_f64_kernel<TM, TN>, (unsigned)((p->rows / size + p->experts) * tiles), pf64::NT, pf64::Shape<TM, TN, false, false>::SMEM, s, groups,
+                         (const double*)x, (const double*)g, p->k, p->n, size, tiles_k, tiles, even(p->k, {x}), even(p->n, {g}), (double*)gw, (double*)gb, (double*)scratch);
   return e == cudaSuccess ? reduce<double>(p, groups, size, gw, gb, scratch, s) : cuda_fail(e);
+}
+int wgrad_f64(const fasteq_product_problem* p, int size, const void* x, const void* g, const int32_t* offsets, void* gw, void* gb, void* scratch, cudaStream_t s) {
+  if (p->n <= 16) return p->k <= 16 ? launch_wgrad_f64<16, 16>(p, size, x, g, offsets, gw, gb, scratch, s) : launch_wgrad_f64<16, 64>(p, size, x, g, offsets, gw, gb, scratch, s);
+  return p->k <= 16 ? launch_wgrad_f64<64, 16>(p, size, x, g, offsets, gw, gb, scratch, s) : launch_wgrad_f64<64, 64>(p, size, x, g, offsets, gw, gb, scratch, s);
 }
 
 template <typename T>
@@ -495,7 +510,7 @@ extern "C" int fasteq_product_forward(const fasteq_product_problem* p, const voi
     return run_tc<true>(p, x, (p->k + 3) & ~3, nullptr, w, bias, residual, offsets, y, slope, need.split ? at : nullptr, s);
   }
   if (p->dtype == FASTEQ_F32) return forward<float>(p, x, w, bias, residual, offsets, y, slope, s);
-  if (p->k == 0 || !in_32_bits(p, pf64::TILE)) return forward<double>(p, x, w, bias, residual, offsets, y, slope, s);
+  if (p->k == 0 || !in_32_bits(p, TILE)) return forward<double>(p, x, w, bias, residual, offsets, y, slope, s);
   return product_f64<true>(p, x, w, bias, residual, offsets, y, slope, s);
 }
 
@@ -540,7 +555,7 @@ extern "C" int fasteq_product_backward(const fasteq_product_problem* p, const vo
     return rc;
   }
   const int rows = chunk_rows(p, on_tensor_cores(p));      // as the scratch was counted with
-  if (p->dtype == FASTEQ_F64 && p->k > 0 && in_32_bits(p, pf64::TILE)) {
+  if (p->dtype == FASTEQ_F64 && p->k > 0 && in_32_bits(p, TILE)) {
     if (slope) {
       e = align_rows<double>(grad_y, slope, p->n, p->n, p->n, p->rows, g_at, s);
       if (e != cudaSuccess) return cuda_fail(e);

@@ -90,6 +90,34 @@ def test_whole_numbers(M, K, N, dtype):
         assert torch.equal(a.double(), e)
 
 
+@pytest.mark.parametrize("N", [1, 7, 8, 9, 16, 17, 31, 32, 33])
+@pytest.mark.parametrize("K", [1, 8, 15, 16, 17, 32, 100])
+def test_whole_numbers_of_few_channels(K, N):
+    """FP64 has narrow tiles for these, of 8, 16 and 32 columns; one matrix and several."""
+    from fasteq_b200.ops.dense_act import dense_act
+    from fasteq_b200.ops.experts import expert_dense, expert_plan
+    r, M, X = _whole(K + 50 * N, torch.float64), 777, 5
+    x, w, b, s, g = r(M, K), r(X, N, K), r(X, N), r(M, N), r(M, N)
+    leaves = [t.cuda().requires_grad_(True) for t in (x, w[0], b[0], s)]
+    y = dense_act(leaves[0], leaves[1], leaves[2], "abs", leaves[3])
+    z = x @ w[0].t() + b[0]
+    gz = g * z.sign()
+    for a, e in zip((y.detach().cpu(), *_grads(y, leaves, g)), (z.abs() + s, gz @ w[0], gz.t() @ x, gz.sum(0), g)):
+        assert torch.equal(a, e)
+    e = torch.arange(M) * 13 % (X + 1) - 1
+    plan = expert_plan(e.cuda(), X)
+    leaves = [t.cuda().requires_grad_(True) for t in (x, w, b)]
+    y = expert_dense(leaves[0], leaves[1], plan, leaves[2])
+    got = [y.detach().cpu(), *_grads(y, leaves, g)]
+    ends = plan.offsets.tolist()
+    want = [torch.zeros_like(t) for t in (g, x, w, b)]
+    for k in range(X):
+        rows = slice(ends[k], ends[k + 1])
+        want[0][rows], want[1][rows], want[2][k], want[3][k] = x[rows] @ w[k].t() + b[k], g[rows] @ w[k], g[rows].t() @ x[rows], g[rows].sum(0)
+    for a, c in zip(got, want):
+        assert torch.equal(a, c)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
 @pytest.mark.parametrize("tokens,slots,experts,K,N", [(40, 2, 5, 33, 7), (3000, 2, 8, 64, 128), (20_011, 1, 89, 64, 64), (900, 1, 600, 300, 12), (9000, 3, 2, 40, 72)])
 def test_whole_numbers_through_experts(tokens, slots, experts, K, N, dtype):
