@@ -124,7 +124,7 @@ template <int WN, int I, int J, typename F> __device__ __forceinline__ void each
 }
 
 // A thread's rows of a column of the turned tile, four at a time: their activations' chains and their residuals' loads run side by side (12,288 rows
-// of 256 to 256 channels with SiLU, residual and slope: 111 us one by one with branches, 80 us).
+// of 256 to 256 channels with SiLU, residual and slope: 111 us one by one with branches, 78 us).
 template <int ACT, int TN> __device__ __forceinline__ void finish_rows(const double* z, double b, const double* more, double* to, double* kept, int rows, int N) {
   constexpr int STEP = NT / TN, PITCH = TN + 2;
 #pragma unroll 1

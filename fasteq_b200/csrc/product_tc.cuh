@@ -26,7 +26,7 @@
 // raw ones of A and the slabs 227 KB of shared memory.  The six products' rate is the bf16 one / 6 (271 TFLOP/s of 1627), a K = 16 step takes 25 + 0.44
 // columns clocks an MMA, 294 for the five.  Measured: 100,000 rows of 256 to 256 channels 99 us (132 TFLOP/s of FP32-accurate products; the ten MMAs
 // are 588 of a block's 1,050 clocks, a wait of their warp 240 while some are queued), 24,576 of 128 to 256 21 us, 644,000 of 64 to 64 with SiLU 78 us (330 MB,
-// 4.2 TB/s: the epilogue's instructions), 192 of 128 to 128 8 us (one tile's chain).  Two tiles side by side with an issuing warp each instead: 90, 21.6,
+// 4.2 TB/s: the epilogue warps' latency, 4,300 clocks a tile, while the split warps idle), 192 of 128 to 128 8 us (one tile's chain).  Two tiles side by side with an issuing warp each instead: 90, 21.6,
 // 77 and 8.4 us, taken back; 16 warps of the epilogue spill at 72 registers.
 #pragma once
 #include "product.cuh"

@@ -9,7 +9,7 @@
 //   warps 4-11   split g into tensor memory, four warps the even and four the odd blocks, and add its columns for gb
 //   warps 12-15  split x into shared memory
 //   warps 16-23  every 256 rows of either add the accumulators to their registers; in the end write the tile's sums
-// Chunks are long enough to give each SM one tile (at least 256 rows); an expert of several chunks leaves partial sums, which a second kernel adds
+// Chunks are long enough to give each SM one tile, at least 64 rows, or 256 where experts have no more than that on average (chunk_rows); an expert of several chunks leaves partial sums, which a second kernel adds
 // in order.  Sums that are not finite are formed again in FP32, the whole tile.  Errors against 64 bits (2-norm, 1e-8; torch's FP32 products, this) at 60, 1,000,
 // 12,288 and 100,003 rows of 128 x 128: 14.0, 5.4; 25.8, 8.3; 63.1, 12.6; 112, 23.6; operands of one sign 11.9, 5.7; 9.8, 6.5; 17.2, 12.0; 19.9, 34.2.
 // Bound: the warps' instructions between the waits (the tensor cores are busy for 31 %, issue slots for 53 % of the time).  Measured, g without a slope:

@@ -2,7 +2,7 @@
 
     plan = expert_plan(expert, num_experts)                       # who goes where: [tokens, slots] expert numbers, -1: to none
     rows = expert_gather(x, plan)                                 # [tokens, ...] -> [tokens * slots, ...] in the experts' order
-    rows = expert_dense(rows, w1, plan, bias=b1, activation="silu")      # one launch for all experts, w1 [experts, N, K]
+    rows = expert_dense(rows, w1, plan, bias=b1, activation="silu")      # one product for all experts, w1 [experts, N, K]
     rows = expert_dense(rows, w2, plan, bias=b2)
     y = expert_combine(rows, plan, weight)                        # [tokens, ...] = sum over slots of weight * row
 
@@ -10,7 +10,7 @@ Everything stays on the device: the plan's offsets are read by the kernels, so t
 in a CUDA graph.  Sums run over slots and rows in a fixed order (no atomics): the same inputs give the same bits.  Entries given to no
 expert lie behind the experts' rows as zeros and take part in no sum and no gradient.  The weights are scalars of a row, so rows may hold
 components of irreps; ``expert_dense`` mixes channels, its rows' components ``[rows, components, K]`` share their expert's matrix.
-Float32 and float64, differentiable to every order.  CUDA tensors only.
+Float32 and float64, differentiable to every order (forward-mode differentiation is refused).  CUDA tensors only.
 """
 from __future__ import annotations
 

@@ -445,8 +445,9 @@ int fasteq_readout_backward(int32_t dtype, const void* g, const void* w, void* g
  * identity) receives act'(z) for the gradients, which take NULL where it is the identity: [rows, n], FP32 rows (n + 3) & ~3 values apart and 16-byte
  * aligned.  With gz = grad_y * slope
  *   grad_x = gz W[e],   grad_w[e] = sum_{r of e} gz[r]^T x[r],   grad_bias[e] = sum_{r of e} gz[r].
- * FP32 data: products of three bf16 parts per operand on the tensor cores, accumulated in FP32 (the accuracy of FP32 products); FP64: FP64
- * throughout.  Sums are formed in a fixed order.  Any extents, any 4- / 8-byte aligned addresses (FP32 ones that are not 16-byte aligned
+ * FP32 data: products of three bf16 parts per operand on the tensor cores, accumulated in FP32 with truncation (2-norm errors against 64 bits up to
+ * 2.3e-7, 3.9e-7 where no signs cancel; sums that FP32 holds exactly are exact); FP64: FP64 throughout.  Sums are formed in a fixed order.  Any
+ * extents up to the limits below, any 4- / 8-byte aligned addresses (FP32 ones that are not 16-byte aligned
  * take FP32 multiply-adds).  The reference leaves such layers to the model package.
  * ------------------------------------------------------------------------- */
 #define FASTEQ_MAX_EXPERTS 1024
